@@ -1,3 +1,4 @@
 from .manager import CacheGroup, PagedCache, group_requests, host
+from .tables import StepTables, step_tables
 
-__all__ = ["CacheGroup", "PagedCache", "group_requests", "host"]
+__all__ = ["CacheGroup", "PagedCache", "StepTables", "group_requests", "host", "step_tables"]

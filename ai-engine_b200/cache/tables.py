@@ -1,0 +1,64 @@
+"""A step's pages, block tables and cache slots, made on the device from the requests' lengths.
+
+The host's bookkeeping (`PagedCache`) knows every length when it packs a step.  A program that verifies drafted tokens does not: how
+many tokens a request kept is known on the device alone until somebody waits for it.  `step_tables` makes from device lengths what
+a step needs, without a word from the host."""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from ..kernels.loader import KernelError, check
+from ..kernels.ops import int_rows, launcher, on_current_device
+from ..kernels.profile import region
+
+MAX_REQUESTS = 4096      # of one call: a block keeps 16 bytes of each
+
+
+class StepTables(NamedTuple):
+    """What `step_tables` makes; all int32, in one buffer."""
+    tables: torch.Tensor        # [R, W] page ids: what a request held, what it took, -1
+    held: torch.Tensor          # [R] pages of each request
+    free_count: torch.Tensor    # [1] pages left in the free list
+    q_start: torch.Tensor       # [R] first token of each request
+    q_len: torch.Tensor         # [R] tokens that go ahead: counts, or 0 for a request that has to wait
+    positions: torch.Tensor     # [max_tokens] place of each token in its request; -1 behind the last token
+    token_req: torch.Tensor     # [max_tokens] row of its request; -1 behind the last token
+    slots: torch.Tensor         # [max_tokens] page * page_size + place in the page; -1 where nothing is to be written
+
+
+def step_tables(cached: torch.Tensor, counts: torch.Tensor, held: torch.Tensor, tables: torch.Tensor, free_pages: torch.Tensor,
+                free_count: torch.Tensor, page_size: int, num_pages: int, max_tokens: int, err: torch.Tensor) -> StepTables:
+    """Request r holds cached[r] tokens in the first held[r] pages of tables[r] and brings counts[r] more; free_pages[:free_count] are
+    free.  In the order of the requests, each takes the pages it is short of from the end of the free list; one that cannot have
+    all of them has to wait (it takes none, its tokens' slots are -1, its q_len is 0), and so has every later one that is
+    short of pages.  Pages held beyond the tokens (drafts that were refused) are used first.  Nothing that is given is changed: the
+    next step passes the outputs on.  Sizes: R up to MAX_REQUESTS; max_tokens bounds the sum of the counts.
+
+    A request whose lengths are negative, do not fit the table's width or bring tokens past max_tokens waits and sets the error
+    word; a page outside the pool sets it too and makes no slot."""
+    if tables.dim() != 2 or tables.shape[1] == 0:
+        raise KernelError("step_tables: the tables must be [requests, pages]")
+    R, W = tables.shape
+    if not 0 < R <= MAX_REQUESTS:
+        raise KernelError(f"step_tables: {R} requests (1 to {MAX_REQUESTS} are taken)")
+    F = free_pages.numel()
+    int_rows("step_tables", cached=(cached, (R,)), counts=(counts, (R,)), held=(held, (R,)), tables=(tables, (R, W)),
+             free_pages=(free_pages, (F,)), free_count=(free_count, (1,)), err=(err, (1,)))
+    if page_size < 1 or num_pages < 0 or num_pages * page_size > 0x7fffffff:
+        raise KernelError(f"step_tables: {num_pages} pages of {page_size} tokens (1 to 2^31 - 1 cache slots are taken)")
+    if not 0 <= max_tokens <= 1 << 30 or R * W > 1 << 30:
+        raise KernelError("step_tables: sizes beyond 2^30")
+    stream = on_current_device("step_tables", cached, counts, held, tables, free_pages, free_count, err)
+    out = torch.empty(R * W + 3 * R + 1 + 3 * max_tokens, dtype=torch.int32, device=tables.device)
+    made, now, left, q_start, q_len, positions, token_req, slots = out.split((R * W, R, 1, R, R, max_tokens, max_tokens, max_tokens))
+    p = out.data_ptr()
+    at = p + 4 * R * W
+    behind = at + 4 * (3 * R + 1)
+    fn = launcher("step_tables.cu", "aie_step_tables", "ppppppiiiiiippppppppp" + "p")
+    with region("step_tables", 4 * (2 * R * W + 6 * R + 3 * max_tokens)):
+        check(fn(cached.data_ptr(), counts.data_ptr(), held.data_ptr(), tables.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), R,
+                 W, F, page_size, num_pages, max_tokens, p, at, at + 4 * R, at + 4 * (R + 1), at + 4 * (2 * R + 1), behind,
+                 behind + 4 * max_tokens, behind + 8 * max_tokens, err.data_ptr(), stream), "step_tables")
+    return StepTables(made.view(R, W), now, left, q_start, q_len, positions, token_req, slots)

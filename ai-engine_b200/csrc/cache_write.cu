@@ -1,0 +1,104 @@
+// Keys and values of a step's tokens written to their cache slots: row t of k and v goes to page slots[t] / P, place
+// slots[t] % P of a layer's pool [pages][kv heads][P][d].  Rows may be columns of a fused projection (any distance between
+// tokens and between heads) and are rounded once where the cache holds fewer bits.  A negative slot leaves its row out.
+//
+// What bounds it: memory.  A thread moves units of eight consecutive elements of one head (16 bytes of bfloat16), four of them under
+// way, the loads of its rows asked for before the slots are known.
+#include "common.cuh"
+
+#define CW_THREADS 256
+#define CW_UNITS 4      // units of a thread under way
+
+template <typename T, int V> struct CwVec { T e[V]; };
+
+// V consecutive elements: 16-byte accesses when V is 8, single ones when it is 1
+template <typename T, int V> __device__ __forceinline__ void cw_load(CwVec<T, V>& v, const T* p) {
+    if constexpr (V == 8) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(v.e)[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+    } else {
+        v.e[0] = *p;
+    }
+}
+
+template <typename I, typename C, int V>
+__global__ void __launch_bounds__(CW_THREADS)
+write_kv_slots_kernel(const I* __restrict__ k, const I* __restrict__ v, long long k_token, long long k_head, long long v_token,
+                      long long v_head, C* __restrict__ k_pages, C* __restrict__ v_pages, const int* __restrict__ slots,
+                      long long total, int per_head, int per_plane, int per_token, int P, int K, int d, int n_slots, unsigned* err) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const long long first = (long long)blockIdx.x * (CW_THREADS * CW_UNITS) + threadIdx.x;
+    alignas(16) CwVec<I, V> x[CW_UNITS];
+    int slot[CW_UNITS], unit[CW_UNITS];
+#pragma unroll
+    for (int u = 0; u < CW_UNITS; ++u) {
+        const long long i = first + u * CW_THREADS;
+        slot[u] = -1;
+        unit[u] = 0;
+        if (i < total) {
+            const long long t = i / per_token;
+            unit[u] = (int)(i - t * per_token);
+            const bool is_v = unit[u] >= per_plane;
+            const int w = is_v ? unit[u] - per_plane : unit[u];
+            const int h = w / per_head, e = (w - h * per_head) * V;
+            cw_load<I, V>(x[u], is_v ? v + t * v_token + h * v_head + e : k + t * k_token + h * k_head + e);
+            slot[u] = slots[t];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < CW_UNITS; ++u) {
+        if (slot[u] < 0) continue;
+        if (slot[u] >= n_slots) { atomicOr(err, AIE_DEV_PAGE_OOB); continue; }
+        const bool is_v = unit[u] >= per_plane;
+        const int w = is_v ? unit[u] - per_plane : unit[u];
+        const int h = w / per_head, e = (w - h * per_head) * V;
+        const int page = slot[u] / P;
+        C* to = (is_v ? v_pages : k_pages) + (((size_t)page * K + h) * P + (slot[u] - page * P)) * d + e;
+        if constexpr (V == 8) {
+            alignas(16) CwVec<C, V> y;
+#pragma unroll
+            for (int j = 0; j < V; ++j) y.e[j] = from_f32<C>(to_f32<I>(x[u].e[j]));
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(C) / 2; ++j) reinterpret_cast<uint4*>(to)[j] = reinterpret_cast<const uint4*>(y.e)[j];
+        } else {
+            *to = from_f32<C>(to_f32<I>(x[u].e[0]));
+        }
+    }
+}
+
+template <typename I, typename C, int V>
+static int launch_write(const void* k, const void* v, long long kt, long long kh, long long vt, long long vh, void* kp, void* vp,
+                        const int* slots, int T, int num_pages, int P, int K, int d, unsigned* err, cudaStream_t st) {
+    const long long total = (long long)T * 2 * K * (d / V);
+    const long long blocks = (total + CW_THREADS * CW_UNITS - 1) / (CW_THREADS * CW_UNITS);
+    if (blocks > 0x7fffffff) return -3;
+    return (int)launch_pdl(write_kv_slots_kernel<I, C, V>, dim3((unsigned)blocks), dim3(CW_THREADS), 0, st, (const I*)k, (const I*)v, kt, kh,
+                           vt, vh, (C*)kp, (C*)vp, slots, total, d / V, K * (d / V), 2 * K * (d / V), P, K, d, num_pages * P, err);
+}
+
+template <typename I, typename C>
+static int launch_write_rows(bool wide, const void* k, const void* v, long long kt, long long kh, long long vt, long long vh, void* kp,
+                             void* vp, const int* slots, int T, int num_pages, int P, int K, int d, unsigned* err, cudaStream_t st) {
+    return wide ? launch_write<I, C, 8>(k, v, kt, kh, vt, vh, kp, vp, slots, T, num_pages, P, K, d, err, st)
+                : launch_write<I, C, 1>(k, v, kt, kh, vt, vh, kp, vp, slots, T, num_pages, P, K, d, err, st);
+}
+
+// k, v [T, K, d] with elements k_token / k_head (v_token / v_head) apart between tokens and heads, 1 apart within a head.
+// num_pages * P and 2 * K * d fit 31 bits.
+extern "C" int aie_write_kv_slots(const void* k, const void* v, int row_dtype, long long k_token, long long k_head, long long v_token,
+                                  long long v_head, void* k_pages, void* v_pages, int cache_dtype, const int* slots, int T, int num_pages,
+                                  int P, int K, int d, unsigned* err, cudaStream_t stream) {
+    if (T <= 0) return 0;
+    if (P <= 0 || K <= 0 || d <= 0 || num_pages < 0) return AIE_BAD_ARG;
+    const long long step = row_dtype == AIE_BF16 ? 8 : 4;      // elements in 16 bytes
+    const bool wide = d % 8 == 0 && (k_token | k_head | v_token | v_head) % step == 0 &&
+                      ((size_t)k | (size_t)v | (size_t)k_pages | (size_t)v_pages) % 16 == 0;
+#define CW_ARGS wide, k, v, k_token, k_head, v_token, v_head, k_pages, v_pages, slots, T, num_pages, P, K, d, err, stream
+    if (row_dtype == AIE_BF16 && cache_dtype == AIE_BF16) return launch_write_rows<bf16, bf16>(CW_ARGS);
+    if (row_dtype == AIE_F32 && cache_dtype == AIE_BF16) return launch_write_rows<float, bf16>(CW_ARGS);
+    if (row_dtype == AIE_F32 && cache_dtype == AIE_F32) return launch_write_rows<float, float>(CW_ARGS);
+    if (row_dtype == AIE_BF16 && cache_dtype == AIE_F32) return launch_write_rows<bf16, float>(CW_ARGS);
+    return AIE_BAD_ARG;
+#undef CW_ARGS
+}

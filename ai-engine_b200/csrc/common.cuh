@@ -20,6 +20,7 @@
 #define AIE_DEV_PAGE_OOB 2u     // block table entry outside the pool
 #define AIE_DEV_WAIT_TIMEOUT 4u // a bounded wait ran out
 #define AIE_DEV_SLOT_OOB 8u     // request row / slot outside its table
+#define AIE_DEV_NO_MASS 16u     // a row of probabilities that is all zero
 
 typedef __nv_bfloat16 bf16;
 

@@ -1,0 +1,246 @@
+// Verification of drafted tokens against the target's probabilities, from given random numbers.
+//
+// Request r drafted n = draft_len[r] tokens x_0 .. x_(n-1) out of distributions q_0 .. q_(n-1) (null: each was certain of its
+// token); rows q_start[r] .. q_start[r] + n of `target` are the target's distributions p_0 .. p_n at the same places.  Draft i is
+// kept while u_i q_i(x_i) < p_i(x_i), u_i in [0, 1) (the product of two floats is exact in 64 bits, so nothing is rounded here).
+// Behind the k kept ones one token is drawn, by v in [0, 1), from the weights
+//     w = max(p_k - q_k, 0)   where draft k was refused,        w = p_n   where all were kept:
+// the first token whose cumulative weight is above floor(v W), W the sum of all.  If every w is 0 (p_k nowhere above q_k: possible only
+// by the rounding of their sums) the weights are p_k.  Which tokens come out then follows the target's distribution exactly.
+// Weights are integers, w clipped to 1 in units of 2^-48 rounded to nearest: 2^-49 is off at most, a float below 2^-25 of
+// the largest mass, and sums are exact, the same whatever their order.
+//
+// What bounds it: one row of p and one of q a request.  A cluster of eight blocks shares a request's row: every warp adds up
+// segments of 512 tokens (eight 16-byte loads a lane under way), the segments' sums stay in shared memory, the blocks' sums meet
+// through the cluster's, and the block that holds the wanted one looks for its segment and reads that once more.  Eight
+// blocks because a row of 128,256 floats twice is 128 KB for each, about 2 us of what an SM can load.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+
+namespace cg = cooperative_groups;
+typedef unsigned long long u64;
+
+#define VD_THREADS 512
+#define VD_CLUSTER 8
+#define VD_SEGMENT 512          // tokens a warp adds up at a time: four of 16 bytes a lane, of each row
+#define VD_MAX_SEGMENTS 256     // a block's: 1,048,576 tokens of vocabulary
+
+// in units of 2^-48; NaN and what is negative weigh nothing
+__device__ __forceinline__ u64 vd_fixed(float w) { return w > 0.f ? __float2ull_rn(fminf(w, 1.f) * 281474976710656.f) : 0ull; }
+
+__device__ __forceinline__ u64 vd_warp_sum(u64 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// what is taken off p: nothing, the draft's row, or everything at one token
+struct VdMinus {
+    const float* row;
+    int token;
+};
+
+// weights of the four tokens t .. t + 3; tokens from `V` on weigh nothing
+template <bool VEC> __device__ __forceinline__ void vd_load(float (&x)[4], const float* row, int t, int V) {
+    if (VEC && t + 4 <= V) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(row + t));
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = t + k < V ? __ldg(row + t + k) : 0.f;
+    }
+}
+// the weights of a warp's segment: lane l has tokens 128 j + 4 l .. + 3 of it
+template <bool VEC> __device__ __forceinline__ void vd_segment(u64 (&w)[4][4], const float* p, const VdMinus& m, int t0, int V, int lane) {
+    float a[4][4], b[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vd_load<VEC>(a[j], p, t0 + 128 * j + 4 * lane, V);
+    if (m.row)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vd_load<VEC>(b[j], m.row, t0 + 128 * j + 4 * lane, V);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float x = m.row ? a[j][k] - b[j][k] : a[j][k];
+            w[j][k] = t0 + 128 * j + 4 * lane + k == m.token ? 0ull : vd_fixed(x);
+        }
+}
+
+template <bool VEC>
+__global__ void __cluster_dims__(VD_CLUSTER, 1, 1) __launch_bounds__(VD_THREADS)
+verify_drafts_kernel(const float* __restrict__ target, long long target_row, int T, int V, const int* __restrict__ q_start,
+                     const int* __restrict__ draft_tokens, const int* __restrict__ draft_len, const float* __restrict__ draft_probs,
+                     long long draft_req, long long draft_place, int N, const float* __restrict__ accept_draws,
+                     const float* __restrict__ token_draws, int* __restrict__ tokens, int* __restrict__ emitted, unsigned* err) {
+    __shared__ u64 seg_sum[VD_MAX_SEGMENTS];
+    __shared__ u64 warp_sum[VD_THREADS / 32];
+    __shared__ u64 block_sum[2];            // of w, of p alone
+    __shared__ int s_kept;
+    cg::cluster_group cluster = cg::this_cluster();
+    pdl_launch_dependents();
+    pdl_wait();
+    const int r = blockIdx.x / VD_CLUSTER, rank = blockIdx.x % VD_CLUSTER;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int start = q_start[r];
+    int n = draft_len ? draft_len[r] : N;
+    int* out = tokens + (size_t)r * (N + 1);
+    const bool bad = n > N || (n >= 0 && (start < 0 || start > T - 1 - n));
+    if (n < 0 || bad) {                     // an idle request, or rows that are not there: the same in all blocks of the cluster
+        if (rank == 0) {
+            for (int i = tid; i <= N; i += VD_THREADS) out[i] = -1;
+            if (tid == 0) {
+                emitted[r] = 0;
+                if (bad) atomicOr(err, AIE_DEV_SLOT_OOB);
+            }
+        }
+        return;
+    }
+
+    // how many drafts are kept: a warp looks at 32 places at a time
+    if (warp == 0) {
+        int kept = n;
+        for (int base = 0; base < n; base += 32) {
+            const int i = base + lane;
+            bool refused = false;
+            if (i < n) {
+                const int x = draft_tokens[(size_t)r * N + i];
+                refused = true;
+                if (x >= 0 && x < V) {
+                    const float p = target[(start + i) * target_row + x];
+                    const float q = draft_probs ? draft_probs[r * draft_req + i * draft_place + x] : 1.f;
+                    refused = !((double)accept_draws[(size_t)r * N + i] * (double)q < (double)p);
+                } else if (rank == 0) {
+                    atomicOr(err, AIE_DEV_TOKEN_OOB);
+                }
+            }
+            const unsigned any = __ballot_sync(0xffffffffu, refused);
+            if (any) { kept = base + __ffs(any) - 1; break; }
+        }
+        if (lane == 0) s_kept = kept;
+    }
+    __syncthreads();
+    const int kept = s_kept;
+    const float* p = target + (start + kept) * target_row;
+    VdMinus minus = {nullptr, -1};
+    if (kept < n) {
+        if (draft_probs) minus.row = draft_probs + r * draft_req + kept * draft_place;
+        else minus.token = draft_tokens[(size_t)r * N + kept];
+    }
+
+    const int segments = (V + VD_SEGMENT - 1) / VD_SEGMENT, per = (segments + VD_CLUSTER - 1) / VD_CLUSTER;
+    const int s0 = rank * per, mine = max(0, min(per, segments - s0));
+    u64 before = 0, total = 0;
+    int round = 0;
+    for (;; ++round) {      // a second round only where something was taken off p and nothing is left: p by itself
+        u64 sum = 0;
+        for (int s = warp; s < mine; s += VD_THREADS / 32) {
+            u64 w[4][4], a = 0;
+            vd_segment<VEC>(w, p, minus, (s0 + s) * VD_SEGMENT, V, lane);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a += (w[j][0] + w[j][1]) + (w[j][2] + w[j][3]);
+            a = vd_warp_sum(a);
+            if (lane == 0) seg_sum[s] = a;
+            sum += a;
+        }
+        if (lane == 0) warp_sum[warp] = sum;
+        __syncthreads();
+        if (tid == 0) {
+            u64 a = 0;
+            for (int w = 0; w < VD_THREADS / 32; ++w) a += warp_sum[w];
+            block_sum[round] = a;
+        }
+        cluster.sync();
+        before = total = 0;
+        for (int b = 0; b < VD_CLUSTER; ++b) {
+            const u64 a = *cluster.map_shared_rank(&block_sum[round], b);
+            if (b < rank) before += a;
+            total += a;
+        }
+        if (total > 0 || round == 1 || kept == n) break;      // the same in all blocks
+        minus.row = nullptr;
+        minus.token = -1;
+    }
+
+    if (rank == 0) {
+        for (int i = tid; i <= N; i += VD_THREADS)
+            if (i != kept) out[i] = i < kept ? draft_tokens[(size_t)r * N + i] : -1;
+        if (tid == 0) {
+            emitted[r] = kept + 1;
+            if (total == 0) {                      // a row of zeros: no token can be drawn from it
+                out[kept] = 0;
+                atomicOr(err, AIE_DEV_NO_MASS);
+            }
+        }
+    }
+    if (total > 0) {
+        // total is below 2^53 for anything that sums to about 1, so the product is rounded once
+        const double v = (double)token_draws[r];
+        u64 goal = v > 0.0 ? (u64)(v * (double)total) : 0ull;
+        if (goal > total - 1) goal = total - 1;
+        const u64 here = block_sum[round];
+        if (warp == 0 && goal >= before && goal - before < here) {
+            goal -= before;
+            int s = 0;                             // the segment: 32 sums at a time
+            for (int base = 0; base < mine; base += 32) {
+                u64 a = base + lane < mine ? seg_sum[base + lane] : 0ull;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const u64 b = __shfl_up_sync(0xffffffffu, a, o);
+                    if (lane >= o) a += b;
+                }
+                const unsigned above = __ballot_sync(0xffffffffu, a > goal);
+                if (above) {
+                    const int at = __ffs(above) - 1;
+                    const u64 prev = __shfl_sync(0xffffffffu, a, at > 0 ? at - 1 : 0);
+                    if (at > 0) goal -= prev;
+                    s = base + at;
+                    break;
+                }
+                goal -= __shfl_sync(0xffffffffu, a, 31);
+            }
+            u64 w[4][4];
+            const int t0 = (s0 + s) * VD_SEGMENT;
+            vd_segment<VEC>(w, p, minus, t0, V, lane);
+            bool found = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                u64 a = (w[j][0] + w[j][1]) + (w[j][2] + w[j][3]);
+                const u64 own = a;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const u64 b = __shfl_up_sync(0xffffffffu, a, o);
+                    if (lane >= o) a += b;
+                }
+                const unsigned above = __ballot_sync(0xffffffffu, a > goal);
+                if (!found && above) {
+                    found = true;
+                    if (lane == __ffs(above) - 1) {
+                        u64 c = a - own;
+                        int k = 0;
+                        while (k < 3 && c + w[j][k] <= goal) c += w[j][k++];
+                        out[kept] = t0 + 128 * j + 4 * lane + k;
+                    }
+                }
+                if (!found) goal -= __shfl_sync(0xffffffffu, a, 31);
+            }
+        }
+    }
+    cluster.sync();      // a block's sums are read by the others until here
+}
+
+// target: rows of V floats, `target_row` apart; draft_probs (or null): row i of request r at r * draft_req + i * draft_place;
+// draft_tokens, accept_draws [R, N]; draft_len [R] or null (N each); tokens [R, N + 1], emitted [R].
+extern "C" int aie_verify_drafts(const float* target, long long target_row, int T, int V, const int* q_start, const int* draft_tokens,
+                                 const int* draft_len, const float* draft_probs, long long draft_req, long long draft_place, int R, int N,
+                                 const float* accept_draws, const float* token_draws, int* tokens, int* emitted, unsigned* err,
+                                 cudaStream_t stream) {
+    if (R <= 0) return 0;
+    if (V <= 0 || N < 0 || T < 0) return AIE_BAD_ARG;
+    if (V > VD_CLUSTER * VD_MAX_SEGMENTS * VD_SEGMENT || R > 0x7fffffff / VD_CLUSTER) return -3;
+    const bool vec = ((size_t)target | (size_t)draft_probs) % 16 == 0 && (target_row | draft_req | draft_place) % 4 == 0;
+    return (int)launch_pdl(vec ? verify_drafts_kernel<true> : verify_drafts_kernel<false>, dim3(R * VD_CLUSTER), dim3(VD_THREADS), 0, stream,
+                           target, target_row, T, V, q_start, draft_tokens, draft_len, draft_probs, draft_req, draft_place, N, accept_draws,
+                           token_draws, tokens, emitted, err);
+}

@@ -37,7 +37,8 @@ class StepError(RuntimeError):
 
 
 _ERR_BITS = {1: "a token id outside the vocabulary", 2: "a block table entry outside the page pool",
-             4: "a bounded wait in a kernel ran out", 8: "a request row outside its table"}
+             4: "a bounded wait in a kernel ran out", 8: "a request row outside its table",
+             16: "a row of probabilities without mass"}
 
 
 class _Staging:

@@ -6,7 +6,7 @@ from __future__ import annotations
 
 import math
 import os
-from ctypes import c_float, c_int, c_longlong, c_void_p
+from ctypes import byref, c_float, c_int, c_longlong, c_void_p
 from typing import Optional
 
 import numpy as np
@@ -713,6 +713,131 @@ def paged_attention(q, k_pages, v_pages, ctx, work, block_table, scale: float, w
         if not took:
             paged_attention_prefill(q, k_pages, v_pages, work.prefill_tiles, ctx.q_start, ctx.q_len,
                                     ctx.ctx_len, block_table, scale, window, ctx.err, out, cost=pre_cost)
+    return out
+
+
+# ---------------------------------------------------------------------------
+# steps whose lengths the device alone knows (drafted tokens and their verification)
+_LAUNCHERS = {}
+
+
+def launcher(source: str, name: str, signature: str):
+    """The launcher `name` of csrc/<source> with its argument types set, so that plain Python numbers can be passed:
+    p a pointer, i an int, l a long long, f a float."""
+    fn = _LAUNCHERS.get(name)
+    if fn is None:
+        fn = getattr(library(source), name)
+        fn.argtypes = [{"p": c_void_p, "i": c_int, "l": c_longlong, "f": c_float}[c] for c in signature]
+        _LAUNCHERS[name] = fn
+    return fn
+
+
+def on_current_device(what: str, *ts) -> int:
+    """The current device's stream as a number, for operands (None: left out) that all live on that device; any others are refused."""
+    require_cuda()
+    dev = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            raise KernelError(f"{what}: operands must live on the current CUDA device (cuda:{dev})")
+    return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+
+
+def int_rows(what: str, **ts) -> None:
+    """Refuses index arrays (name=(tensor, shape)) that are not contiguous int32 of their shape."""
+    for name, (t, shape) in ts.items():
+        if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+            raise KernelError(f"{what}: {name} must be a contiguous int32 tensor {list(shape)}, got {t.dtype} {list(t.shape)}")
+
+
+def _pools(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor):
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
+        raise KernelError(f"{what}: keys and values must be pools of one shape and dtype, [pages, kv heads, page, d]")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise KernelError(f"{what}: the pools must be contiguous")
+    dtype_code(k_pages)
+    N, K, P, d = k_pages.shape
+    if not (K and P and d) or N * P > 0x7fffffff:
+        raise KernelError(f"{what}: the pools' sizes {list(k_pages.shape)} are not taken (up to 2^31 - 1 cache slots, nothing empty)")
+    return N, K, P, d
+
+
+def write_kv_slots(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor,
+                   err: torch.Tensor) -> None:
+    """k_pages[slots[t] // P, :, slots[t] % P] = k[t], and the same for v: a step's keys and values into a layer's pools
+    [pages, K, P, d], at the slots that `cache.step_tables` made.  k, v: [T, K, d] float32 or bfloat16, each with any distance between
+    tokens and between heads (columns of a fused projection); rounded once where the pool holds fewer bits.  A negative slot
+    leaves its row out; one past the pool is left out and sets the error word.  Slots that are named must differ."""
+    N, K, P, d = _pools("write_kv_slots", k_pages, v_pages)
+    T = k.shape[0]
+    if k.shape != (T, K, d) or v.shape != k.shape or v.dtype != k.dtype:
+        raise KernelError(f"write_kv_slots: keys {list(k.shape)} and values {list(v.shape)} must be [T, {K}, {d}], of one dtype")
+    code = dtype_code(k)
+    if T and d > 1 and (k.stride(2) != 1 or v.stride(2) != 1):
+        raise KernelError("write_kv_slots: the elements of a head must be contiguous")
+    if 2 * K * d > 0x7fffffff:
+        raise KernelError("write_kv_slots: a token's rows are too long")
+    int_rows("write_kv_slots", slots=(slots, (T,)), err=(err, (1,)))
+    stream = on_current_device("write_kv_slots", k, v, k_pages, v_pages, slots, err)
+    if T == 0:
+        return
+    fn = launcher("cache_write.cu", "aie_write_kv_slots", "ppillllppipiiiiipp")
+    with region("write_kv_slots", 2 * T * K * d * (k.element_size() + k_pages.element_size())):
+        check(fn(k.data_ptr(), v.data_ptr(), code, k.stride(0), k.stride(1), v.stride(0), v.stride(1), k_pages.data_ptr(),
+                 v_pages.data_ptr(), dtype_code(k_pages), slots.data_ptr(), T, N, P, K, d, err.data_ptr(), stream), "write_kv_slots")
+
+
+def paged_attention_chunks(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor,
+                           ctx_len: torch.Tensor, block_table: torch.Tensor, scale: float, window: int, err: torch.Tensor,
+                           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of every request's new tokens over its pages, with the lengths on the device alone: request r (of R) brings
+    q_len[r] tokens, rows q_start[r] .. of q, behind the ctx_len[r] that its pages hold already (its new keys and values are in
+    the pages too).  softmax(q.k * scale over keys j <= position, and j > position - window where window > 0) . v per token and head,
+    query head h with key head h // (H / K).  q [T, H, d] in the pools' dtype, any distance between tokens and heads (multiples of 16
+    bytes); block_table [R, W]; out [T, H, d] contiguous: rows that no request names are left as they are (in an `out` made
+    here they hold nothing).  Few tokens behind many keys are what it is made for: the keys are shared out over the whole machine.
+    Any head size up to 256 that is a multiple of 8.  Lengths that do not fit q or the table bring nothing and set the error word, so
+    does a page outside the pool, whose keys count as zeros.  How a token's sums are ordered depends on the whole batch's lengths; a
+    non-finite key or value reaches all of its request's tokens in the step."""
+    N, K, P, d = _pools("paged_attention_chunks", k_pages, v_pages)
+    if q.dim() != 3 or q.shape[2] != d or q.shape[1] == 0 or q.shape[1] % K or q.dtype != k_pages.dtype:
+        raise KernelError(f"paged_attention_chunks: queries {q.dtype} {list(q.shape)} must be [T, a multiple of {K}, {d}] in {k_pages.dtype}")
+    T, H, _ = q.shape
+    if d % 8 or d > 256:
+        raise KernelError(f"paged_attention_chunks: head size {d} must be a multiple of 8, at most 256")
+    if T * H > 0x7fffffff or N == 0:
+        raise KernelError("paged_attention_chunks: too many rows of queries, or no pages")
+    if block_table.dim() != 2 or block_table.shape[1] == 0:
+        raise KernelError("paged_attention_chunks: the block table must be [requests, pages]")
+    R, W = block_table.shape
+    int_rows("paged_attention_chunks", q_start=(q_start, (R,)), q_len=(q_len, (R,)), ctx_len=(ctx_len, (R,)),
+             block_table=(block_table, (R, W)), err=(err, (1,)))
+    if W * P > 0x7fffffff - 1024:
+        raise KernelError("paged_attention_chunks: the table names more than 2^31 keys a request")
+    if not 0 <= window <= 0x7fffffff:
+        raise KernelError("paged_attention_chunks: a window is 0 (none) or a number of keys")
+    per = 16 // q.element_size()
+    if T and (q.stride(2) != 1 or q.stride(0) % per or q.stride(1) % per or q.data_ptr() % 16):
+        raise KernelError("paged_attention_chunks: every head's row of q must be contiguous and start on 16 bytes")
+    if k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16:
+        raise KernelError("paged_attention_chunks: the pools must start on 16 bytes")
+    if out is None:
+        out = torch.empty((T, H, d), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16:
+        raise KernelError("paged_attention_chunks: out must be contiguous, of q's shape and dtype, and start on 16 bytes")
+    stream = on_current_device("paged_attention_chunks", q, k_pages, v_pages, q_start, q_len, ctx_len, block_table, err, out)
+    if T == 0 or R == 0:
+        return out
+    rows = c_int()
+    blocks = launcher("attention_chunks_f32.cu", "aie_attention_chunks_f32_blocks", "ip")(d, byref(rows))
+    wide = 64 if d <= 64 else 128 if d <= 128 else 256
+    parts = 2 * blocks * rows.value
+    scratch = torch.empty(parts * (wide + 2) + 4 * blocks, dtype=torch.float32, device=q.device)
+    at = scratch.data_ptr()
+    fn = launcher("attention_chunks_f32.cu", "aie_attention_chunks_f32", "pllpppippppiiiiiiiiifppppp")
+    with region("attention_chunks", 2 * _nb(q)):
+        check(fn(q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), dtype_code(q),
+                 q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), block_table.data_ptr(), R, W, T, N, P, H, K, d, window, scale,
+                 at, at + 4 * parts * wide, at + 4 * parts * (wide + 2), err.data_ptr(), stream), "paged_attention_chunks")
     return out
 
 
