@@ -9,8 +9,8 @@ from typing import NamedTuple
 
 import torch
 
-from ..kernels.loader import KernelError, check
-from ..kernels.ops import int_rows, launcher, on_current_device
+from ..kernels.loader import KernelError
+from ..kernels.ops import Launcher, check_operands
 from ..kernels.profile import region
 
 MAX_REQUESTS = 4096      # of one call: a block keeps 16 bytes of each
@@ -44,21 +44,19 @@ def step_tables(cached: torch.Tensor, counts: torch.Tensor, held: torch.Tensor, 
     if not 0 < R <= MAX_REQUESTS:
         raise KernelError(f"step_tables: {R} requests (1 to {MAX_REQUESTS} are taken)")
     F = free_pages.numel()
-    int_rows("step_tables", cached=(cached, (R,)), counts=(counts, (R,)), held=(held, (R,)), tables=(tables, (R, W)),
-             free_pages=(free_pages, (F,)), free_count=(free_count, (1,)), err=(err, (1,)))
     if page_size < 1 or num_pages < 0 or num_pages * page_size > 0x7fffffff:
         raise KernelError(f"step_tables: {num_pages} pages of {page_size} tokens (1 to 2^31 - 1 cache slots are taken)")
     if not 0 <= max_tokens <= 1 << 30 or R * W > 1 << 30:
         raise KernelError("step_tables: sizes beyond 2^30")
-    stream = on_current_device("step_tables", cached, counts, held, tables, free_pages, free_count, err)
+    each = (R,)
+    stream = check_operands("step_tables", (("cached", cached, each), ("counts", counts, each), ("held", held, each), ("tables", tables, (R, W)),
+                                            ("free_pages", free_pages, (F,)), ("free_count", free_count, (1,)), ("err", err, (1,))))
     out = torch.empty(R * W + 3 * R + 1 + 3 * max_tokens, dtype=torch.int32, device=tables.device)
-    made, now, left, q_start, q_len, positions, token_req, slots = out.split((R * W, R, 1, R, R, max_tokens, max_tokens, max_tokens))
-    p = out.data_ptr()
-    at = p + 4 * R * W
-    behind = at + 4 * (3 * R + 1)
-    fn = launcher("step_tables.cu", "aie_step_tables", "ppppppiiiiiippppppppp" + "p")
     with region("step_tables", 4 * (2 * R * W + 6 * R + 3 * max_tokens)):
-        check(fn(cached.data_ptr(), counts.data_ptr(), held.data_ptr(), tables.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), R,
-                 W, F, page_size, num_pages, max_tokens, p, at, at + 4 * R, at + 4 * (R + 1), at + 4 * (2 * R + 1), behind,
-                 behind + 4 * max_tokens, behind + 8 * max_tokens, err.data_ptr(), stream), "step_tables")
-    return StepTables(made.view(R, W), now, left, q_start, q_len, positions, token_req, slots)
+        _TABLES((cached.data_ptr(), counts.data_ptr(), held.data_ptr(), tables.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
+                 out.data_ptr(), err.data_ptr(), R, W, F, page_size, num_pages, max_tokens), stream)
+    made, *rest = out.split_with_sizes((R * W, R, 1, R, R, max_tokens, max_tokens, max_tokens))
+    return StepTables(made.view(R, W), *rest)
+
+
+_TABLES = Launcher("step_tables.cu", "aie_step_tables", "8P6i")

@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(CfShape<D>::NW * 32) chunk_f32_kernel(const Ch
     if (bad) atomicOr(a.err, bad);
 }
 
-template <typename T, int D> static int launch_chunk_f32(ChArgs a, int C, cudaStream_t st) {
+template <typename T, int D> static int launch_chunk_f32(const ChArgs& a, int C, cudaStream_t st) {
     using S = CfShape<D>;
     auto kern = chunk_f32_kernel<T, D>;
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes);
@@ -279,26 +279,18 @@ template <typename T, int D> static int launch_chunk_f32(ChArgs a, int C, cudaSt
     return (int)launch_pdl(chunk_join_kernel<T, S::M, D>, dim3(C, S::M * D / 4 / 256), dim3(256), 0, st, a);
 }
 
-// Blocks of the kernel, and through `rows` the rows of an item: the scratch is [2 * blocks * rows * (D + 2)] floats and [blocks] int4, D the
-// head size rounded up to 64, 128 or 256.
-extern "C" int aie_attention_chunks_f32_blocks(int d, int* rows) {
-    if (d <= 0 || d > 256 || d % 8) return AIE_UNSUPPORTED;
-    *rows = d > 128 ? CfShape<256>::M : CfShape<128>::M;
-    return aie_sm_count() * (d <= 64 ? 2 : 1);
-}
+// Rows of an item, and blocks of the kernel.  The scratch is [2 * blocks * rows * (D + 2)] floats and [blocks] int4, D the head size
+// rounded up to 64, 128 or 256.
+extern "C" int aie_attention_chunks_f32_rows(int d) { return d > 128 ? CfShape<256>::M : CfShape<128>::M; }
+extern "C" int aie_attention_chunks_f32_blocks(int d) { return aie_sm_count() * (d <= 64 ? 2 : 1); }
 
-extern "C" int aie_attention_chunks_f32(const void* q, long long q_token, long long q_head, const void* k_pages, const void* v_pages,
-                                        void* out, int dtype, const int* q_start, const int* q_len, const int* ctx_len, const int* table,
-                                        int R, int W, int T, int num_pages, int P, int H, int K, int d, int window, float scale,
-                                        float* part_o, float* part_ml, void* meta, unsigned* err, cudaStream_t stream) {
-    int rows = 0;
-    const int C = aie_attention_chunks_f32_blocks(d, &rows);
-    if (C < 0) return C;
-    if (R <= 0 || T <= 0) return 0;
-    if (W <= 0 || num_pages <= 0 || P <= 0 || K <= 0 || H % K) return AIE_BAD_ARG;
-    ChArgs a = {q, k_pages, v_pages, out, q_start, q_len, ctx_len, table, part_o, part_ml, (int4*)meta, q_token, q_head,
-                R, W, T, num_pages, P, H, K, H / K, d, window, scale * 1.4426950408889634f, err};
-    if (dtype == AIE_F32) return d <= 64 ? launch_chunk_f32<float, 64>(a, C, stream) : d <= 128 ? launch_chunk_f32<float, 128>(a, C, stream) : launch_chunk_f32<float, 256>(a, C, stream);
-    if (dtype == AIE_BF16) return d <= 64 ? launch_chunk_f32<bf16, 64>(a, C, stream) : d <= 128 ? launch_chunk_f32<bf16, 128>(a, C, stream) : launch_chunk_f32<bf16, 256>(a, C, stream);
+extern "C" int aie_attention_chunks_f32(const ChArgs* args, int dtype, cudaStream_t stream) {
+    const ChArgs& a = *args;
+    if (a.R <= 0 || a.T <= 0) return 0;
+    if (a.d <= 0 || a.d > 256 || a.d % 8) return AIE_UNSUPPORTED;
+    if (a.W <= 0 || a.num_pages <= 0 || a.P <= 0 || a.K <= 0 || a.H % a.K) return AIE_BAD_ARG;
+    const int C = aie_attention_chunks_f32_blocks(a.d), w = a.d <= 64 ? 0 : a.d <= 128 ? 1 : 2;
+    if (dtype == AIE_F32) return w == 0 ? launch_chunk_f32<float, 64>(a, C, stream) : w == 1 ? launch_chunk_f32<float, 128>(a, C, stream) : launch_chunk_f32<float, 256>(a, C, stream);
+    if (dtype == AIE_BF16) return w == 0 ? launch_chunk_f32<bf16, 64>(a, C, stream) : w == 1 ? launch_chunk_f32<bf16, 128>(a, C, stream) : launch_chunk_f32<bf16, 256>(a, C, stream);
     return AIE_BAD_ARG;
 }

@@ -84,21 +84,27 @@ static int launch_write_rows(bool wide, const void* k, const void* v, long long 
                 : launch_write<I, C, 1>(k, v, kt, kh, vt, vh, kp, vp, slots, T, num_pages, P, K, d, err, st);
 }
 
-// k, v [T, K, d] with elements k_token / k_head (v_token / v_head) apart between tokens and heads, 1 apart within a head.
-// num_pages * P and 2 * K * d fit 31 bits.
-extern "C" int aie_write_kv_slots(const void* k, const void* v, int row_dtype, long long k_token, long long k_head, long long v_token,
-                                  long long v_head, void* k_pages, void* v_pages, int cache_dtype, const int* slots, int T, int num_pages,
-                                  int P, int K, int d, unsigned* err, cudaStream_t stream) {
-    if (T <= 0) return 0;
-    if (P <= 0 || K <= 0 || d <= 0 || num_pages < 0) return AIE_BAD_ARG;
-    const long long step = row_dtype == AIE_BF16 ? 8 : 4;      // elements in 16 bytes
-    const bool wide = d % 8 == 0 && (k_token | k_head | v_token | v_head) % step == 0 &&
-                      ((size_t)k | (size_t)v | (size_t)k_pages | (size_t)v_pages) % 16 == 0;
-#define CW_ARGS wide, k, v, k_token, k_head, v_token, v_head, k_pages, v_pages, slots, T, num_pages, P, K, d, err, stream
-    if (row_dtype == AIE_BF16 && cache_dtype == AIE_BF16) return launch_write_rows<bf16, bf16>(CW_ARGS);
-    if (row_dtype == AIE_F32 && cache_dtype == AIE_BF16) return launch_write_rows<float, bf16>(CW_ARGS);
-    if (row_dtype == AIE_F32 && cache_dtype == AIE_F32) return launch_write_rows<float, float>(CW_ARGS);
-    if (row_dtype == AIE_BF16 && cache_dtype == AIE_F32) return launch_write_rows<bf16, float>(CW_ARGS);
+struct CwArgs {                       // what a caller packs, in this order
+    const void *k, *v;                // [T, K, d], elements k_token / k_head (v_token / v_head) apart between tokens and heads
+    void *k_pages, *v_pages;
+    const int* slots;
+    unsigned* err;
+    long long k_token, k_head, v_token, v_head;
+    int row_dtype, cache_dtype, T, num_pages, P, K, d;      // num_pages * P and 2 * K * d fit 31 bits
+};
+
+extern "C" int aie_write_kv_slots(const CwArgs* args, cudaStream_t stream) {
+    const CwArgs& a = *args;
+    if (a.T <= 0) return 0;
+    if (a.P <= 0 || a.K <= 0 || a.d <= 0 || a.num_pages < 0) return AIE_BAD_ARG;
+    const long long step = a.row_dtype == AIE_BF16 ? 8 : 4;      // elements in 16 bytes
+    const bool wide = a.d % 8 == 0 && (a.k_token | a.k_head | a.v_token | a.v_head) % step == 0 &&
+                      ((size_t)a.k | (size_t)a.v | (size_t)a.k_pages | (size_t)a.v_pages) % 16 == 0;
+#define CW_ARGS wide, a.k, a.v, a.k_token, a.k_head, a.v_token, a.v_head, a.k_pages, a.v_pages, a.slots, a.T, a.num_pages, a.P, a.K, a.d, a.err, stream
+    if (a.row_dtype == AIE_BF16 && a.cache_dtype == AIE_BF16) return launch_write_rows<bf16, bf16>(CW_ARGS);
+    if (a.row_dtype == AIE_F32 && a.cache_dtype == AIE_BF16) return launch_write_rows<float, bf16>(CW_ARGS);
+    if (a.row_dtype == AIE_F32 && a.cache_dtype == AIE_F32) return launch_write_rows<float, float>(CW_ARGS);
+    if (a.row_dtype == AIE_BF16 && a.cache_dtype == AIE_F32) return launch_write_rows<bf16, float>(CW_ARGS);
     return AIE_BAD_ARG;
 #undef CW_ARGS
 }

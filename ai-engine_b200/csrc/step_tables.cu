@@ -167,14 +167,22 @@ step_tables_kernel(const int* __restrict__ cached, const int* __restrict__ count
     if (bad) atomicOr(err, bad);
 }
 
-// cached, counts, held [R], tables [R, W], free_pages [F], free_count [1]; the outputs lie elsewhere.  num_pages * P fits 31 bits.
-extern "C" int aie_step_tables(const int* cached, const int* counts, const int* held_in, const int* tables_in, const int* free_pages,
-                               const int* free_count, int R, int W, int F, int P, int num_pages, int capacity, int* tables, int* held,
-                               int* free_left, int* q_start, int* q_len, int* positions, int* token_req, int* slots, unsigned* err,
-                               cudaStream_t stream) {
-    if (R <= 0 || W <= 0 || F < 0 || P <= 0 || num_pages < 0 || capacity < 0) return AIE_BAD_ARG;
+struct StArgs {                       // what a caller packs, in this order
+    const int *cached, *counts, *held_in, *tables_in, *free_pages, *free_count;      // [R], [R], [R], [R, W], [F], [1]
+    int* out;                         // tables [R, W], held [R], free_left [1], q_start [R], q_len [R], then positions, token_req, slots [capacity]
+    unsigned* err;
+    int R, W, F, P, num_pages, capacity;      // num_pages * P fits 31 bits
+};
+
+extern "C" int aie_step_tables(const StArgs* args, cudaStream_t stream) {
+    const StArgs& a = *args;
+    const int R = a.R, W = a.W, capacity = a.capacity;
+    if (R <= 0 || W <= 0 || a.F < 0 || a.P <= 0 || a.num_pages < 0 || capacity < 0) return AIE_BAD_ARG;
     if (R > ST_MAX_REQUESTS) return -3;
-    const bool vec = W % 4 == 0 && ((size_t)tables_in | (size_t)tables) % 16 == 0;
+    int* held = a.out + (size_t)R * W;
+    int *free_left = held + R, *q_start = free_left + 1, *q_len = q_start + R, *positions = q_len + R, *token_req = positions + capacity,
+        *slots = token_req + capacity;
+    const bool vec = W % 4 == 0 && ((size_t)a.tables_in | (size_t)a.out) % 16 == 0;
     const int most = 2 * aie_sm_count();
     const long long entries = (long long)R * (vec ? W / 4 : W);
     const long long tb = (entries + ST_THREADS - 1) / ST_THREADS, kb = (capacity + ST_THREADS - 1) / ST_THREADS;
@@ -182,7 +190,7 @@ extern "C" int aie_step_tables(const int* cached, const int* counts, const int* 
     auto kern = vec ? step_tables_kernel<true> : step_tables_kernel<false>;
     const size_t smem = (size_t)R * sizeof(StRow);
     if (smem > 48 * 1024) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    return (int)launch_pdl(kern, dim3(table_blocks + token_blocks), dim3(ST_THREADS), smem, stream, cached, counts, held_in, tables_in,
-                           free_pages, free_count, R, W, F, P, num_pages, capacity, table_blocks, tables, held, free_left, q_start, q_len,
-                           positions, token_req, slots, err);
+    return (int)launch_pdl(kern, dim3(table_blocks + token_blocks), dim3(ST_THREADS), smem, stream, a.cached, a.counts, a.held_in, a.tables_in,
+                           a.free_pages, a.free_count, R, W, a.F, a.P, a.num_pages, capacity, table_blocks, a.out, held, free_left, q_start,
+                           q_len, positions, token_req, slots, a.err);
 }

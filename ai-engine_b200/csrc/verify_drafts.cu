@@ -230,17 +230,24 @@ verify_drafts_kernel(const float* __restrict__ target, long long target_row, int
     cluster.sync();      // a block's sums are read by the others until here
 }
 
-// target: rows of V floats, `target_row` apart; draft_probs (or null): row i of request r at r * draft_req + i * draft_place;
-// draft_tokens, accept_draws [R, N]; draft_len [R] or null (N each); tokens [R, N + 1], emitted [R].
-extern "C" int aie_verify_drafts(const float* target, long long target_row, int T, int V, const int* q_start, const int* draft_tokens,
-                                 const int* draft_len, const float* draft_probs, long long draft_req, long long draft_place, int R, int N,
-                                 const float* accept_draws, const float* token_draws, int* tokens, int* emitted, unsigned* err,
-                                 cudaStream_t stream) {
-    if (R <= 0) return 0;
-    if (V <= 0 || N < 0 || T < 0) return AIE_BAD_ARG;
-    if (V > VD_CLUSTER * VD_MAX_SEGMENTS * VD_SEGMENT || R > 0x7fffffff / VD_CLUSTER) return -3;
-    const bool vec = ((size_t)target | (size_t)draft_probs) % 16 == 0 && (target_row | draft_req | draft_place) % 4 == 0;
-    return (int)launch_pdl(vec ? verify_drafts_kernel<true> : verify_drafts_kernel<false>, dim3(R * VD_CLUSTER), dim3(VD_THREADS), 0, stream,
-                           target, target_row, T, V, q_start, draft_tokens, draft_len, draft_probs, draft_req, draft_place, N, accept_draws,
-                           token_draws, tokens, emitted, err);
+struct VdArgs {                       // what a caller packs, in this order
+    const float* target;              // rows of V floats, target_row apart
+    const int *q_start, *draft_tokens, *draft_len;      // [R], [R, N], [R] or null: N each
+    const float* draft_probs;         // row i of request r at r * draft_req + i * draft_place, or null
+    const float *accept_draws, *token_draws;            // [R, N], [R]
+    int *tokens, *emitted;            // [R, N + 1], [R]
+    unsigned* err;
+    long long target_row, draft_req, draft_place;
+    int T, V, R, N;
+};
+
+extern "C" int aie_verify_drafts(const VdArgs* args, cudaStream_t stream) {
+    const VdArgs& a = *args;
+    if (a.R <= 0) return 0;
+    if (a.V <= 0 || a.N < 0 || a.T < 0) return AIE_BAD_ARG;
+    if (a.V > VD_CLUSTER * VD_MAX_SEGMENTS * VD_SEGMENT || a.R > 0x7fffffff / VD_CLUSTER) return -3;
+    const bool vec = ((size_t)a.target | (size_t)a.draft_probs) % 16 == 0 && (a.target_row | a.draft_req | a.draft_place) % 4 == 0;
+    return (int)launch_pdl(vec ? verify_drafts_kernel<true> : verify_drafts_kernel<false>, dim3(a.R * VD_CLUSTER), dim3(VD_THREADS), 0, stream,
+                           a.target, a.target_row, a.T, a.V, a.q_start, a.draft_tokens, a.draft_len, a.draft_probs, a.draft_req,
+                           a.draft_place, a.N, a.accept_draws, a.token_draws, a.tokens, a.emitted, a.err);
 }

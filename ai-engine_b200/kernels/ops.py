@@ -6,7 +6,8 @@ from __future__ import annotations
 
 import math
 import os
-from ctypes import byref, c_float, c_int, c_longlong, c_void_p
+import struct
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
 from typing import Optional
 
 import numpy as np
@@ -718,35 +719,43 @@ def paged_attention(q, k_pages, v_pages, ctx, work, block_table, scale: float, w
 
 # ---------------------------------------------------------------------------
 # steps whose lengths the device alone knows (drafted tokens and their verification)
-_LAUNCHERS = {}
+class Launcher:
+    """A launcher of csrc/<source> that takes one packed struct of arguments, then plain integers: packing and one call of three
+    arguments take 2 us of the host's time, a call of twenty arguments 5.  `layout`: the struct's fields in the order of the C
+    declaration, as the struct module names them (native sizes and alignment)."""
+
+    def __init__(self, source: str, name: str, layout: str, ints: int = 0):
+        self.source, self.name, self.pack = source, name, struct.Struct("@" + layout).pack
+        self.argtypes = [c_char_p] + [c_int] * ints + [c_void_p]
+        self.fn = None
+
+    def __call__(self, fields: tuple, stream: int, *ints: int) -> None:
+        if self.fn is None:
+            self.fn = getattr(library(self.source), self.name)
+            self.fn.argtypes = self.argtypes
+        check(self.fn(self.pack(*fields), *ints, stream), self.name[4:])
 
 
-def launcher(source: str, name: str, signature: str):
-    """The launcher `name` of csrc/<source> with its argument types set, so that plain Python numbers can be passed:
-    p a pointer, i an int, l a long long, f a float."""
-    fn = _LAUNCHERS.get(name)
-    if fn is None:
-        fn = getattr(library(source), name)
-        fn.argtypes = [{"p": c_void_p, "i": c_int, "l": c_longlong, "f": c_float}[c] for c in signature]
-        _LAUNCHERS[name] = fn
-    return fn
-
-
-def on_current_device(what: str, *ts) -> int:
-    """The current device's stream as a number, for operands (None: left out) that all live on that device; any others are refused."""
-    require_cuda()
-    dev = torch.cuda.current_device()
-    for t in ts:
-        if t is not None and t.get_device() != dev:
-            raise KernelError(f"{what}: operands must live on the current CUDA device (cuda:{dev})")
-    return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
-
-
-def int_rows(what: str, **ts) -> None:
-    """Refuses index arrays (name=(tensor, shape)) that are not contiguous int32 of their shape."""
-    for name, (t, shape) in ts.items():
-        if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+def check_operands(what: str, ints, others=()) -> int:
+    """The current device's stream as a number, for operands that live on that device.  `ints`: (name, tensor, shape) of index arrays, which
+    have to be contiguous int32 of their shape; `others`: further tensors.  None stands for an operand that was left out."""
+    for name, t, shape in ints:
+        if t is not None and (t.dtype is not _I32 or t.shape != shape or not t.is_contiguous()):
             raise KernelError(f"{what}: {name} must be a contiguous int32 tensor {list(shape)}, got {t.dtype} {list(t.shape)}")
+    if not ints[0][1].is_cuda:
+        require_cuda()
+        raise KernelError(f"{what}: operands must live on the CUDA device")
+    dev = torch._C._cuda_getDevice()
+    for name, t, shape in ints:
+        if t is not None and t.get_device() != dev:
+            raise KernelError(f"{what}: {name} must live on the current CUDA device (cuda:{dev}), not on {t.device}")
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise KernelError(f"{what}: operands must live on the current CUDA device (cuda:{dev}), not on {t.device}")
+    return _raw_stream(dev)
+
+
+_I32 = torch.int32
 
 
 def _pools(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor):
@@ -776,14 +785,28 @@ def write_kv_slots(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
         raise KernelError("write_kv_slots: the elements of a head must be contiguous")
     if 2 * K * d > 0x7fffffff:
         raise KernelError("write_kv_slots: a token's rows are too long")
-    int_rows("write_kv_slots", slots=(slots, (T,)), err=(err, (1,)))
-    stream = on_current_device("write_kv_slots", k, v, k_pages, v_pages, slots, err)
+    stream = check_operands("write_kv_slots", (("slots", slots, (T,)), ("err", err, (1,))), (k, v, k_pages, v_pages))
     if T == 0:
         return
-    fn = launcher("cache_write.cu", "aie_write_kv_slots", "ppillllppipiiiiipp")
+    (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
     with region("write_kv_slots", 2 * T * K * d * (k.element_size() + k_pages.element_size())):
-        check(fn(k.data_ptr(), v.data_ptr(), code, k.stride(0), k.stride(1), v.stride(0), v.stride(1), k_pages.data_ptr(),
-                 v_pages.data_ptr(), dtype_code(k_pages), slots.data_ptr(), T, N, P, K, d, err.data_ptr(), stream), "write_kv_slots")
+        _WRITE((k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), slots.data_ptr(), err.data_ptr(), kt, kh, vt, vh, code,
+                dtype_code(k_pages), T, N, P, K, d), stream)
+
+
+_WRITE = Launcher("cache_write.cu", "aie_write_kv_slots", "6P4q7i")
+_CHUNK_ARGS = "11P2q10ifP"
+_CHUNKS_F32 = Launcher("attention_chunks_f32.cu", "aie_attention_chunks_f32", _CHUNK_ARGS, 1)
+_CHUNKS_BF16 = Launcher("attention_chunks.cu", "aie_attention_chunks_bf16", _CHUNK_ARGS, 1)
+
+
+def chunk_form(bf16: bool, d: int, rows: float):
+    """(rows of an item, blocks an SM, width of the scratch's rows) of the kernel that takes heads of d; `rows`: of queries that a request
+    has for a key head, on average."""
+    if bf16 and d in (64, 128):
+        return (16 if rows <= 16 else 32), 2, d
+    wide = 64 if d <= 64 else 128 if d <= 128 else 256
+    return (16 if wide == 256 else 32), (2 if wide == 64 else 1), wide
 
 
 def paged_attention_chunks(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor,
@@ -809,14 +832,13 @@ def paged_attention_chunks(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     if block_table.dim() != 2 or block_table.shape[1] == 0:
         raise KernelError("paged_attention_chunks: the block table must be [requests, pages]")
     R, W = block_table.shape
-    int_rows("paged_attention_chunks", q_start=(q_start, (R,)), q_len=(q_len, (R,)), ctx_len=(ctx_len, (R,)),
-             block_table=(block_table, (R, W)), err=(err, (1,)))
     if W * P > 0x7fffffff - 1024:
         raise KernelError("paged_attention_chunks: the table names more than 2^31 keys a request")
     if not 0 <= window <= 0x7fffffff:
         raise KernelError("paged_attention_chunks: a window is 0 (none) or a number of keys")
+    by_token, by_head, by_element = q.stride()
     per = 16 // q.element_size()
-    if T and (q.stride(2) != 1 or q.stride(0) % per or q.stride(1) % per or q.data_ptr() % 16):
+    if T and (by_element != 1 or by_token % per or by_head % per or q.data_ptr() % 16):
         raise KernelError("paged_attention_chunks: every head's row of q must be contiguous and start on 16 bytes")
     if k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16:
         raise KernelError("paged_attention_chunks: the pools must start on 16 bytes")
@@ -824,20 +846,25 @@ def paged_attention_chunks(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
         out = torch.empty((T, H, d), dtype=q.dtype, device=q.device)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16:
         raise KernelError("paged_attention_chunks: out must be contiguous, of q's shape and dtype, and start on 16 bytes")
-    stream = on_current_device("paged_attention_chunks", q, k_pages, v_pages, q_start, q_len, ctx_len, block_table, err, out)
+    stream = check_operands("paged_attention_chunks",
+                            (("q_start", q_start, (R,)), ("q_len", q_len, (R,)), ("ctx_len", ctx_len, (R,)),
+                             ("block_table", block_table, (R, W)), ("err", err, (1,))), (q, k_pages, v_pages, out))
     if T == 0 or R == 0:
         return out
-    rows = c_int()
-    blocks = launcher("attention_chunks_f32.cu", "aie_attention_chunks_f32_blocks", "ip")(d, byref(rows))
-    wide = 64 if d <= 64 else 128 if d <= 128 else 256
-    parts = 2 * blocks * rows.value
+    bf16 = q.dtype is torch.bfloat16
+    rows, an_sm, wide = chunk_form(bf16, d, T * (H // K) / R)
+    blocks = an_sm * sm_count()
+    parts = 2 * blocks * rows
     scratch = torch.empty(parts * (wide + 2) + 4 * blocks, dtype=torch.float32, device=q.device)
     at = scratch.data_ptr()
-    fn = launcher("attention_chunks_f32.cu", "aie_attention_chunks_f32", "pllpppippppiiiiiiiiifppppp")
+    fields = (q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), q_start.data_ptr(), q_len.data_ptr(),
+              ctx_len.data_ptr(), block_table.data_ptr(), at, at + 4 * parts * wide, at + 4 * parts * (wide + 2), by_token, by_head,
+              R, W, T, N, P, H, K, H // K, d, window, scale * 1.4426950408889634, err.data_ptr())
     with region("attention_chunks", 2 * _nb(q)):
-        check(fn(q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), dtype_code(q),
-                 q_start.data_ptr(), q_len.data_ptr(), ctx_len.data_ptr(), block_table.data_ptr(), R, W, T, N, P, H, K, d, window, scale,
-                 at, at + 4 * parts * wide, at + 4 * parts * (wide + 2), err.data_ptr(), stream), "paged_attention_chunks")
+        if bf16 and d in (64, 128):
+            _CHUNKS_BF16(fields, stream, rows)
+        else:
+            _CHUNKS_F32(fields, stream, BF16 if bf16 else F32)
     return out
 
 
