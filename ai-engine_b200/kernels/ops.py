@@ -800,13 +800,19 @@ _CHUNKS_F32 = Launcher("attention_chunks_f32.cu", "aie_attention_chunks_f32", _C
 _CHUNKS_BF16 = Launcher("attention_chunks.cu", "aie_attention_chunks_bf16", _CHUNK_ARGS, 1)
 
 
-def chunk_form(bf16: bool, d: int, rows: float):
-    """(rows of an item, blocks an SM, width of the scratch's rows) of the kernel that takes heads of d; `rows`: of queries that a request
-    has for a key head, on average."""
+_CHUNKS_TC = Launcher("attention_chunks_tc.cu", "aie_attention_chunks_tc", _CHUNK_ARGS)
+
+
+def chunk_form(bf16: bool, d: int, page: int, rows: float, groups: int = 0):
+    """(launcher, its further arguments, rows of an item, blocks an SM, width of the scratch's rows) of the kernel for heads of d on pages
+    of `page` keys; `rows`: of queries that a request has for a key head, on average; `groups`: of 8 keys in a pool."""
     if bf16 and d in (64, 128):
-        return (16 if rows <= 16 else 32), 2, d
+        if rows > 32 and page % 8 == 0 and (128 % page == 0 or page % 128 == 0) and groups < 0x7fffffff:
+            return _CHUNKS_TC, (), 256, 1, d
+        m = 16 if rows <= 16 else 32
+        return _CHUNKS_BF16, (m,), m, 2, d
     wide = 64 if d <= 64 else 128 if d <= 128 else 256
-    return (16 if wide == 256 else 32), (2 if wide == 64 else 1), wide
+    return _CHUNKS_F32, (BF16 if bf16 else F32,), (16 if wide == 256 else 32), (2 if wide == 64 else 1), wide
 
 
 def paged_attention_chunks(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor,
@@ -851,8 +857,7 @@ def paged_attention_chunks(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
                              ("block_table", block_table, (R, W)), ("err", err, (1,))), (q, k_pages, v_pages, out))
     if T == 0 or R == 0:
         return out
-    bf16 = q.dtype is torch.bfloat16
-    rows, an_sm, wide = chunk_form(bf16, d, T * (H // K) / R)
+    launch, more, rows, an_sm, wide = chunk_form(q.dtype is torch.bfloat16, d, P, T * (H // K) / R, N * K * P // 8)
     blocks = an_sm * sm_count()
     parts = 2 * blocks * rows
     scratch = torch.empty(parts * (wide + 2) + 4 * blocks, dtype=torch.float32, device=q.device)
@@ -861,10 +866,7 @@ def paged_attention_chunks(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
               ctx_len.data_ptr(), block_table.data_ptr(), at, at + 4 * parts * wide, at + 4 * parts * (wide + 2), by_token, by_head,
               R, W, T, N, P, H, K, H // K, d, window, scale * 1.4426950408889634, err.data_ptr())
     with region("attention_chunks", 2 * _nb(q)):
-        if bf16 and d in (64, 128):
-            _CHUNKS_BF16(fields, stream, rows)
-        else:
-            _CHUNKS_F32(fields, stream, BF16 if bf16 else F32)
+        launch(fields, stream, *more)
     return out
 
 

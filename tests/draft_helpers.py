@@ -61,7 +61,7 @@ def plain_attention(b, dtype):
             x = (qs @ k[:, kh].T * b["scale"]).masked_fill(hidden, -math.inf)
             p = torch.softmax(x, dim=-1)
             o, size = p @ v[:, kh], p @ v[:, kh].abs()
-            most = qs.norm(dim=-1).max() * k[:, kh].norm(dim=-1).max() * b["scale"]
+            most = qs.norm(dim=-1).max() * k[:, kh].norm(dim=-1).max() * abs(b["scale"])      # a size, whatever the sign
             t = U * (4 * math.sqrt(d) + 4) * most
             e = 2 * t * v[:, kh].abs().max() + 4 * U * math.sqrt(c + n) * v[:, kh].abs().max()
             if dtype == torch.bfloat16:
