@@ -61,10 +61,9 @@ __global__ void __launch_bounds__(CB_WARPS * 32, 2) chunk_bf16_kernel(const ChAr
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int c = blockIdx.x, C = gridDim.x;
-    if (tid == 0) a.meta[c] = make_int4(0, 0, 0, 0);
+    if (tid == 0) a.meta[2 * c] = make_int4(0, 0, 0, 0);
     ChWalk w;
-    if (!ch_begin<CB_WARPS * 32, M, KT, 2>(a, c, C, &sh, w)) return;
-    const long long per = w.end - w.at;
+    if (!ch_begin<CB_WARPS * 32, M, KT>(a, c, C, &sh, w)) return;
     bf16* ring = reinterpret_cast<bf16*>(cb_smem) + warp * NST * S::stage;
     bf16* q_s = reinterpret_cast<bf16*>(cb_smem + S::q_off);
     float* ml = reinterpret_cast<float*>(cb_smem + S::ml_off);      // [warps][M][2]
@@ -77,7 +76,7 @@ __global__ void __launch_bounds__(CB_WARPS * 32, 2) chunk_bf16_kernel(const ChAr
     for (;;) {
         const int n = ch_share(w);
         const ChTile tl = w.tile;
-        const int c0 = w.req.c, s0 = a.q_start[w.r], hi = c0 + tl.i1 + 1;
+        const int c0 = w.req.c, s0 = w.s0, hi = c0 + tl.i1 + 1;
         const int* bt = a.table + (size_t)w.r * a.W;
         const int kt0 = tl.first + w.k;
         const int low_all = a.window > 0 ? c0 + tl.i0 - a.window + 1 : 0;      // first key that any row sees
@@ -89,7 +88,7 @@ __global__ void __launch_bounds__(CB_WARPS * 32, 2) chunk_bf16_kernel(const ChAr
                 const int k_at = (kt0 + i) * KT + warp * CK + (lane & (CK - 1));
                 long long row_at = -1;
                 if (k_at < hi && k_at >= low_all) {
-                    const int pi = k_at / a.P, page = __ldg(bt + pi);
+                    const int pi = ch_over(k_at, a.by_p), page = __ldg(bt + pi);
                     if (page >= 0 && page < a.num_pages) row_at = ((long long)page * a.K + w.kh) * a.P + (k_at - pi * a.P);
                     else bad |= AIE_DEV_PAGE_OOB;
                 }
@@ -112,7 +111,7 @@ __global__ void __launch_bounds__(CB_WARPS * 32, 2) chunk_bf16_kernel(const ChAr
             const int row = i / PC, pc = i % PC;
             uint4 x = make_uint4(0u, 0u, 0u, 0u);
             if (row < tl.rows) {
-                const int full = tl.row0 + row, t = full / a.G, g = full - t * a.G;
+                const int full = tl.row0 + row, t = ch_over(full, a.by_g), g = full - t * a.G;
                 x = *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.q) + (s0 + t) * a.q_token +
                                                     (long long)(w.kh * a.G + g) * a.q_head + pc * 8);
             }
@@ -128,7 +127,7 @@ __global__ void __launch_bounds__(CB_WARPS * 32, 2) chunk_bf16_kernel(const ChAr
             for (int e = 0; e < 2; ++e) {
                 m_run[mt][e] = -INFINITY;
                 l_run[mt][e] = 0.f;
-                pos[mt][e] = c0 + (tl.row0 + mt * 16 + r0 + 8 * e) / a.G;
+                pos[mt][e] = c0 + ch_over(tl.row0 + mt * 16 + r0 + 8 * e, a.by_g);
             }
 #pragma unroll
             for (int x = 0; x < D / 8; ++x)
@@ -269,8 +268,8 @@ __global__ void __launch_bounds__(CB_WARPS * 32, 2) chunk_bf16_kernel(const ChAr
                 y.x += f * z.x, y.y += f * z.y, y.z += f * z.z, y.w += f * z.w;
             }
             if (begins && ends) {
-                const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-                const int full = tl.row0 + row, t = full / a.G, h = w.kh * a.G + full - t * a.G;
+                const float inv = ch_inverse(l);
+                const int full = tl.row0 + row, t = ch_over(full, a.by_g), h = w.kh * a.G + full - t * a.G;
                 store4<bf16>(reinterpret_cast<bf16*>(a.out) + ((size_t)(s0 + t) * a.H + h) * D + e,
                              make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
             } else {
@@ -278,7 +277,7 @@ __global__ void __launch_bounds__(CB_WARPS * 32, 2) chunk_bf16_kernel(const ChAr
                 if (e == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * M + row) * 2) = make_float2(m, l);
             }
         }
-        if (begins && !ends && tid == 0) a.meta[c] = make_int4(w.r, w.kh, w.m, ch_parts(w, n, per));
+        if (begins && !ends && tid == 0) ch_leave(a, w, c, n);
         if (!ch_next<M, KT>(a, w, n)) break;
         __syncthreads();                      // the ring's memory is the next item's
     }
@@ -291,17 +290,18 @@ template <int D, int MT> static int launch_chunk_bf16(const ChArgs& a, int C, cu
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes);
     const int rc = (int)launch_pdl(kern, dim3(C), dim3(CB_WARPS * 32), S::bytes, st, a);
     if (rc) return rc;
-    return (int)launch_pdl(chunk_join_kernel<bf16, S::M, D>, dim3(C, S::M * D / 4 / 256), dim3(256), 0, st, a);
+    return launch_chunk_join<bf16, S::M, D>(a, C, st);
 }
 
-// Blocks of the kernels: two an SM.  The scratch is [2 * blocks * rows * (d + 2)] floats and [blocks] int4.
+// Blocks of the kernels: two an SM.  The scratch is [2 * blocks * rows * (d + 2)] floats and [2 * blocks] int4.
 extern "C" int aie_attention_chunks_bf16_blocks() { return 2 * aie_sm_count(); }
 
 // rows: 16 or 32 of an item
-extern "C" int aie_attention_chunks_bf16(const ChArgs* args, int rows, cudaStream_t stream) {
-    ChArgs a = *args;
-    if (a.R <= 0 || a.T <= 0) return 0;
-    if (a.W <= 0 || a.num_pages <= 0 || a.P <= 0 || a.K <= 0 || a.H % a.K) return AIE_BAD_ARG;
+extern "C" int aie_attention_chunks_bf16(const ChCall* call, int rows, cudaStream_t stream) {
+    if (call->R <= 0 || call->T <= 0) return 0;
+    ChArgs a;
+    const int rc = ch_args(call, 16, 64, &a);
+    if (rc) return rc;
     const int C = aie_attention_chunks_bf16_blocks();
     if (a.d == 64 && rows == 16) return launch_chunk_bf16<64, 1>(a, C, stream);
     if (a.d == 64 && rows == 32) return launch_chunk_bf16<64, 2>(a, C, stream);

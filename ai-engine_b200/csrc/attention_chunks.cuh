@@ -7,7 +7,7 @@
 //
 // All items' key tiles stand in one line, in the order of requests, key heads and row tiles; block c of C takes those from c * per to
 // (c + 1) * per - 1, per = ceil(all / C), so every block has the same number of tiles whatever the requests' lengths.  Every
-// block works out the line from the lengths by itself (two passes of sums over the requests), so nothing comes from the host and a
+// block works out the line from the lengths by itself (sums over the requests), so nothing comes from the host and a
 // captured call follows the lengths.  An item that a block does not finish is left as a part: sums of exp2(x - m) v without
 // division, m and l, in a place of the block's own (one for an item that it began, one for an item that it continued), and a second,
 // small kernel joins the parts of every item in their order.  The split depends on all requests' lengths: the sums of a token
@@ -15,7 +15,19 @@
 #pragma once
 #include "common.cuh"
 
-struct ChArgs {
+// n / d for n < 2^31 by a multiplication (Granlund and Montgomery, 1994): (n + high half of n * mul) >> shift
+struct ChDiv {
+    unsigned mul, shift;
+};
+static inline ChDiv ch_div(unsigned d) {
+    ChDiv v = {0u, 0u};
+    while ((1ull << v.shift) < d) ++v.shift;
+    v.mul = (unsigned)(((1ull << 32) * ((1ull << v.shift) - d)) / d + 1);
+    return v;
+}
+__device__ __forceinline__ int ch_over(int n, ChDiv d) { return (int)((__umulhi((unsigned)n, d.mul) + (unsigned)n) >> d.shift); }
+
+struct ChCall {                       // what a caller packs, in this order
     const void* q;                    // [T, H, d], elements q_token / q_head apart
     const void* k_pages;              // [num_pages, K, P, d]
     const void* v_pages;
@@ -23,17 +35,33 @@ struct ChArgs {
     const int *q_start, *q_len, *ctx_len, *table;
     float* part_o;                    // [2 * C][M][D]
     float* part_ml;                   // [2 * C][M][2]
-    int4* meta;                       // [C] (request, key head, row tile, parts) of the item that block c began and did not finish
+    int4* meta;                       // [C][2] of the item that block c began and did not finish: key head, first row, rows, parts; first token
     long long q_token, q_head;
     int R, W, T, num_pages, P, H, K, G, d, window;
     float scale2;                     // scale * log2 e: exponentials are powers of two
     unsigned* err;
 };
+struct ChArgs : ChCall {
+    ChDiv by_g, by_p;
+};
+
+// Checks a call and completes it; `tiles`: rows of an item and keys of a tile of the kernel that takes it.
+static inline int ch_args(const ChCall* call, int M, int KT, ChArgs* a) {
+    *static_cast<ChCall*>(a) = *call;
+    if (a->W <= 0 || a->num_pages <= 0 || a->P <= 0 || a->K <= 0 || a->H <= 0 || a->H % a->K || a->G != a->H / a->K) return AIE_BAD_ARG;
+    // the line's length has to fit 31 bits: every request at least one row tile a key head, each over all the table's keys
+    const double items = (double)a->T * a->H / M + (double)a->R * a->K, keys = (double)a->W * a->P / KT + 2;
+    if (items * keys > 2147000000.0) return -3;
+    a->by_g = ch_div((unsigned)a->G);
+    a->by_p = ch_div((unsigned)a->P);
+    return 0;
+}
 
 struct ChReq { int n, c; };           // tokens it brings (0: none, or lengths that do not fit), tokens it has
 __device__ __forceinline__ ChReq ch_req(const ChArgs& a, int r, unsigned* bad = nullptr) {
     const int n = a.q_len[r], c = a.ctx_len[r], s = a.q_start[r];
-    const bool fits = n >= 0 && c >= 0 && s >= 0 && s <= a.T && n <= a.T - s && ((long long)c + n + a.P - 1) / a.P <= a.W;
+    // W * P fits 31 bits
+    const bool fits = n >= 0 && c >= 0 && s >= 0 && s <= a.T && n <= a.T - s && c <= a.W * a.P && n <= a.W * a.P - c;
     if (!fits && bad) *bad |= AIE_DEV_SLOT_OOB;
     return {fits ? n : 0, c};
 }
@@ -43,41 +71,44 @@ template <int M, int KT> __device__ __forceinline__ ChTile ch_tile(const ChArgs&
     ChTile t;
     t.row0 = m * M;
     t.rows = min(M, q.n * a.G - t.row0);
-    t.i0 = t.row0 / a.G;
-    t.i1 = (t.row0 + t.rows - 1) / a.G;
+    t.i0 = ch_over(t.row0, a.by_g);
+    t.i1 = ch_over(t.row0 + t.rows - 1, a.by_g);
     const int lo = a.window > 0 ? max(0, q.c + t.i0 - a.window + 1) : 0;
     t.first = lo / KT;
     t.tiles = (q.c + t.i1) / KT - t.first + 1;
     return t;
 }
-template <int M, int KT> __device__ __forceinline__ long long ch_tiles(const ChArgs& a, const ChReq& q) {      // of one key head
-    long long s = 0;
+template <int M, int KT> __device__ __forceinline__ int ch_tiles(const ChArgs& a, const ChReq& q) {      // of one key head
+    int s = 0;
     for (int m = 0; m * M < q.n * a.G; ++m) s += ch_tile<M, KT>(a, q, m).tiles;
     return s;
 }
 
 // Where a block is in the line.
 struct ChWalk {
-    long long at, end;       // next key tile of the line, end of this block's share
-    int r, kh, m, k;         // item, and key tile within it
+    int left, per;           // key tiles that are left of this block's share, tiles of a share
+    int r, kh, m, k, s0;     // item, key tile within it, the request's first token
     ChReq req;
     ChTile tile;
 };
-struct ChShared { long long sums[32]; long long all; long long off; int r; };
+struct ChShared {
+    int sums[32];
+    int r, off, n, c, s0;    // request in which the share begins, how far behind the request's first tile, its lengths
+};
 
 // Adds up `v` over the block in the order of threads; the result is what comes before this thread's, `all` the sum.
-template <int THREADS> __device__ __forceinline__ long long ch_scan(long long v, ChShared* s, long long* all) {
+template <int THREADS> __device__ __forceinline__ int ch_scan(int v, ChShared* s, int* all) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long x = v;
+    int x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
     __syncthreads();
     if (lane == 31) s->sums[warp] = x;
     __syncthreads();
-    long long before = 0, total = 0;
+    int before = 0, total = 0;
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) {
         if (w == warp) before = total;
@@ -88,59 +119,69 @@ template <int THREADS> __device__ __forceinline__ long long ch_scan(long long v,
 }
 
 // This block's share of the line; false: none.  All threads of the block call it.
-template <int THREADS, int M, int KT, int MIN_TILES>
+template <int THREADS, int M, int KT>
 __device__ __forceinline__ bool ch_begin(const ChArgs& a, int c, int C, ChShared* s, ChWalk& w) {
     const int tid = threadIdx.x;
-    long long all = 0, mine = 0, before = 0;
+    int all = 0, mine = 0, before = 0;
+    ChReq q = {0, 0};
     for (int base = 0; base < a.R; base += THREADS) {
         const int r = base + tid;
         unsigned bad = 0;
         mine = 0;
         if (r < a.R) {
-            const ChReq q = ch_req(a, r, &bad);
+            q = ch_req(a, r, &bad);
             mine = a.K * ch_tiles<M, KT>(a, q);
             if (bad && c == 0) atomicOr(a.err, bad);
         }
-        long long sum;
+        int sum;
         before = all + ch_scan<THREADS>(mine, s, &sum);
         all += sum;
     }
-    long long per = (all + C - 1) / C;
-    if (per < MIN_TILES) per = MIN_TILES;
-    w.at = c * per;
-    w.end = min(all, w.at + per);
-    if (w.at >= all) return false;
+    w.per = (int)(((unsigned)all + C - 1) / (unsigned)C);
+    const long long first = (long long)c * w.per;
+    if (first >= all) return false;
+    const int at = (int)first;
+    w.left = min(w.per, all - at);
+    auto leave = [&](int r, const ChReq& x, int off) {
+        s->r = r;
+        s->off = off;
+        s->n = x.n;
+        s->c = x.c;
+        s->s0 = a.q_start[r];
+    };
     if (a.R <= THREADS) {
-        if (w.at >= before && w.at < before + mine) { s->r = tid; s->off = w.at - before; }
+        if (at >= before && at < before + mine) leave(tid, q, at - before);
     } else {
-        long long upto = 0;
+        int upto = 0;
         for (int base = 0; base < a.R; base += THREADS) {
             const int r = base + tid;
-            const long long here = r < a.R ? a.K * ch_tiles<M, KT>(a, ch_req(a, r)) : 0;
-            long long sum;
-            const long long b = upto + ch_scan<THREADS>(here, s, &sum);
-            if (w.at >= b && w.at < b + here) { s->r = r; s->off = w.at - b; }
+            q = r < a.R ? ch_req(a, r) : ChReq{0, 0};
+            const int here = r < a.R ? a.K * ch_tiles<M, KT>(a, q) : 0;
+            int sum;
+            const int b = upto + ch_scan<THREADS>(here, s, &sum);
+            if (at >= b && at < b + here) leave(r, q, at - b);
             upto += sum;
         }
     }
     __syncthreads();
     w.r = s->r;
-    w.req = ch_req(a, w.r);
-    const long long one = ch_tiles<M, KT>(a, w.req);
-    w.kh = (int)(s->off / one);
-    long long k = s->off % one;
+    w.s0 = s->s0;
+    w.req = {s->n, s->c};
+    const unsigned one = (unsigned)ch_tiles<M, KT>(a, w.req), off = (unsigned)s->off;
+    w.kh = (int)(off / one);
+    w.k = (int)(off - w.kh * one);
     for (w.m = 0;; ++w.m) {
         w.tile = ch_tile<M, KT>(a, w.req, w.m);
-        if (k < w.tile.tiles) break;
-        k -= w.tile.tiles;
+        if (w.k < w.tile.tiles) break;
+        w.k -= w.tile.tiles;
     }
-    w.k = (int)k;
     return true;
 }
-// ... the next item after `n` tiles of this one; false: the share is done
+__device__ __forceinline__ int ch_share(const ChWalk& w) { return min(w.tile.tiles - w.k, w.left); }      // key tiles of the item that are this block's
+// ... the next item behind the `n` tiles of this one; false: the share is done
 template <int M, int KT> __device__ __forceinline__ bool ch_next(const ChArgs& a, ChWalk& w, int n) {
-    w.at += n;
-    if (w.at >= w.end) return false;
+    w.left -= n;
+    if (w.left <= 0) return false;
     w.k = 0;
     ++w.m;
     if (w.m * M >= w.req.n * a.G) {
@@ -148,19 +189,19 @@ template <int M, int KT> __device__ __forceinline__ bool ch_next(const ChArgs& a
         if (++w.kh == a.K) {
             w.kh = 0;
             do { w.req = ch_req(a, ++w.r); } while (w.req.n == 0);
+            w.s0 = a.q_start[w.r];
         }
     }
     w.tile = ch_tile<M, KT>(a, w.req, w.m);
     return true;
 }
-__device__ __forceinline__ int ch_share(const ChWalk& w) {      // key tiles of the item that are this block's
-    return (int)min((long long)(w.tile.tiles - w.k), w.end - w.at);
+// What the joining kernel has to know of the item that block c begins here and does not finish with its `n` tiles.
+__device__ __forceinline__ void ch_leave(const ChArgs& a, const ChWalk& w, int c, int n) {
+    const int rest = w.tile.tiles - w.k - n;
+    a.meta[2 * c] = make_int4(w.kh, w.tile.row0, w.tile.rows, 1 + (rest + w.per - 1) / w.per);
+    a.meta[2 * c + 1] = make_int4(w.s0, 0, 0, 0);
 }
-// Blocks that have a part of the item which block `c` begins and leaves at `w` (its last `n` tiles of the share).
-__device__ __forceinline__ int ch_parts(const ChWalk& w, int n, long long per) {
-    const long long rest = w.tile.tiles - w.k - n;
-    return 1 + (int)((rest + per - 1) / per);
-}
+__device__ __forceinline__ float ch_inverse(float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); }      // of a row's sum; a row that sees nothing is zero
 
 // Joins the parts of the item that block c began: out = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p.  A thread has four columns of a row.
 template <typename T, int M, int D>
@@ -168,30 +209,53 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const ChArgs a) {
     pdl_launch_dependents();
     pdl_wait();
     const int c = blockIdx.x;
-    const int4 it = a.meta[c];
+    const int4 it = a.meta[2 * c], more = a.meta[2 * c + 1];
     if (it.w == 0) return;
-    const int r = it.x, n = a.q_len[r];
-    const int rows = min(M, n * a.G - it.z * M);
     constexpr int CH = D / 4;
-    for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * CH; i += gridDim.y * 256) {
+    for (int i = blockIdx.y * 256 + threadIdx.x; i < it.z * CH; i += gridDim.y * 256) {
         const int row = i / CH, e = (i - row * CH) * 4;
         if (e >= a.d) continue;
-        auto place = [&](int p) { return (size_t)(p == 0 ? 2 * c + 1 : 2 * (c + p)) * M + row; };
-        float m = -INFINITY;
-        for (int p = 0; p < it.w; ++p) m = fmaxf(m, a.part_ml[place(p) * 2]);
-        float l = 0.f;
+        // part 0 lies in block c's place for items begun, part p in block c + p's for items continued
+        const float* ml = a.part_ml + ((size_t)2 * c * M + row) * 2;
+        const float* po = a.part_o + ((size_t)2 * c * M + row) * D + e;
+        float m = -INFINITY, l = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int p = 0; p < it.w; ++p) {
-            const size_t at = place(p);
-            const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
-            const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
-            const float4 x = *reinterpret_cast<const float4*>(a.part_o + at * D + e);
-            l += f * ml.y;
-            o.x += f * x.x, o.y += f * x.y, o.z += f * x.z, o.w += f * x.w;
+        // eight parts at a time, so that their loads are under way together
+        for (int p0 = 0; p0 < it.w; p0 += 8) {
+            float2 g[8];
+            float4 x[8];
+#pragma unroll
+            for (int p = 0; p < 8; ++p) {
+                const bool there = p0 + p < it.w;
+                const size_t place = there ? (p0 + p == 0 ? 1 : 2 * (p0 + p)) : 1;
+                g[p] = there ? *reinterpret_cast<const float2*>(ml + place * (M * 2)) : make_float2(-INFINITY, 0.f);
+                x[p] = *reinterpret_cast<const float4*>(po + place * ((size_t)M * D));
+            }
+            float top = m;
+#pragma unroll
+            for (int p = 0; p < 8; ++p) top = fmaxf(top, g[p].x);
+            const float was = m == -INFINITY ? 0.f : exp2f(m - top);
+            l *= was;
+            o.x *= was, o.y *= was, o.z *= was, o.w *= was;
+#pragma unroll
+            for (int p = 0; p < 8; ++p) {
+                if (g[p].x == -INFINITY) continue;
+                const float f = exp2f(g[p].x - top);
+                l += f * g[p].y;
+                o.x += f * x[p].x, o.y += f * x[p].y, o.z += f * x[p].z, o.w += f * x[p].w;
+            }
+            m = top;
         }
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-        const int full = it.z * M + row, i_tok = full / a.G, h = it.y * a.G + full - i_tok * a.G;
-        store4<T>(reinterpret_cast<T*>(a.out) + ((size_t)(a.q_start[r] + i_tok) * a.H + h) * a.d + e,
+        const float inv = ch_inverse(l);
+        const int full = it.y + row, tok = ch_over(full, a.by_g), h = it.x * a.G + full - tok * a.G;
+        store4<T>(reinterpret_cast<T*>(a.out) + ((size_t)(more.x + tok) * a.H + h) * a.d + e,
                   make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
     }
+}
+// ... with as much shared memory an SM as the kernel before it, which would otherwise have to leave the SM before it changes
+template <typename T, int M, int D> static int launch_chunk_join(const ChArgs& a, int C, cudaStream_t st) {
+    auto kern = chunk_join_kernel<T, M, D>;
+    cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    constexpr int blocks = M * D / 4 / 256;
+    return (int)launch_pdl(kern, dim3(C, blocks > 8 ? 8 : blocks), dim3(256), 0, st, a);
 }

@@ -62,10 +62,9 @@ __global__ void __launch_bounds__(CfShape<D>::NW * 32) chunk_f32_kernel(const Ch
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int c = blockIdx.x, C = gridDim.x;
-    if (tid == 0) a.meta[c] = make_int4(0, 0, 0, 0);
+    if (tid == 0) a.meta[2 * c] = make_int4(0, 0, 0, 0);
     ChWalk w;
-    if (!ch_begin<NW * 32, M, KT, 1>(a, c, C, &sh, w)) return;
-    const long long per = w.end - w.at;           // that of all blocks, or less in the last one with a share, which leaves no parts
+    if (!ch_begin<NW * 32, M, KT>(a, c, C, &sh, w)) return;
     float* ring = cf_smem + warp * NST * S::stage;
     float* q_s = cf_smem + S::q_off;              // [M][D], 16-byte pieces at (piece ^ row & 7)
     float* p_s = cf_smem + S::p_off + warp * 8 * M;      // this warp's [8 keys][M]
@@ -78,14 +77,14 @@ __global__ void __launch_bounds__(CfShape<D>::NW * 32) chunk_f32_kernel(const Ch
     for (;;) {
         const int n = ch_share(w);
         const ChTile tl = w.tile;
-        const int c0 = w.req.c, s0 = a.q_start[w.r], hi = c0 + tl.i1 + 1;
+        const int c0 = w.req.c, s0 = w.s0, hi = c0 + tl.i1 + 1;
         const int jn = (tl.rows + 3) >> 2;        // fours of rows that are there
         // queries of the item
         for (int i = tid; i < M * CH; i += NW * 32) {
             const int row = i / CH, ch = i - row * CH, e = ch * 4;
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
             if (row < tl.rows && e < a.d) {
-                const int full = tl.row0 + row, t = full / a.G, g = full - t * a.G;
+                const int full = tl.row0 + row, t = ch_over(full, a.by_g), g = full - t * a.G;
                 x = load4<T>(reinterpret_cast<const T*>(a.q) + (s0 + t) * a.q_token + (long long)(w.kh * a.G + g) * a.q_head + e);
             }
             *reinterpret_cast<float4*>(q_s + row * D + ((ch ^ (row & 7)) << 2)) = x;
@@ -100,7 +99,7 @@ __global__ void __launch_bounds__(CfShape<D>::NW * 32) chunk_f32_kernel(const Ch
                 const int k_at = (kt0 + i) * KT + warp * 8 + (lane & 7);
                 long long row_at = -1;
                 if (k_at < hi && (a.window <= 0 || k_at > c0 + tl.i0 - a.window)) {
-                    const int pi = k_at / a.P, page = bt[pi];
+                    const int pi = ch_over(k_at, a.by_p), page = bt[pi];
                     if (page >= 0 && page < a.num_pages) row_at = ((long long)page * a.K + w.kh) * a.P + (k_at - pi * a.P);
                     else bad |= AIE_DEV_PAGE_OOB;
                 }
@@ -157,7 +156,7 @@ __global__ void __launch_bounds__(CfShape<D>::NW * 32) chunk_f32_kernel(const Ch
                 corr[j] = 1.f;
                 if (j < jn) {
                     const float2 f = cf_both(s2[j]);
-                    const int row = j * 4 + rg, pos = c0 + (tl.row0 + row) / a.G;
+                    const int row = j * 4 + rg, pos = c0 + ch_over(tl.row0 + row, a.by_g);
                     const bool sees = row < tl.rows && k_at <= pos && (a.window <= 0 || k_at > pos - a.window);
                     const float x = sees ? (f.x + f.y) * a.scale2 : -INFINITY;
                     float top = x;
@@ -253,8 +252,8 @@ __global__ void __launch_bounds__(CfShape<D>::NW * 32) chunk_f32_kernel(const Ch
                 y.x += f * z.x, y.y += f * z.y, y.z += f * z.z, y.w += f * z.w;
             }
             if (begins && ends) {
-                const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-                const int full = tl.row0 + row, t = full / a.G, h = w.kh * a.G + full - t * a.G;
+                const float inv = ch_inverse(l);
+                const int full = tl.row0 + row, t = ch_over(full, a.by_g), h = w.kh * a.G + full - t * a.G;
                 if (e < a.d)
                     store4<T>(reinterpret_cast<T*>(a.out) + ((size_t)(s0 + t) * a.H + h) * a.d + e,
                               make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
@@ -263,7 +262,7 @@ __global__ void __launch_bounds__(CfShape<D>::NW * 32) chunk_f32_kernel(const Ch
                 if (e == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * M + row) * 2) = make_float2(m, l);
             }
         }
-        if (begins && !ends && tid == 0) a.meta[c] = make_int4(w.r, w.kh, w.m, ch_parts(w, n, per));
+        if (begins && !ends && tid == 0) ch_leave(a, w, c, n);
         if (!ch_next<M, KT>(a, w, n)) break;
         __syncthreads();                          // the ring's memory is the next item's
     }
@@ -276,19 +275,20 @@ template <typename T, int D> static int launch_chunk_f32(const ChArgs& a, int C,
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes);
     const int rc = (int)launch_pdl(kern, dim3(C), dim3(S::NW * 32), S::bytes, st, a);
     if (rc) return rc;
-    return (int)launch_pdl(chunk_join_kernel<T, S::M, D>, dim3(C, S::M * D / 4 / 256), dim3(256), 0, st, a);
+    return launch_chunk_join<T, S::M, D>(a, C, st);
 }
 
-// Rows of an item, and blocks of the kernel.  The scratch is [2 * blocks * rows * (D + 2)] floats and [blocks] int4, D the head size
+// Rows of an item, and blocks of the kernel.  The scratch is [2 * blocks * rows * (D + 2)] floats and [2 * blocks] int4, D the head size
 // rounded up to 64, 128 or 256.
 extern "C" int aie_attention_chunks_f32_rows(int d) { return d > 128 ? CfShape<256>::M : CfShape<128>::M; }
 extern "C" int aie_attention_chunks_f32_blocks(int d) { return aie_sm_count() * (d <= 64 ? 2 : 1); }
 
-extern "C" int aie_attention_chunks_f32(const ChArgs* args, int dtype, cudaStream_t stream) {
-    const ChArgs& a = *args;
-    if (a.R <= 0 || a.T <= 0) return 0;
-    if (a.d <= 0 || a.d > 256 || a.d % 8) return AIE_UNSUPPORTED;
-    if (a.W <= 0 || a.num_pages <= 0 || a.P <= 0 || a.K <= 0 || a.H % a.K) return AIE_BAD_ARG;
+extern "C" int aie_attention_chunks_f32(const ChCall* call, int dtype, cudaStream_t stream) {
+    if (call->R <= 0 || call->T <= 0) return 0;
+    if (call->d <= 0 || call->d > 256 || call->d % 8) return AIE_UNSUPPORTED;
+    ChArgs a;
+    const int rc = ch_args(call, 16, 32, &a);
+    if (rc) return rc;
     const int C = aie_attention_chunks_f32_blocks(a.d), w = a.d <= 64 ? 0 : a.d <= 128 ? 1 : 2;
     if (dtype == AIE_F32) return w == 0 ? launch_chunk_f32<float, 64>(a, C, stream) : w == 1 ? launch_chunk_f32<float, 128>(a, C, stream) : launch_chunk_f32<float, 256>(a, C, stream);
     if (dtype == AIE_BF16) return w == 0 ? launch_chunk_f32<bf16, 64>(a, C, stream) : w == 1 ? launch_chunk_f32<bf16, 128>(a, C, stream) : launch_chunk_f32<bf16, 256>(a, C, stream);

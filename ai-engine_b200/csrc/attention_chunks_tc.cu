@@ -9,13 +9,14 @@
 //   warps 0-3, 4-7   softmax of stream 0 / 1, a thread a row: the row of S in registers (tcgen05.ld), masked on tiles that
 //                    touch the diagonal or a window's edge; its reference maximum moves by more than 8 (log2 units) or not at all, so that
 //                    outputs are rarely rescaled; probabilities go as bfloat16 pairs over the scores in tensor memory;
-//   warp 8           keys and values by TMA: a box a page (128 keys of a larger page), in the order in which the products read them, into
+//   warps 8, 10      keys, values by TMA: a box a page (128 keys of a larger page), in the order in which the products read them, into
 //                    one ring of 128-key tiles of both that runs on from item to item.  A page that is not there has a box past the pool's
-//                    end, which arrives as zeros;
+//                    end, which arrives as zeros.  (One warp for both spent 2,000 cycles a tile of eight pages on asking, more than
+//                    the tile's bytes take at heads of 64.)
 //   warp 9           issues the products: S = Q K^T and O += P V of a step of a stream, P from tensor memory, V as the MN-major
 //                    operand; zeroes the values past a request's last key, since a probability of 0 must not meet what an unwritten slot
 //                    holds;
-//   warps 10, 11     queries: rows = (token, head of the group) gathered by cp.async into the swizzled tile that TMA would write (tokens
+//   warp 11          queries: rows = (token, head of the group) gathered by cp.async into the swizzled tile that TMA would write (tokens
 //                    and heads may lie any distance apart), ahead of the item that uses them where a place is free.
 // Tensor memory: scores of stream t at columns 128 t (P over the first 64), outputs at 256 + 128 t.
 // What bounds it: long chunks the exponentials (16 a cycle and SM: 2,048 cycles for two rows' tiles of 128 keys, against 2,048 of
@@ -37,7 +38,7 @@ template <int D> struct CtShape {
     static constexpr int NS = D == 128 ? 5 : 10;       // tiles of keys or values in the ring
     // [3 KB: barriers, what the walk and the streams tell one another | queries x 2 | ring], 227 KB at heads of 128: nothing is left
     // for aligning the start, which the runtime puts on 1 KB as long as there is no other shared memory
-    static constexpr int walk_off = 256, meet_off = 1024, q_off = 3072, kv_off = q_off + 2 * tile, bytes = kv_off + NS * tile;
+    static constexpr int walk_off = 256, warps_off = 480, meet_off = 1024, q_off = 3072, kv_off = q_off + 2 * tile, bytes = kv_off + NS * tile;
 };
 
 // The order in which an item's tiles of keys (K) and values (V) pass through the ring: `ahead` tiles of keys, then V(j), K(j + ahead).
@@ -50,6 +51,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     constexpr int M = S::M, NS = S::NS, TILE = S::tile, HV = D / 64, GROUP = HV * 1024, PC = D / 8;
     extern __shared__ __align__(1024) unsigned char sm[];
     ChShared* sh = reinterpret_cast<ChShared*>(sm + S::walk_off);
+    ChWalk* walks = reinterpret_cast<ChWalk*>(sm + S::warps_off);      // [8] where a softmax warp is, while its registers hold a row
+    static_assert(sizeof(ChShared) <= S::warps_off - S::walk_off && 8 * sizeof(ChWalk) <= S::meet_off - S::warps_off, "places");
     float2(*meet)[CT_M] = reinterpret_cast<float2(*)[CT_M]>(sm + S::meet_off);      // [2] (m, l) of a row's two streams
     unsigned long long* full = reinterpret_cast<unsigned long long*>(sm);      // [NS]
     unsigned long long* empty = full + NS;          // [NS]
@@ -59,39 +62,40 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     unsigned long long* o_done = s_full + 2;        // [2] the last product of an item's stream is done
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(o_done + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    int* asked = reinterpret_cast<int*>(tmem_slot + 2);
+    unsigned* armed = tmem_slot + 2;                // [2][2] tiles of the ring that the loaders asked for last, and of what phase (a bit each)
     unsigned char* q_s = sm + S::q_off;
     unsigned char* kv_s = sm + S::kv_off;
 
+    // what needs nothing from the kernel before this one
     pdl_launch_dependents();
-    pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int c = blockIdx.x, C = gridDim.x;
-    if (tid == 0) a.meta[c] = make_int4(0, 0, 0, 0);
-    ChWalk w;
-    if (tc_smem(sm) & 1023u) {                      // swizzled tiles would not be where the products look for them
-        if (tid == 0) atomicOr(a.err, AIE_DEV_WAIT_TIMEOUT);
-        return;
-    }
-    if (!ch_begin<CT_THREADS, M, CT_KT, 2>(a, c, C, sh, w)) return;
-    const long long per = w.end - w.at;
-
     if (tid == 0) {
         for (int s = 0; s < NS; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
         for (int t = 0; t < 2; ++t) {
-            mbar_init(&q_full[t], 2);
+            mbar_init(&q_full[t], 1);
             mbar_init(&q_empty[t], 1);
             mbar_init(&s_full[t], 1);
             mbar_init(&o_done[t], 1);
         }
         *abort_flag = 0;
-        *asked = 0;
+        for (int i = 0; i < 4; ++i) armed[i] = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        tma_prefetch_map(&map_k);
+        tma_prefetch_map(&map_v);
     }
+    pdl_wait();
+    if (tid == 0) a.meta[2 * c] = make_int4(0, 0, 0, 0);
+    if (tc_smem(sm) & 1023u) {                      // swizzled tiles would not be where the products look for them
+        if (tid == 0) atomicOr(a.err, AIE_DEV_WAIT_TIMEOUT);
+        return;
+    }
+    ChWalk w;
+    if (!ch_begin<CT_THREADS, M, CT_KT>(a, c, C, sh, w)) return;
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc_smem(tmem_slot)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
@@ -105,54 +109,68 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     // each, 88 + 2 x 208 = 3 x 168 (an increase waits for what a decrease has released)
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n");
-        if (warp == 8) {
+        if (warp == 8 || warp == 10) {
+            // keys / values.  In the ring an item's first L tiles of keys come first, then V(0), K(L), V(1), K(L + 1), .. and
+            // the last tiles of values: the order in which the products read them
+            const bool values = warp == 10;
+            const CUtensorMap* map = values ? &map_v : &map_k;
             const int BP = min(a.P, CT_KT), boxes = CT_KT / BP;      // rows of a box; lane i asks for box i of a tile
-            int slot = 0, ph = 1, n_asked = 0;
-            unsigned bad = 0;
+            int slot = 0, ph = 1;
+            unsigned bad = 0, mine = 0, phase = 0;
             bool ok = true;
-            for (; ok;) {
-                const int n = ch_share(w), L = ct_ahead(w.tile), kt0 = w.tile.first + w.k;
+            auto skip = [&](int n) {                                 // n < NS
+                slot += n;
+                if (slot >= NS) {
+                    slot -= NS;
+                    ph ^= 1;
+                }
+            };
+            for (;;) {
+                const int n = ch_share(w), L = min(ct_ahead(w.tile), n), kt0 = w.tile.first + w.k;
                 const int hi = w.req.c + w.tile.i1 + 1, low = a.window > 0 ? w.req.c + w.tile.i0 - a.window + 1 : 0;
                 const int* bt = a.table + (size_t)w.r * a.W;
-                // first group of 8 rows of this lane's box of tile j
-                auto group_of = [&](int j) {
-                    if (j >= n || lane >= boxes) return end_group;
+                // the page of this lane's box of tile j (read some tiles ahead of its use), and its first group of 8 rows
+                auto wanted = [&](int j) {
                     const int key = (kt0 + j) * CT_KT + lane * BP;
-                    if (key >= hi || key + BP <= low) return end_group;
-                    const int pi = key / a.P, page = bt[pi];
-                    if (page >= 0 && page < a.num_pages) return (int)((((long long)page * a.K + w.kh) * a.P + (key - pi * a.P)) >> 3);
+                    return j < n && lane < boxes && key < hi && key + BP > low;
+                };
+                auto page_of = [&](int j) { return wanted(j) ? __ldg(bt + ch_over((kt0 + j) * CT_KT + lane * BP, a.by_p)) : -1; };
+                auto group_of = [&](int j, int page) {
+                    if (!wanted(j)) return end_group;
+                    if (page >= 0 && page < a.num_pages) {
+                        const int key = (kt0 + j) * CT_KT + lane * BP, in = key - ch_over(key, a.by_p) * a.P;
+                        return (int)((((long long)page * a.K + w.kh) * a.P + in) >> 3);
+                    }
                     bad |= AIE_DEV_PAGE_OOB;
                     return end_group;
                 };
-                auto ask = [&](const CUtensorMap* map, int group) {
-                    if (lane == 0) {
+                int p1 = page_of(0), p2 = page_of(1);
+                if (values) skip(L);
+                for (int j = 0; j < n; ++j) {
+                    const int p3 = page_of(j + 2), group = group_of(j, p1);
+                    if (lane == 0 && ok) {
                         ok = mbar_wait(&empty[slot], (unsigned)ph, abort_flag, a.err);
                         if (ok) mbar_expect_tx(&full[slot], TILE);
                     }
                     ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-                    if (!ok) return;
+                    if (!ok) break;
                     if (lane < boxes) tma_load_4d(kv_s + slot * TILE + lane * BP * (D * 2), map, &full[slot], 0, 0, 0, group);
-                    ++n_asked;
+                    mine |= 1u << slot;
+                    phase = (phase & ~(1u << slot)) | (ph ? 0u : 1u << slot);
                     __syncwarp();
-                    if (++slot == NS) {
-                        slot = 0;
-                        ph ^= 1;
-                    }
-                };
-                int g0 = group_of(0), g1 = group_of(1), g2 = group_of(2);
-                ask(&map_k, g0);
-                if (ok && L == 2 && n > 1) ask(&map_k, g1);
-                for (int j = 0; j < n && ok; ++j) {
-                    const int g3 = group_of(j + 3);
-                    ask(&map_v, g0);
-                    if (ok && j + L < n) ask(&map_k, L == 1 ? g1 : g2);
-                    g0 = g1;
-                    g1 = g2;
-                    g2 = g3;
+                    p1 = p2;
+                    p2 = p3;
+                    // to the next one: K(j) has a tile of values before it from K(L) on, V(j) one of keys behind it up to V(n - L - 1)
+                    skip(values ? (j < n - L ? 2 : 1) : (j < L - 1 || j == n - 1 ? 1 : 2));
                 }
-                if (!ok || !ch_next<M, CT_KT>(a, w, n)) break;
+                if (!ok) break;
+                if (!values) skip(L);
+                if (!ch_next<M, CT_KT>(a, w, n)) break;
             }
-            if (lane == 0) *asked = n_asked;
+            if (lane == 0) {
+                armed[2 * values] = mine;
+                armed[2 * values + 1] = phase;
+            }
             if (bad) atomicOr(a.err, bad);
         } else if (warp == 9) {
             // the whole warp walks the steps (it meets the softmax warps at named barriers); one lane issues
@@ -256,25 +274,27 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                 if (!ch_next<M, CT_KT>(a, w, n)) break;
             }
         } else {
-            // queries, 64 threads: row (token, head) of an item's tile; rows beyond the item's are zeros
-            const int i0 = tid - 320;
+            // queries: every lane has four rows (token, head) of an item's tile; rows beyond the item's are zeros
             int nq = 0;
             bool ok = true;
             for (; ok;) {
-                const int n = ch_share(w), tiles = w.tile.rows > CT_M ? 2 : 1, s0 = a.q_start[w.r];
+                const int n = ch_share(w), tiles = w.tile.rows > CT_M ? 2 : 1;
                 for (int t = 0; t < tiles && ok; ++t, ++nq) {
                     if (lane == 0) ok = mbar_wait(&q_empty[nq & 1], (unsigned)(((nq >> 1) & 1) ^ 1), abort_flag, a.err);
                     ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
                     if (!ok) break;
-                    unsigned char* dst = q_s + (nq & 1) * TILE;
-                    for (int i = i0; i < CT_M * PC; i += 64) {
-                        const int row = i / PC, x = i % PC, at = t * CT_M + row;
+#pragma unroll
+                    for (int x4 = 0; x4 < 4; ++x4) {
+                        const int row = x4 * 32 + lane, at = t * CT_M + row;
                         const bool there = at < w.tile.rows;
-                        const int fl = w.tile.row0 + (there ? at : 0), tok = fl / a.G, g = fl - tok * a.G;
-                        const bf16* src = reinterpret_cast<const bf16*>(a.q) + (s0 + tok) * a.q_token + (long long)(w.kh * a.G + g) * a.q_head + x * 8;
+                        const int fl = w.tile.row0 + (there ? at : 0), tok = ch_over(fl, a.by_g), g = fl - tok * a.G;
+                        const bf16* src = reinterpret_cast<const bf16*>(a.q) + (w.s0 + tok) * a.q_token + (long long)(w.kh * a.G + g) * a.q_head;
                         // [halves of 64 columns][128 rows][128 bytes], 16-byte pieces permuted by row & 7
-                        const unsigned d = tc_smem(dst + (x >> 3) * 16384 + row * 128 + (((x & 7) ^ (row & 7)) << 4));
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(d), "l"(src), "r"(there ? 16 : 0));
+                        const unsigned d = tc_smem(q_s + (nq & 1) * TILE + row * 128);
+#pragma unroll
+                        for (int x = 0; x < PC; ++x)
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n"
+                                         ::"r"(d + (x >> 3) * 16384 + (((x & 7) ^ (row & 7)) << 4)), "l"(src + x * 8), "r"(there ? 16 : 0));
                     }
                     asm volatile("cp.async.wait_all;\n" ::: "memory");
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
@@ -298,11 +318,12 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             const bool pair = w.tile.rows > CT_M;
             const int at = pair ? t * CT_M + row : row;                // row of the item
             const bool live = at - lane < w.tile.rows;                 // any row of this warp
-            const int qpos = w.req.c + (w.tile.row0 + at) / a.G;
-            const int p_min = w.req.c + (w.tile.row0 + (pair ? t * CT_M : 0)) / a.G;
+            const int qpos = w.req.c + ch_over(w.tile.row0 + at, a.by_g);
+            const int p_min = w.req.c + ch_over(w.tile.row0 + (pair ? t * CT_M : 0), a.by_g);
             const int low = a.window > 0 ? qpos - a.window + 1 : 0, low_last = a.window > 0 ? w.req.c + w.tile.i1 - a.window + 1 : 0;
             float m_run = -INFINITY, l_run = 0.f;
             bool first = true;
+            if (lane == 0) walks[warp] = w;
             for (int j = pair ? 0 : t; j < n; j += pair ? 1 : 2, first = false) {
                 // (a warp that gave up still arrives for every step: the issuing warp waits there without a limit)
                 if (ok) {
@@ -383,6 +404,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                 asm volatile("bar.arrive %0, %1;\n" ::"r"(CT_BAR_P + t), "r"(CT_M + 32) : "memory");
             }
             // the item's end
+            __syncwarp();
+            w = walks[warp];
             if (!first) {
                 if (ok) {
                     if (lane == 0) ok = mbar_wait(&o_done[t], o_ph, abort_flag, a.err);
@@ -392,9 +415,9 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             }
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             const bool begins = w.k == 0, ends = w.k + n == w.tile.tiles, whole = begins && ends, there = ok && at < w.tile.rows;
-            const int fl = w.tile.row0 + at, tok = fl / a.G, h = w.kh * a.G + fl - tok * a.G;
+            const int fl = w.tile.row0 + at, tok = ch_over(fl, a.by_g), h = w.kh * a.G + fl - tok * a.G;
             const size_t place = ((size_t)2 * c + (begins ? 1 : 0)) * M + at;
-            bf16* dst = reinterpret_cast<bf16*>(a.out) + ((size_t)(a.q_start[w.r] + tok) * a.H + h) * D;
+            bf16* dst = reinterpret_cast<bf16*>(a.out) + ((size_t)(w.s0 + tok) * a.H + h) * D;
             float f0 = 1.f, f1 = 0.f;                                  // of this stream's outputs, of the other's
             if (!pair) {
                 // both streams have read the same rows: each puts together half of the columns
@@ -410,7 +433,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                 m_run = m;
             }
             if (live && ok) {
-                const float inv = !whole ? 1.f : l_run > 0.f ? 1.f / l_run : (l_run == 0.f ? 0.f : l_run);
+                const float inv = whole ? ch_inverse(l_run) : 1.f;
                 f0 *= inv;
                 f1 *= inv;
                 const int from = pair ? 0 : t * (D / 2), to = pair ? D : from + D / 2;
@@ -449,7 +472,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                 }
                 if (there && !whole && (pair || t == 0)) *reinterpret_cast<float2*>(a.part_ml + place * 2) = make_float2(m_run, l_run);
             }
-            if (begins && !ends && tid == 0) a.meta[c] = ok ? make_int4(w.r, w.kh, w.m, ch_parts(w, n, per)) : make_int4(0, 0, 0, 0);
+            if (begins && !ends && tid == 0 && ok) ch_leave(a, w, c, n);
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
             if (!pair) asm volatile("bar.sync %0, %1;\n" ::"r"(CT_BAR_MEET + 1), "r"(2 * CT_M) : "memory");      // both have read the outputs
             if (!ch_next<M, CT_KT>(a, w, n)) break;
@@ -458,7 +481,11 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
     __syncthreads();
-    if (*abort_flag && tid == 0) tc_drain(full, NS, *asked);
+    if (*abort_flag && tid < 2) {                   // copies that are still in flight are given a bounded time to land
+        for (int s = 0; s < NS; ++s)
+            if (armed[2 * tid] >> s & 1u)
+                for (unsigned i = 0; i < TC_DRAIN_LIMIT && !mbar_try_wait(&full[s], armed[2 * tid + 1] >> s & 1u); ++i) {}
+    }
     __syncthreads();
     if (warp == 9) {
         __syncwarp();
@@ -479,15 +506,16 @@ template <int D> static int launch_chunk_tc(const ChArgs& a, int C, cudaStream_t
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes);
     rc = (int)launch_pdl(kern, dim3(C), dim3(CT_THREADS), S::bytes, st, mk, mv, a, (int)(rows / 8));
     if (rc) return rc;
-    return (int)launch_pdl(chunk_join_kernel<bf16, S::M, D>, dim3(C, S::M * D / 4 / 256), dim3(256), 0, st, a);
+    return launch_chunk_join<bf16, S::M, D>(a, C, st);
 }
 
 // Scratch as for the other forms, with 256 rows an item and a block an SM.  Pages of 8 .. 128 keys that divide 128, or of a multiple of 128; up
 // to 2^31 - 1 groups of 8 rows in a pool.
-extern "C" int aie_attention_chunks_tc(const ChArgs* args, cudaStream_t stream) {
-    const ChArgs& a = *args;
-    if (a.R <= 0 || a.T <= 0) return 0;
-    if (a.W <= 0 || a.num_pages <= 0 || a.P <= 0 || a.K <= 0 || a.H % a.K) return AIE_BAD_ARG;
+extern "C" int aie_attention_chunks_tc(const ChCall* call, cudaStream_t stream) {
+    if (call->R <= 0 || call->T <= 0) return 0;
+    ChArgs a;
+    const int rc = ch_args(call, 128, CT_KT, &a);
+    if (rc) return rc;
     if (a.P % 8 || (CT_KT % a.P && a.P % CT_KT) || (long long)a.num_pages * a.K * a.P / 8 > 0x7ffffffe) return AIE_UNSUPPORTED;
     if (a.d == 64) return launch_chunk_tc<64>(a, aie_sm_count(), stream);
     if (a.d == 128) return launch_chunk_tc<128>(a, aie_sm_count(), stream);

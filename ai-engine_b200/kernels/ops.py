@@ -860,7 +860,7 @@ def paged_attention_chunks(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     launch, more, rows, an_sm, wide = chunk_form(q.dtype is torch.bfloat16, d, P, T * (H // K) / R, N * K * P // 8)
     blocks = an_sm * sm_count()
     parts = 2 * blocks * rows
-    scratch = torch.empty(parts * (wide + 2) + 4 * blocks, dtype=torch.float32, device=q.device)
+    scratch = torch.empty(parts * (wide + 2) + 8 * blocks, dtype=torch.float32, device=q.device)
     at = scratch.data_ptr()
     fields = (q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), q_start.data_ptr(), q_len.data_ptr(),
               ctx_len.data_ptr(), block_table.data_ptr(), at, at + 4 * parts * wide, at + 4 * parts * (wide + 2), by_token, by_head,
