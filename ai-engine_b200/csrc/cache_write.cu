@@ -9,6 +9,18 @@
 #define CW_THREADS 256
 #define CW_UNITS 4      // units of a thread under way
 
+// n / d for n < 2^31 by a multiplication (Granlund and Montgomery, 1994)
+struct CwDiv {
+    unsigned mul, shift;
+};
+static inline CwDiv cw_div(unsigned d) {
+    CwDiv v = {0u, 0u};
+    while ((1ull << v.shift) < d) ++v.shift;
+    v.mul = (unsigned)(((1ull << 32) * ((1ull << v.shift) - d)) / d + 1);
+    return v;
+}
+__device__ __forceinline__ unsigned cw_over(unsigned n, CwDiv d) { return (__umulhi(n, d.mul) + n) >> d.shift; }
+
 template <typename T, int V> struct CwVec { T e[V]; };
 
 // V consecutive elements: 16-byte accesses when V is 8, single ones when it is 1
@@ -25,36 +37,33 @@ template <typename I, typename C, int V>
 __global__ void __launch_bounds__(CW_THREADS)
 write_kv_slots_kernel(const I* __restrict__ k, const I* __restrict__ v, long long k_token, long long k_head, long long v_token,
                       long long v_head, C* __restrict__ k_pages, C* __restrict__ v_pages, const int* __restrict__ slots,
-                      long long total, int per_head, int per_plane, int per_token, int P, int K, int d, int n_slots, unsigned* err) {
+                      unsigned total, unsigned per_plane, CwDiv by_token, CwDiv by_head, CwDiv by_p, int P, int K, int d, int n_slots,
+                      unsigned* err) {
     pdl_launch_dependents();
     pdl_wait();
-    const long long first = (long long)blockIdx.x * (CW_THREADS * CW_UNITS) + threadIdx.x;
+    const unsigned first = blockIdx.x * (CW_THREADS * CW_UNITS) + threadIdx.x, per_head = d / V;
     alignas(16) CwVec<I, V> x[CW_UNITS];
-    int slot[CW_UNITS], unit[CW_UNITS];
+    int slot[CW_UNITS], head[CW_UNITS], at[CW_UNITS];      // head: K and more for values; at: element of the head
 #pragma unroll
     for (int u = 0; u < CW_UNITS; ++u) {
-        const long long i = first + u * CW_THREADS;
+        const unsigned i = first + u * CW_THREADS;
         slot[u] = -1;
-        unit[u] = 0;
         if (i < total) {
-            const long long t = i / per_token;
-            unit[u] = (int)(i - t * per_token);
-            const bool is_v = unit[u] >= per_plane;
-            const int w = is_v ? unit[u] - per_plane : unit[u];
-            const int h = w / per_head, e = (w - h * per_head) * V;
-            cw_load<I, V>(x[u], is_v ? v + t * v_token + h * v_head + e : k + t * k_token + h * k_head + e);
-            slot[u] = slots[t];
+            const unsigned t = cw_over(i, by_token), unit = i - t * (2 * per_plane), h = cw_over(unit, by_head);
+            head[u] = (int)h;
+            at[u] = (int)(unit - h * per_head) * V;
+            const bool is_v = (int)h >= K;
+            slot[u] = __ldg(slots + t);
+            cw_load<I, V>(x[u], is_v ? v + t * v_token + (long long)(h - K) * v_head + at[u] : k + t * k_token + (long long)h * k_head + at[u]);
         }
     }
 #pragma unroll
     for (int u = 0; u < CW_UNITS; ++u) {
         if (slot[u] < 0) continue;
         if (slot[u] >= n_slots) { atomicOr(err, AIE_DEV_PAGE_OOB); continue; }
-        const bool is_v = unit[u] >= per_plane;
-        const int w = is_v ? unit[u] - per_plane : unit[u];
-        const int h = w / per_head, e = (w - h * per_head) * V;
-        const int page = slot[u] / P;
-        C* to = (is_v ? v_pages : k_pages) + (((size_t)page * K + h) * P + (slot[u] - page * P)) * d + e;
+        const bool is_v = head[u] >= K;
+        const int page = (int)cw_over((unsigned)slot[u], by_p);
+        C* to = (is_v ? v_pages : k_pages) + (((size_t)page * K + (is_v ? head[u] - K : head[u])) * P + (slot[u] - page * P)) * d + at[u];
         if constexpr (V == 8) {
             alignas(16) CwVec<C, V> y;
 #pragma unroll
@@ -71,10 +80,11 @@ template <typename I, typename C, int V>
 static int launch_write(const void* k, const void* v, long long kt, long long kh, long long vt, long long vh, void* kp, void* vp,
                         const int* slots, int T, int num_pages, int P, int K, int d, unsigned* err, cudaStream_t st) {
     const long long total = (long long)T * 2 * K * (d / V);
-    const long long blocks = (total + CW_THREADS * CW_UNITS - 1) / (CW_THREADS * CW_UNITS);
-    if (blocks > 0x7fffffff) return -3;
-    return (int)launch_pdl(write_kv_slots_kernel<I, C, V>, dim3((unsigned)blocks), dim3(CW_THREADS), 0, st, (const I*)k, (const I*)v, kt, kh,
-                           vt, vh, (C*)kp, (C*)vp, slots, total, d / V, K * (d / V), 2 * K * (d / V), P, K, d, num_pages * P, err);
+    if (total > 0x7ffffc00) return -3;
+    const unsigned blocks = (unsigned)((total + CW_THREADS * CW_UNITS - 1) / (CW_THREADS * CW_UNITS)), per_plane = (unsigned)(K * (d / V));
+    return (int)launch_pdl(write_kv_slots_kernel<I, C, V>, dim3(blocks), dim3(CW_THREADS), 0, st, (const I*)k, (const I*)v, kt, kh, vt, vh,
+                           (C*)kp, (C*)vp, slots, (unsigned)total, per_plane, cw_div(2 * per_plane), cw_div((unsigned)(d / V)),
+                           cw_div((unsigned)P), P, K, d, num_pages * P, err);
 }
 
 template <typename I, typename C>

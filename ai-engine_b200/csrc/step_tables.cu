@@ -9,12 +9,13 @@
 // its pages from the end of the free list, the first of them free_pages[free_count - 1 - (upto[r] - need[r])].
 //
 // What bounds it: nothing but the launch and two rounds to memory for small steps, writing the table for large
-// ones.  So that one launch does it, every block adds up the lengths of all requests by itself (256 at a time;
+// ones.  So that one launch does it, every block adds up the lengths of all requests by itself (512 at a time;
 // 12 bytes a request out of L2) and keeps what its tokens and table rows ask of them in shared memory; then the
-// grid shares out the table, four entries a thread, and the tokens, which find their request by bisection.
+// grid shares out the table, a warp taking pieces of 512 entries of a row (four 16-byte loads a lane under way), and the
+// tokens, which find their request by bisection.
 #include "common.cuh"
 
-#define ST_THREADS 256
+#define ST_THREADS 512
 #define ST_MAX_REQUESTS 4096      // 16 bytes of shared memory each
 
 struct StRow {       // what a block keeps of a request
@@ -109,33 +110,43 @@ step_tables_kernel(const int* __restrict__ cached, const int* __restrict__ count
 
     if ((int)blockIdx.x < table_blocks) {
         // entry w of row r: what it held, then the pages it takes, then -1
-        constexpr int V = VEC ? 4 : 1;
-        const int wv = W / V;
-        const long long n = (long long)R * wv;
-        for (long long i = (long long)blockIdx.x * ST_THREADS + tid; i < n; i += (long long)table_blocks * ST_THREADS) {
-            const int r = (int)(i / wv), w = (int)(i - (long long)r * wv) * V;
+        constexpr int V = VEC ? 4 : 1, U = 4, PIECE = 32 * V * U;
+        const unsigned pieces = (W + PIECE - 1) / PIECE, tasks = R * pieces;
+        for (unsigned i = blockIdx.x * (ST_THREADS / 32) + warp; i < tasks; i += table_blocks * (ST_THREADS / 32)) {
+            const unsigned r = i / pieces;
+            const int w0 = (int)(i - r * pieces) * PIECE + lane * V;
             const StRow s = rows[r];
             const int now = s.now < 0 ? ~s.now : s.now;
-            int e[V];
-            if (VEC && w + V <= s.held) {
-                const int4 v = *reinterpret_cast<const int4*>(tables_in + (size_t)r * W + w);
-                e[0] = v.x;
-                e[V > 1 ? 1 : 0] = V > 1 ? v.y : v.x;
-                e[V > 2 ? 2 : 0] = V > 2 ? v.z : v.x;
-                e[V > 3 ? 3 : 0] = V > 3 ? v.w : v.x;
-            } else {
+            const int* from = tables_in + (size_t)r * W;
+            int* to = tables + (size_t)r * W;
+            int4 e[U];
 #pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    e[k] = -1;
-                    if (w + k < s.held) e[k] = tables_in[(size_t)r * W + w + k];
-                    else if (w + k < now) {
-                        e[k] = free_pages[s.first - (w + k - s.held)];
-                        if (e[k] < 0 || e[k] >= num_pages) bad |= AIE_DEV_PAGE_OOB;
-                    }
+            for (int u = 0; u < U; ++u) {
+                const int w = w0 + u * 32 * V;
+                e[u] = make_int4(-1, -1, -1, -1);
+                if (VEC ? w + V <= s.held : w < s.held) {
+                    if (VEC) e[u] = __ldg(reinterpret_cast<const int4*>(from + w));
+                    else e[u].x = __ldg(from + w);
                 }
             }
-            if (VEC) *reinterpret_cast<int4*>(tables + (size_t)r * W + w) = make_int4(e[0], e[V > 1 ? 1 : 0], e[V > 2 ? 2 : 0], e[V > 3 ? 3 : 0]);
-            else tables[(size_t)r * W + w] = e[0];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int w = w0 + u * 32 * V;
+                if (w >= W) continue;
+                if (w + V > s.held && w < now) {      // the rows' ends
+                    int* x = reinterpret_cast<int*>(&e[u]);
+#pragma unroll
+                    for (int k = 0; k < V; ++k) {
+                        if (w + k < s.held) x[k] = from[w + k];
+                        else if (w + k < now) {
+                            x[k] = free_pages[s.first - (w + k - s.held)];
+                            if (x[k] < 0 || x[k] >= num_pages) bad |= AIE_DEV_PAGE_OOB;
+                        }
+                    }
+                }
+                if (VEC) *reinterpret_cast<int4*>(to + w) = e[u];
+                else to[w] = e[u].x;
+            }
         }
     } else {
         const int stride = (gridDim.x - table_blocks) * ST_THREADS;
@@ -184,8 +195,8 @@ extern "C" int aie_step_tables(const StArgs* args, cudaStream_t stream) {
         *slots = token_req + capacity;
     const bool vec = W % 4 == 0 && ((size_t)a.tables_in | (size_t)a.out) % 16 == 0;
     const int most = 2 * aie_sm_count();
-    const long long entries = (long long)R * (vec ? W / 4 : W);
-    const long long tb = (entries + ST_THREADS - 1) / ST_THREADS, kb = (capacity + ST_THREADS - 1) / ST_THREADS;
+    const int piece = vec ? 512 : 128, warps = ST_THREADS / 32;
+    const long long tb = ((long long)R * ((W + piece - 1) / piece) + warps - 1) / warps, kb = (capacity + ST_THREADS - 1) / ST_THREADS;
     const int table_blocks = (int)(tb < most ? tb : most), token_blocks = (int)(kb < most ? kb : most);
     auto kern = vec ? step_tables_kernel<true> : step_tables_kernel<false>;
     const size_t smem = (size_t)R * sizeof(StRow);

@@ -12,8 +12,9 @@
 //
 // What bounds it: one row of p and one of q a request.  A cluster of eight blocks shares a request's row: every warp adds up
 // segments of 512 tokens (eight 16-byte loads a lane under way), the segments' sums stay in shared memory, the blocks' sums meet
-// through the cluster's, and the block that holds the wanted one looks for its segment and reads that once more.  Eight
-// blocks because a row of 128,256 floats twice is 128 KB for each, about 2 us of what an SM can load.
+// in everyone's shared memory, and the block that holds the wanted one looks for its segment and reads that once more.  Eight
+// blocks because a row of 128,256 floats twice is 128 KB for each, about 2 us of what an SM can load; of 256 threads and 64
+// registers, so that four fit an SM and 64 requests' clusters are all there at once.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -21,10 +22,13 @@
 namespace cg = cooperative_groups;
 typedef unsigned long long u64;
 
-#define VD_THREADS 512
+#define VD_THREADS 256
 #define VD_CLUSTER 8
 #define VD_SEGMENT 512          // tokens a warp adds up at a time: four of 16 bytes a lane, of each row
 #define VD_MAX_SEGMENTS 256     // a block's: 1,048,576 tokens of vocabulary
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory"); }
 
 // in units of 2^-48; NaN and what is negative weigh nothing
 __device__ __forceinline__ u64 vd_fixed(float w) { return w > 0.f ? __float2ull_rn(fminf(w, 1.f) * 281474976710656.f) : 0ull; }
@@ -69,22 +73,31 @@ template <bool VEC> __device__ __forceinline__ void vd_segment(u64 (&w)[4][4], c
 }
 
 template <bool VEC>
-__global__ void __cluster_dims__(VD_CLUSTER, 1, 1) __launch_bounds__(VD_THREADS)
+__global__ void __cluster_dims__(VD_CLUSTER, 1, 1) __launch_bounds__(VD_THREADS, 4)
 verify_drafts_kernel(const float* __restrict__ target, long long target_row, int T, int V, const int* __restrict__ q_start,
                      const int* __restrict__ draft_tokens, const int* __restrict__ draft_len, const float* __restrict__ draft_probs,
                      long long draft_req, long long draft_place, int N, const float* __restrict__ accept_draws,
                      const float* __restrict__ token_draws, int* __restrict__ tokens, int* __restrict__ emitted, unsigned* err) {
     __shared__ u64 seg_sum[VD_MAX_SEGMENTS];
     __shared__ u64 warp_sum[VD_THREADS / 32];
-    __shared__ u64 block_sum[2];            // of w, of p alone
+    __shared__ u64 sums[2][VD_CLUSTER];     // of every block: of w, of p alone
     __shared__ int s_kept;
     cg::cluster_group cluster = cg::this_cluster();
     pdl_launch_dependents();
     pdl_wait();
+    cluster_arrive();                       // (waited for before the first write to another block's memory: that it has started)
     const int r = blockIdx.x / VD_CLUSTER, rank = blockIdx.x % VD_CLUSTER;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // what the first decision needs, all asked for at once
     const int start = q_start[r];
-    int n = draft_len ? draft_len[r] : N;
+    const int n = draft_len ? draft_len[r] : N;
+    int x0 = 0;
+    float u0 = 0.f;
+    if (warp == 0 && lane < N) {
+        x0 = draft_tokens[(size_t)r * N + lane];
+        u0 = accept_draws[(size_t)r * N + lane];
+    }
+    const float v0 = token_draws[r];
     int* out = tokens + (size_t)r * (N + 1);
     const bool bad = n > N || (n >= 0 && (start < 0 || start > T - 1 - n));
     if (n < 0 || bad) {                     // an idle request, or rows that are not there: the same in all blocks of the cluster
@@ -95,6 +108,7 @@ verify_drafts_kernel(const float* __restrict__ target, long long target_row, int
                 if (bad) atomicOr(err, AIE_DEV_SLOT_OOB);
             }
         }
+        cluster_wait();
         return;
     }
 
@@ -104,13 +118,16 @@ verify_drafts_kernel(const float* __restrict__ target, long long target_row, int
         for (int base = 0; base < n; base += 32) {
             const int i = base + lane;
             bool refused = false;
+            if (base > 0 && i < n) {
+                x0 = draft_tokens[(size_t)r * N + i];
+                u0 = accept_draws[(size_t)r * N + i];
+            }
             if (i < n) {
-                const int x = draft_tokens[(size_t)r * N + i];
                 refused = true;
-                if (x >= 0 && x < V) {
-                    const float p = target[(start + i) * target_row + x];
-                    const float q = draft_probs ? draft_probs[r * draft_req + i * draft_place + x] : 1.f;
-                    refused = !((double)accept_draws[(size_t)r * N + i] * (double)q < (double)p);
+                if (x0 >= 0 && x0 < V) {
+                    const float p = target[(start + i) * target_row + x0];
+                    const float q = draft_probs ? draft_probs[r * draft_req + i * draft_place + x0] : 1.f;
+                    refused = !((double)u0 * (double)q < (double)p);
                 } else if (rank == 0) {
                     atomicOr(err, AIE_DEV_TOKEN_OOB);
                 }
@@ -146,15 +163,18 @@ verify_drafts_kernel(const float* __restrict__ target, long long target_row, int
         }
         if (lane == 0) warp_sum[warp] = sum;
         __syncthreads();
-        if (tid == 0) {
+        if (round == 0) cluster_wait();
+        if (tid < VD_CLUSTER) {                    // to block `tid`
             u64 a = 0;
+#pragma unroll
             for (int w = 0; w < VD_THREADS / 32; ++w) a += warp_sum[w];
-            block_sum[round] = a;
+            *cluster.map_shared_rank(&sums[round][rank], tid) = a;
         }
         cluster.sync();
         before = total = 0;
+#pragma unroll
         for (int b = 0; b < VD_CLUSTER; ++b) {
-            const u64 a = *cluster.map_shared_rank(&block_sum[round], b);
+            const u64 a = sums[round][b];
             if (b < rank) before += a;
             total += a;
         }
@@ -176,10 +196,10 @@ verify_drafts_kernel(const float* __restrict__ target, long long target_row, int
     }
     if (total > 0) {
         // total is below 2^53 for anything that sums to about 1, so the product is rounded once
-        const double v = (double)token_draws[r];
+        const double v = (double)v0;
         u64 goal = v > 0.0 ? (u64)(v * (double)total) : 0ull;
         if (goal > total - 1) goal = total - 1;
-        const u64 here = block_sum[round];
+        const u64 here = sums[round][rank];
         if (warp == 0 && goal >= before && goal - before < here) {
             goal -= before;
             int s = 0;                             // the segment: 32 sums at a time
@@ -227,7 +247,6 @@ verify_drafts_kernel(const float* __restrict__ target, long long target_row, int
             }
         }
     }
-    cluster.sync();      // a block's sums are read by the others until here
 }
 
 struct VdArgs {                       // what a caller packs, in this order
