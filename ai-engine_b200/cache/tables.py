@@ -9,11 +9,7 @@ from typing import NamedTuple
 
 import torch
 
-from ..kernels.loader import KernelError
-from ..kernels.ops import Launcher, check_operands
-from ..kernels.profile import region
-
-MAX_REQUESTS = 4096      # of one call: a block keeps 16 bytes of each
+from ..kernels.ops import _nb, draft_call
 
 
 class StepTables(NamedTuple):
@@ -34,29 +30,9 @@ def step_tables(cached: torch.Tensor, counts: torch.Tensor, held: torch.Tensor, 
     free.  In the order of the requests, each takes the pages it is short of from the end of the free list; one that cannot have
     all of them has to wait (it takes none, its tokens' slots are -1, its q_len is 0), and so has every later one that is
     short of pages.  Pages held beyond the tokens (drafts that were refused) are used first.  Nothing that is given is changed: the
-    next step passes the outputs on.  Sizes: R up to MAX_REQUESTS; max_tokens bounds the sum of the counts.
+    next step passes the outputs on.  Sizes: R up to 4,096; max_tokens bounds the sum of the counts.
 
     A request whose lengths are negative, do not fit the table's width or bring tokens past max_tokens waits and sets the error
     word; a page outside the pool sets it too and makes no slot."""
-    if tables.dim() != 2 or tables.shape[1] == 0:
-        raise KernelError("step_tables: the tables must be [requests, pages]")
-    R, W = tables.shape
-    if not 0 < R <= MAX_REQUESTS:
-        raise KernelError(f"step_tables: {R} requests (1 to {MAX_REQUESTS} are taken)")
-    F = free_pages.numel()
-    if page_size < 1 or num_pages < 0 or num_pages * page_size > 0x7fffffff:
-        raise KernelError(f"step_tables: {num_pages} pages of {page_size} tokens (1 to 2^31 - 1 cache slots are taken)")
-    if not 0 <= max_tokens <= 1 << 30 or R * W > 1 << 30:
-        raise KernelError("step_tables: sizes beyond 2^30")
-    each = (R,)
-    stream = check_operands("step_tables", (("cached", cached, each), ("counts", counts, each), ("held", held, each), ("tables", tables, (R, W)),
-                                            ("free_pages", free_pages, (F,)), ("free_count", free_count, (1,)), ("err", err, (1,))))
-    out = torch.empty(R * W + 3 * R + 1 + 3 * max_tokens, dtype=torch.int32, device=tables.device)
-    with region("step_tables", 4 * (2 * R * W + 6 * R + 3 * max_tokens)):
-        _TABLES((cached.data_ptr(), counts.data_ptr(), held.data_ptr(), tables.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
-                 out.data_ptr(), err.data_ptr(), R, W, F, page_size, num_pages, max_tokens), stream)
-    made, *rest = out.split_with_sizes((R * W, R, 1, R, R, max_tokens, max_tokens, max_tokens))
-    return StepTables(made.view(R, W), *rest)
-
-
-_TABLES = Launcher("step_tables.cu", "aie_step_tables", "8P6i")
+    return StepTables(*draft_call("step_tables", 1, 2 * _nb(tables), cached, counts, held, tables, free_pages, free_count, page_size,
+                                  num_pages, max_tokens, err))

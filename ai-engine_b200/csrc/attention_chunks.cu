@@ -287,7 +287,8 @@ __global__ void __launch_bounds__(CB_WARPS * 32, 2) chunk_bf16_kernel(const ChAr
 template <int D, int MT> static int launch_chunk_bf16(const ChArgs& a, int C, cudaStream_t st) {
     using S = CbShape<D, MT>;
     auto kern = chunk_bf16_kernel<D, MT>;
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes);
+    static unsigned long long done = 0;
+    ch_prepare(kern, S::bytes, &done);
     const int rc = (int)launch_pdl(kern, dim3(C), dim3(CB_WARPS * 32), S::bytes, st, a);
     if (rc) return rc;
     return launch_chunk_join<bf16, S::M, D>(a, C, st);

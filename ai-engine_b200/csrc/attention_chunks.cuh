@@ -252,10 +252,19 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const ChArgs a) {
                   make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
     }
 }
+// What a kernel is told once on each device: the shared memory it takes (0: none), and that it wants as much of it an SM as there is.
+template <typename F> static void ch_prepare(F kern, int bytes, unsigned long long* done) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && dev < 64 && (*done >> dev & 1)) return;
+    if (bytes) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (dev < 64) *done |= 1ull << dev;
+}
 // ... with as much shared memory an SM as the kernel before it, which would otherwise have to leave the SM before it changes
 template <typename T, int M, int D> static int launch_chunk_join(const ChArgs& a, int C, cudaStream_t st) {
     auto kern = chunk_join_kernel<T, M, D>;
-    cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    static unsigned long long done = 0;
+    ch_prepare(kern, 0, &done);
     constexpr int blocks = M * D / 4 / 256;
     return (int)launch_pdl(kern, dim3(C, blocks > 8 ? 8 : blocks), dim3(256), 0, st, a);
 }

@@ -3,7 +3,7 @@
 //   o = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m),   x_j = (q . k_j) * scale * log2 e,   keys j <= position (and > position - window)
 //
 // A block has NW warps; of every key tile each warp takes eight keys of its own and keeps a running maximum, sum and output of all M rows
-// for them, so that warps meet only at an item's end.  A warp's keys and values come through a ring of its own (cp.async, three stages).
+// for them, so that warps meet only at an item's end.  The loop over key tiles exists for 8, 16, 24 and 32 rows.  A warp's keys and values come through a ring of its own (cp.async, three stages).
 // Scores: a lane has one key and every fourth row, products and sums two at a time (fma.rn.f32x2) along the head; outputs: a lane has
 // D / 32 columns of all rows.  Operands are 16-byte reads of shared memory, most of them the same for many lanes:
 // at 32 rows and heads of 128, 9 reads a step of 32 multiply-adds for the scores and 12 for 128 for the outputs.
@@ -31,6 +31,8 @@ __device__ __forceinline__ float2 cf_both(u64 v) {
     asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
     return f;
 }
+
+template <int N> struct CfInt { static constexpr int value = N; };
 
 template <int D> struct CfShape {
     static constexpr int M = D > 128 ? 16 : 32;      // rows of an item: M * D / 32 floats of output a lane
@@ -78,7 +80,6 @@ __global__ void __launch_bounds__(CfShape<D>::NW * 32) chunk_f32_kernel(const Ch
         const int n = ch_share(w);
         const ChTile tl = w.tile;
         const int c0 = w.req.c, s0 = w.s0, hi = c0 + tl.i1 + 1;
-        const int jn = (tl.rows + 3) >> 2;        // fours of rows that are there
         // queries of the item
         for (int i = tid; i < M * CH; i += NW * 32) {
             const int row = i / CH, ch = i - row * CH, e = ch * 4;
@@ -117,9 +118,16 @@ __global__ void __launch_bounds__(CfShape<D>::NW * 32) chunk_f32_kernel(const Ch
         };
 
         float m_run[RJ], l_run[RJ];
+        int lim[RJ], low[RJ];                     // a row sees the keys from low + 1 to lim
         u64 o[M][CP];
 #pragma unroll
-        for (int j = 0; j < RJ; ++j) { m_run[j] = -INFINITY; l_run[j] = 0.f; }
+        for (int j = 0; j < RJ; ++j) {
+            m_run[j] = -INFINITY;
+            l_run[j] = 0.f;
+            const int row = j * 4 + rg, pos = c0 + ch_over(tl.row0 + row, a.by_g);
+            lim[j] = row < tl.rows ? pos : -1;
+            low[j] = a.window > 0 ? pos - a.window : -1;
+        }
 #pragma unroll
         for (int i = 0; i < M; ++i)
 #pragma unroll
@@ -127,88 +135,98 @@ __global__ void __launch_bounds__(CfShape<D>::NW * 32) chunk_f32_kernel(const Ch
 
 #pragma unroll
         for (int i = 0; i < NST - 1; ++i) issue(i);
-        for (int i = 0; i < n; ++i) {
-            issue(i + NST - 1);
-            asm volatile("cp.async.wait_group %0;\n" ::"n"(NST - 1));
-            __syncwarp();
-            const float* ks = ring + (i % NST) * S::stage;
-            const float* vs = ks + 8 * D;
-            u64 s2[RJ];
+        // fours of rows that are there, rounded up to eights: a loop for each number, without branches between its loads
+        auto walk = [&](auto fours) {
+            constexpr int JN = decltype(fours)::value;
+            for (int i = 0; i < n; ++i) {
+                issue(i + NST - 1);
+                asm volatile("cp.async.wait_group %0;\n" ::"n"(NST - 1));
+                __syncwarp();
+                const float* ks = ring + (i % NST) * S::stage;
+                const float* vs = ks + 8 * D;
+                u64 s2[JN];
 #pragma unroll
-            for (int j = 0; j < RJ; ++j) s2[j] = 0ull;
+                for (int j = 0; j < JN; ++j) s2[j] = 0ull;
 #pragma unroll 4
-            for (int ch = 0; ch < CH; ++ch) {
-                const ulonglong2 k2 = *reinterpret_cast<const ulonglong2*>(ks + key * D + ((ch ^ key) << 2));
+                for (int ch = 0; ch < CH; ++ch) {
+                    const ulonglong2 k2 = *reinterpret_cast<const ulonglong2*>(ks + key * D + ((ch ^ key) << 2));
 #pragma unroll
-                for (int j = 0; j < RJ; ++j)
-                    if (j < jn) {
-                        const int row = j * 4 + rg;
-                        const ulonglong2 q2 = *reinterpret_cast<const ulonglong2*>(q_s + row * D + ((ch ^ (row & 7)) << 2));
-                        s2[j] = cf_fma2(k2.x, q2.x, s2[j]);
-                        s2[j] = cf_fma2(k2.y, q2.y, s2[j]);
-                    }
-            }
-            const int k_at = (kt0 + i) * KT + warp * 8 + key;
-            float corr[RJ];
-            bool moved = false;
+                    for (int j = 0; j < JN; ++j) {
+                            const int row = j * 4 + rg;
+                            const ulonglong2 q2 = *reinterpret_cast<const ulonglong2*>(q_s + row * D + ((ch ^ (row & 7)) << 2));
+                            s2[j] = cf_fma2(k2.x, q2.x, s2[j]);
+                            s2[j] = cf_fma2(k2.y, q2.y, s2[j]);
+                        }
+                }
+                const int k_at = (kt0 + i) * KT + warp * 8 + key;
+                float top[JN];
 #pragma unroll
-            for (int j = 0; j < RJ; ++j) {
-                corr[j] = 1.f;
-                if (j < jn) {
+                for (int j = 0; j < JN; ++j) {
                     const float2 f = cf_both(s2[j]);
-                    const int row = j * 4 + rg, pos = c0 + ch_over(tl.row0 + row, a.by_g);
-                    const bool sees = row < tl.rows && k_at <= pos && (a.window <= 0 || k_at > pos - a.window);
-                    const float x = sees ? (f.x + f.y) * a.scale2 : -INFINITY;
-                    float top = x;
+                    top[j] = k_at <= lim[j] && k_at > low[j] ? (f.x + f.y) * a.scale2 : -INFINITY;
+                    s2[j] = cf_pack(top[j], 0.f);
+                }
 #pragma unroll
-                    for (int b = 1; b < 8; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
-                    const float m_new = fmaxf(m_run[j], top), m_use = m_new == -INFINITY ? 0.f : m_new;
-                    const float p = sees ? exp2f(x - m_use) : 0.f;
-                    corr[j] = m_run[j] == m_new ? 1.f : exp2f(m_run[j] - m_use);
-                    moved |= corr[j] != 1.f;
-                    m_run[j] = m_new;
+                for (int b = 1; b < 8; b <<= 1)
+#pragma unroll
+                    for (int j = 0; j < JN; ++j) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], b));
+                float corr[JN];
+                bool moved = false;
+#pragma unroll
+                for (int j = 0; j < JN; ++j) {
+                    // the reference moves by more than 8 or not at all: weights stay below 2^8, outputs are rarely rescaled
+                    corr[j] = 1.f;
+                    if (top[j] > m_run[j] + 8.f) {
+                        corr[j] = m_run[j] == -INFINITY ? 0.f : exp2f(m_run[j] - top[j]);
+                        m_run[j] = top[j];
+                        moved = true;
+                    }
+                    const float x = cf_both(s2[j]).x, p = x == -INFINITY ? 0.f : exp2f(x - m_run[j]);
                     l_run[j] = l_run[j] * corr[j] + p;          // of this lane's keys
-                    p_s[key * M + row] = p;
+                    p_s[key * M + j * 4 + rg] = p;
                 }
-            }
-            if (__any_sync(0xffffffffu, moved)) {
+                if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-                for (int i2 = 0; i2 < M; ++i2) {
-                    const float f = __shfl_sync(0xffffffffu, corr[i2 >> 2], (i2 & 3) * 8);
-                    const u64 ff = cf_pack(f, f);
+                    for (int i2 = 0; i2 < 4 * JN; ++i2) {
+                        const float f = __shfl_sync(0xffffffffu, corr[i2 >> 2], (i2 & 3) * 8);
+                        const u64 ff = cf_pack(f, f);
 #pragma unroll
-                    for (int x = 0; x < CP; ++x) o[i2][x] = cf_mul2(o[i2][x], ff);
-                }
-            }
-            __syncwarp();
-#pragma unroll 2
-            for (int kk = 0; kk < 8; ++kk) {
-                u64 v2[CP];
-                if constexpr (CP == 1) {
-                    v2[0] = *reinterpret_cast<const u64*>(vs + kk * D + (((lane >> 1) ^ kk) << 2) + (lane & 1) * 2);
-                } else {
-#pragma unroll
-                    for (int x = 0; x < CP / 2; ++x) {
-                        const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(vs + kk * D + (((lane + 32 * x) ^ kk) << 2));
-                        v2[2 * x] = t.x;
-                        v2[2 * x + 1] = t.y;
+                        for (int x = 0; x < CP; ++x) o[i2][x] = cf_mul2(o[i2][x], ff);
                     }
                 }
+                __syncwarp();
+#pragma unroll 2
+                for (int kk = 0; kk < 8; ++kk) {
+                    u64 v2[CP];
+                    if constexpr (CP == 1) {
+                        v2[0] = *reinterpret_cast<const u64*>(vs + kk * D + (((lane >> 1) ^ kk) << 2) + (lane & 1) * 2);
+                    } else {
 #pragma unroll
-                for (int j = 0; j < RJ; ++j)
-                    if (j < jn) {
-                        const float4 p4 = *reinterpret_cast<const float4*>(p_s + kk * M + j * 4);
-                        const float p[4] = {p4.x, p4.y, p4.z, p4.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const u64 pp = cf_pack(p[e], p[e]);
-#pragma unroll
-                            for (int x = 0; x < CP; ++x) o[j * 4 + e][x] = cf_fma2(pp, v2[x], o[j * 4 + e][x]);
+                        for (int x = 0; x < CP / 2; ++x) {
+                            const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(vs + kk * D + (((lane + 32 * x) ^ kk) << 2));
+                            v2[2 * x] = t.x;
+                            v2[2 * x + 1] = t.y;
                         }
                     }
+#pragma unroll
+                    for (int j = 0; j < JN; ++j) {
+                            const float4 p4 = *reinterpret_cast<const float4*>(p_s + kk * M + j * 4);
+                            const float p[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const u64 pp = cf_pack(p[e], p[e]);
+#pragma unroll
+                                for (int x = 0; x < CP; ++x) o[j * 4 + e][x] = cf_fma2(pp, v2[x], o[j * 4 + e][x]);
+                            }
+                        }
+                }
+                __syncwarp();
             }
-            __syncwarp();
-        }
+        };
+        if (tl.rows <= 8) walk(CfInt<2>());
+        else if (tl.rows <= 16 || RJ == 4) walk(CfInt<4>());
+        else if (tl.rows <= 24) walk(CfInt<RJ < 6 ? RJ : 6>());
+        else walk(CfInt<RJ>());
         asm volatile("cp.async.wait_group 0;\n" ::);
 
         // the warps meet: every row's maximum, then outputs and sums
@@ -272,7 +290,8 @@ __global__ void __launch_bounds__(CfShape<D>::NW * 32) chunk_f32_kernel(const Ch
 template <typename T, int D> static int launch_chunk_f32(const ChArgs& a, int C, cudaStream_t st) {
     using S = CfShape<D>;
     auto kern = chunk_f32_kernel<T, D>;
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes);
+    static unsigned long long done = 0;
+    ch_prepare(kern, S::bytes, &done);
     const int rc = (int)launch_pdl(kern, dim3(C), dim3(S::NW * 32), S::bytes, st, a);
     if (rc) return rc;
     return launch_chunk_join<T, S::M, D>(a, C, st);

@@ -503,7 +503,8 @@ template <int D> static int launch_chunk_tc(const ChArgs& a, int C, cudaStream_t
     if (rc == 0) rc = tc_make_map_rows8(&mv, a.v_pages, rows, D / 64, box);
     if (rc) return rc;
     auto kern = chunk_tc_kernel<D>;
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes);
+    static unsigned long long done = 0;
+    ch_prepare(kern, S::bytes, &done);
     rc = (int)launch_pdl(kern, dim3(C), dim3(CT_THREADS), S::bytes, st, mk, mv, a, (int)(rows / 8));
     if (rc) return rc;
     return launch_chunk_join<bf16, S::M, D>(a, C, st);

@@ -151,11 +151,41 @@ def host_module_path() -> str:
     return _build(target, [cxx], srcs, deps, flags, "csrc/host (cache manager, scheduler)")
 
 
+def draft_module_path() -> str:
+    """Path of the extension module of csrc/host/draft_ops.cpp, compiled against the installed torch."""
+    import torch
+
+    folder = os.path.join(CSRC, "host")
+    src = os.path.join(folder, "draft_ops.cpp")
+    root = os.path.dirname(os.path.abspath(torch.__file__))
+    cuda = os.path.dirname(os.path.dirname(find_nvcc()))
+    flags = CXX_FLAGS + [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
+    places = [f"-I{p}" for p in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                                 os.path.join(cuda, "include"), sysconfig.get_paths()["include"])]
+    lib = os.path.join(root, "lib")
+    libs = [f"-L{lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", f"-Wl,-rpath,{lib}"]
+    key = _hash([src], flags + [torch.__version__, sysconfig.get_config_var("SOABI") or sys.version])
+    target = os.path.join(build_dir(), f"_aie_draft_ops-{key}.so")
+    if os.path.exists(target):
+        return target
+    cxx = os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++")
+    if not cxx:
+        raise BuildError("no C++ compiler found (g++): the host side of the draft operators cannot be built")
+    return _build(target, [cxx], [src] + libs, [src], flags + places, "csrc/host/draft_ops.cpp")
+
+
 def load_host_module():
+    return _import("_aie_host", host_module_path())
+
+
+def load_draft_module():
+    return _import("_aie_draft_ops", draft_module_path())
+
+
+def _import(name: str, path: str):
     import importlib.util
 
-    path = host_module_path()
-    spec = importlib.util.spec_from_file_location("_aie_host", path)
+    spec = importlib.util.spec_from_file_location(name, path)
     mod = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(mod)
     return mod
@@ -163,7 +193,7 @@ def load_host_module():
 
 def build_all() -> List[str]:
     """Compile everything (used by the build check); returns the library paths."""
-    out = [host_module_path()]
+    out = [host_module_path(), draft_module_path()]
     for s in CUDA_SOURCES:
         if os.path.exists(os.path.join(CSRC, s)):
             out.append(cuda_library(s))

@@ -28,7 +28,7 @@ struct StRow {       // what a block keeps of a request
 __device__ __forceinline__ long long st_shfl_up(long long v, int o) { return __shfl_up_sync(0xffffffffu, v, o); }
 
 template <bool VEC>
-__global__ void __launch_bounds__(ST_THREADS)
+__global__ void __launch_bounds__(ST_THREADS, 2)
 step_tables_kernel(const int* __restrict__ cached, const int* __restrict__ counts, const int* __restrict__ held_in,
                    const int* __restrict__ tables_in, const int* __restrict__ free_pages, const int* __restrict__ free_count, int R, int W,
                    int F, int P, int num_pages, int capacity, int table_blocks, int* __restrict__ tables, int* __restrict__ held,

@@ -13,8 +13,9 @@
 // What bounds it: one row of p and one of q a request.  A cluster of eight blocks shares a request's row: every warp adds up
 // segments of 512 tokens (eight 16-byte loads a lane under way), the segments' sums stay in shared memory, the blocks' sums meet
 // in everyone's shared memory, and the block that holds the wanted one looks for its segment and reads that once more.  Eight
-// blocks because a row of 128,256 floats twice is 128 KB for each, about 2 us of what an SM can load; of 256 threads and 64
-// registers, so that four fit an SM and 64 requests' clusters are all there at once.
+// blocks because a row of 128,256 floats twice is 128 KB for each, about 2 us of what an SM can load.  At 64 registers a thread an SM
+// holds one block of 1,024 threads or four of 256: up to 16 requests (two clusters of eight fit each of eight groups of SMs) take
+// 1,024, which read their part of a row in one go, 17 to 32 take 512, more take 256, whose clusters are then all there at once.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -22,7 +23,6 @@
 namespace cg = cooperative_groups;
 typedef unsigned long long u64;
 
-#define VD_THREADS 256
 #define VD_CLUSTER 8
 #define VD_SEGMENT 512          // tokens a warp adds up at a time: four of 16 bytes a lane, of each row
 #define VD_MAX_SEGMENTS 256     // a block's: 1,048,576 tokens of vocabulary
@@ -72,8 +72,8 @@ template <bool VEC> __device__ __forceinline__ void vd_segment(u64 (&w)[4][4], c
         }
 }
 
-template <bool VEC>
-__global__ void __cluster_dims__(VD_CLUSTER, 1, 1) __launch_bounds__(VD_THREADS, 4)
+template <bool VEC, int VD_THREADS>
+__global__ void __cluster_dims__(VD_CLUSTER, 1, 1) __launch_bounds__(VD_THREADS, 1024 / VD_THREADS)
 verify_drafts_kernel(const float* __restrict__ target, long long target_row, int T, int V, const int* __restrict__ q_start,
                      const int* __restrict__ draft_tokens, const int* __restrict__ draft_len, const float* __restrict__ draft_probs,
                      long long draft_req, long long draft_place, int N, const float* __restrict__ accept_draws,
@@ -266,7 +266,11 @@ extern "C" int aie_verify_drafts(const VdArgs* args, cudaStream_t stream) {
     if (a.V <= 0 || a.N < 0 || a.T < 0) return AIE_BAD_ARG;
     if (a.V > VD_CLUSTER * VD_MAX_SEGMENTS * VD_SEGMENT || a.R > 0x7fffffff / VD_CLUSTER) return -3;
     const bool vec = ((size_t)a.target | (size_t)a.draft_probs) % 16 == 0 && (a.target_row | a.draft_req | a.draft_place) % 4 == 0;
-    return (int)launch_pdl(vec ? verify_drafts_kernel<true> : verify_drafts_kernel<false>, dim3(a.R * VD_CLUSTER), dim3(VD_THREADS), 0, stream,
+    const int threads = a.R <= 16 ? 1024 : a.R <= 32 ? 512 : 256;
+    auto kern = threads == 1024 ? (vec ? verify_drafts_kernel<true, 1024> : verify_drafts_kernel<false, 1024>)
+                : threads == 512 ? (vec ? verify_drafts_kernel<true, 512> : verify_drafts_kernel<false, 512>)
+                                 : (vec ? verify_drafts_kernel<true, 256> : verify_drafts_kernel<false, 256>);
+    return (int)launch_pdl(kern, dim3(a.R * VD_CLUSTER), dim3(threads), 0, stream,
                            a.target, a.target_row, a.T, a.V, a.q_start, a.draft_tokens, a.draft_len, a.draft_probs, a.draft_req,
                            a.draft_place, a.N, a.accept_draws, a.token_draws, a.tokens, a.emitted, a.err);
 }

@@ -6,14 +6,14 @@ from __future__ import annotations
 
 import math
 import os
-import struct
-from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
+from ctypes import c_float, c_int, c_longlong, c_void_p, cast as cast_pointer
 from typing import Optional
 
 import numpy as np
 import torch
 
-from .loader import KernelError, check, library, require_cuda
+from ..csrc import build
+from .loader import LAUNCHES, KernelError, KernelUnavailable, check, library, require_cuda
 from .profile import enabled as _profiling, region
 
 F32, BF16 = 0, 1
@@ -719,55 +719,39 @@ def paged_attention(q, k_pages, v_pages, ctx, work, block_table, scale: float, w
 
 # ---------------------------------------------------------------------------
 # steps whose lengths the device alone knows (drafted tokens and their verification)
-class Launcher:
-    """A launcher of csrc/<source> that takes one packed struct of arguments, then plain integers: packing and one call of three
-    arguments take 2 us of the host's time, a call of twenty arguments 5.  `layout`: the struct's fields in the order of the C
-    declaration, as the struct module names them (native sizes and alignment)."""
-
-    def __init__(self, source: str, name: str, layout: str, ints: int = 0):
-        self.source, self.name, self.pack = source, name, struct.Struct("@" + layout).pack
-        self.argtypes = [c_char_p] + [c_int] * ints + [c_void_p]
-        self.fn = None
-
-    def __call__(self, fields: tuple, stream: int, *ints: int) -> None:
-        if self.fn is None:
-            self.fn = getattr(library(self.source), self.name)
-            self.fn.argtypes = self.argtypes
-        check(self.fn(self.pack(*fields), *ints, stream), self.name[4:])
+_DRAFT_SOURCES = {"aie_step_tables": "step_tables.cu", "aie_write_kv_slots": "cache_write.cu", "aie_verify_drafts": "verify_drafts.cu",
+                  "aie_attention_chunks_f32": "attention_chunks_f32.cu", "aie_attention_chunks_bf16": "attention_chunks.cu",
+                  "aie_attention_chunks_tc": "attention_chunks_tc.cu"}
+_DRAFT = [None]
 
 
-def check_operands(what: str, ints, others=()) -> int:
-    """The current device's stream as a number, for operands that live on that device.  `ints`: (name, tensor, shape) of index arrays, which
-    have to be contiguous int32 of their shape; `others`: further tensors.  None stands for an operand that was left out."""
-    for name, t, shape in ints:
-        if t is not None and (t.dtype is not _I32 or t.shape != shape or not t.is_contiguous()):
-            raise KernelError(f"{what}: {name} must be a contiguous int32 tensor {list(shape)}, got {t.dtype} {list(t.shape)}")
-    if not ints[0][1].is_cuda:
-        require_cuda()
-        raise KernelError(f"{what}: operands must live on the CUDA device")
-    dev = torch._C._cuda_getDevice()
-    for name, t, shape in ints:
-        if t is not None and t.get_device() != dev:
-            raise KernelError(f"{what}: {name} must live on the current CUDA device (cuda:{dev}), not on {t.device}")
-    for t in others:
-        if t is not None and t.get_device() != dev:
-            raise KernelError(f"{what}: operands must live on the current CUDA device (cuda:{dev}), not on {t.device}")
-    return _raw_stream(dev)
+def draft_ops():
+    """The host side of these operators (csrc/host/draft_ops.cpp): it checks operands, allocates and launches.  Made at first use; a
+    launcher's library is loaded by the first call that wants it."""
+    if _DRAFT[0] is None:
+        try:
+            mod = build.load_draft_module()
+        except (build.BuildError, ImportError) as e:
+            raise KernelUnavailable(f"the host module csrc/host/draft_ops.cpp is missing and could not be built: {e}") from None
+
+        def load(name: str) -> None:
+            mod.set_launcher(name, cast_pointer(getattr(library(_DRAFT_SOURCES[name]), name), c_void_p).value)
+
+        mod.set_up(KernelError, KernelUnavailable, load)
+        _DRAFT[0] = mod
+    return _DRAFT[0]
 
 
-_I32 = torch.int32
-
-
-def _pools(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor):
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
-        raise KernelError(f"{what}: keys and values must be pools of one shape and dtype, [pages, kv heads, page, d]")
-    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
-        raise KernelError(f"{what}: the pools must be contiguous")
-    dtype_code(k_pages)
-    N, K, P, d = k_pages.shape
-    if not (K and P and d) or N * P > 0x7fffffff:
-        raise KernelError(f"{what}: the pools' sizes {list(k_pages.shape)} are not taken (up to 2^31 - 1 cache slots, nothing empty)")
-    return N, K, P, d
+def draft_call(name: str, launches: int, cost: float, *args):
+    """One call of an operator of csrc/host/draft_ops.cpp; `cost`: bytes that it has to move, for the timers."""
+    fn = getattr(_DRAFT[0] or draft_ops(), name)
+    if _profiling():
+        with region(name, cost):
+            r = fn(*args)
+    else:
+        r = fn(*args)
+    LAUNCHES[0] += launches
+    return r
 
 
 def write_kv_slots(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor,
@@ -776,43 +760,10 @@ def write_kv_slots(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     [pages, K, P, d], at the slots that `cache.step_tables` made.  k, v: [T, K, d] float32 or bfloat16, each with any distance between
     tokens and between heads (columns of a fused projection); rounded once where the pool holds fewer bits.  A negative slot
     leaves its row out; one past the pool is left out and sets the error word.  Slots that are named must differ."""
-    N, K, P, d = _pools("write_kv_slots", k_pages, v_pages)
-    T = k.shape[0]
-    if k.shape != (T, K, d) or v.shape != k.shape or v.dtype != k.dtype:
-        raise KernelError(f"write_kv_slots: keys {list(k.shape)} and values {list(v.shape)} must be [T, {K}, {d}], of one dtype")
-    code = dtype_code(k)
-    if T and d > 1 and (k.stride(2) != 1 or v.stride(2) != 1):
-        raise KernelError("write_kv_slots: the elements of a head must be contiguous")
-    if 2 * K * d > 0x7fffffff:
-        raise KernelError("write_kv_slots: a token's rows are too long")
-    stream = check_operands("write_kv_slots", (("slots", slots, (T,)), ("err", err, (1,))), (k, v, k_pages, v_pages))
-    if T == 0:
-        return
-    (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
-    with region("write_kv_slots", 2 * T * K * d * (k.element_size() + k_pages.element_size())):
-        _WRITE((k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), slots.data_ptr(), err.data_ptr(), kt, kh, vt, vh, code,
-                dtype_code(k_pages), T, N, P, K, d), stream)
+    draft_call("write_kv_slots", 1, _nb(k, v), k, v, k_pages, v_pages, slots, err)
 
 
-_WRITE = Launcher("cache_write.cu", "aie_write_kv_slots", "6P4q7i")
-_CHUNK_ARGS = "11P2q10ifP"
-_CHUNKS_F32 = Launcher("attention_chunks_f32.cu", "aie_attention_chunks_f32", _CHUNK_ARGS, 1)
-_CHUNKS_BF16 = Launcher("attention_chunks.cu", "aie_attention_chunks_bf16", _CHUNK_ARGS, 1)
-
-
-_CHUNKS_TC = Launcher("attention_chunks_tc.cu", "aie_attention_chunks_tc", _CHUNK_ARGS)
-
-
-def chunk_form(bf16: bool, d: int, page: int, rows: float, groups: int = 0):
-    """(launcher, its further arguments, rows of an item, blocks an SM, width of the scratch's rows) of the kernel for heads of d on pages
-    of `page` keys; `rows`: of queries that a request has for a key head, on average; `groups`: of 8 keys in a pool."""
-    if bf16 and d in (64, 128):
-        if rows > 32 and page % 8 == 0 and (128 % page == 0 or page % 128 == 0) and groups < 0x7fffffff:
-            return _CHUNKS_TC, (), 256, 1, d
-        m = 16 if rows <= 16 else 32
-        return _CHUNKS_BF16, (m,), m, 2, d
-    wide = 64 if d <= 64 else 128 if d <= 128 else 256
-    return _CHUNKS_F32, (BF16 if bf16 else F32,), (16 if wide == 256 else 32), (2 if wide == 64 else 1), wide
+CHUNK_FORM = -1      # the form that attention of new tokens takes (csrc/host/draft_ops.cpp: chunk_form); -1: by the sizes
 
 
 def paged_attention_chunks(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor,
@@ -827,47 +778,8 @@ def paged_attention_chunks(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     Any head size up to 256 that is a multiple of 8.  Lengths that do not fit q or the table bring nothing and set the error word, so
     does a page outside the pool, whose keys count as zeros.  How a token's sums are ordered depends on the whole batch's lengths; a
     non-finite key or value reaches all of its request's tokens in the step."""
-    N, K, P, d = _pools("paged_attention_chunks", k_pages, v_pages)
-    if q.dim() != 3 or q.shape[2] != d or q.shape[1] == 0 or q.shape[1] % K or q.dtype != k_pages.dtype:
-        raise KernelError(f"paged_attention_chunks: queries {q.dtype} {list(q.shape)} must be [T, a multiple of {K}, {d}] in {k_pages.dtype}")
-    T, H, _ = q.shape
-    if d % 8 or d > 256:
-        raise KernelError(f"paged_attention_chunks: head size {d} must be a multiple of 8, at most 256")
-    if T * H > 0x7fffffff or N == 0:
-        raise KernelError("paged_attention_chunks: too many rows of queries, or no pages")
-    if block_table.dim() != 2 or block_table.shape[1] == 0:
-        raise KernelError("paged_attention_chunks: the block table must be [requests, pages]")
-    R, W = block_table.shape
-    if W * P > 0x7fffffff - 1024:
-        raise KernelError("paged_attention_chunks: the table names more than 2^31 keys a request")
-    if not 0 <= window <= 0x7fffffff:
-        raise KernelError("paged_attention_chunks: a window is 0 (none) or a number of keys")
-    by_token, by_head, by_element = q.stride()
-    per = 16 // q.element_size()
-    if T and (by_element != 1 or by_token % per or by_head % per or q.data_ptr() % 16):
-        raise KernelError("paged_attention_chunks: every head's row of q must be contiguous and start on 16 bytes")
-    if k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16:
-        raise KernelError("paged_attention_chunks: the pools must start on 16 bytes")
-    if out is None:
-        out = torch.empty((T, H, d), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16:
-        raise KernelError("paged_attention_chunks: out must be contiguous, of q's shape and dtype, and start on 16 bytes")
-    stream = check_operands("paged_attention_chunks",
-                            (("q_start", q_start, (R,)), ("q_len", q_len, (R,)), ("ctx_len", ctx_len, (R,)),
-                             ("block_table", block_table, (R, W)), ("err", err, (1,))), (q, k_pages, v_pages, out))
-    if T == 0 or R == 0:
-        return out
-    launch, more, rows, an_sm, wide = chunk_form(q.dtype is torch.bfloat16, d, P, T * (H // K) / R, N * K * P // 8)
-    blocks = an_sm * sm_count()
-    parts = 2 * blocks * rows
-    scratch = torch.empty(parts * (wide + 2) + 8 * blocks, dtype=torch.float32, device=q.device)
-    at = scratch.data_ptr()
-    fields = (q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), q_start.data_ptr(), q_len.data_ptr(),
-              ctx_len.data_ptr(), block_table.data_ptr(), at, at + 4 * parts * wide, at + 4 * parts * (wide + 2), by_token, by_head,
-              R, W, T, N, P, H, K, H // K, d, window, scale * 1.4426950408889634, err.data_ptr())
-    with region("attention_chunks", 2 * _nb(q)):
-        launch(fields, stream, *more)
-    return out
+    return draft_call("paged_attention_chunks", 2, 2 * _nb(q), q, k_pages, v_pages, q_start, q_len, ctx_len, block_table, scale, window,
+                      err, out, CHUNK_FORM)
 
 
 # ---------------------------------------------------------------------------

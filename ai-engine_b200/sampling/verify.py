@@ -5,11 +5,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from ..kernels.loader import KernelError
-from ..kernels.ops import Launcher, check_operands
-from ..kernels.profile import region
-
-MAX_VOCAB = 1 << 20
+from ..kernels.ops import _nb, draft_call
 
 
 def verify_drafts(target_probs: torch.Tensor, q_start: torch.Tensor, draft_tokens: torch.Tensor, draft_len: Optional[torch.Tensor],
@@ -29,35 +25,5 @@ def verify_drafts(target_probs: torch.Tensor, q_start: torch.Tensor, draft_token
     ones, the new one, -1) and emitted [R] = k + 1 (0 for an idle request): by how many tokens the request has grown.  Rows that are
     not there (the request is left idle), a drafted token outside the vocabulary (refused) and a row without mass (token 0) set the
     error word."""
-    if target_probs.dim() != 2 or draft_tokens.dim() != 2:
-        raise KernelError("verify_drafts: target_probs must be [T, V] and draft_tokens [R, N]")
-    (T, V), (R, N) = target_probs.shape, draft_tokens.shape
-    if not 0 < V <= MAX_VOCAB:
-        raise KernelError(f"verify_drafts: a vocabulary of {V} (1 to {MAX_VOCAB} are taken)")
-    for name, t, shape in (("target_probs", target_probs, (T, V)), ("draft_probs", draft_probs, (R, N, V)),
-                           ("accept_draws", accept_draws, (R, N)), ("token_draws", token_draws, (R,))):
-        if t is not None and (t.dtype != torch.float32 or t.shape != shape):
-            raise KernelError(f"verify_drafts: {name} must be float32 {list(shape)}, got {t.dtype} {list(t.shape)}")
-    row, element = target_probs.stride()
-    guess, by_req, by_place = None, 0, 0
-    if draft_probs is not None:
-        guess, (by_req, by_place, last) = draft_probs.data_ptr(), draft_probs.stride()
-        element = element if last == 1 else last
-    if element != 1 and V > 1:
-        raise KernelError("verify_drafts: the probabilities of a row must be contiguous")
-    if not (accept_draws.is_contiguous() and token_draws.is_contiguous()):
-        raise KernelError("verify_drafts: draws must be contiguous")
-    stream = check_operands("verify_drafts", (("q_start", q_start, (R,)), ("draft_tokens", draft_tokens, (R, N)), ("draft_len", draft_len, (R,)),
-                                              ("err", err, (1,))), (target_probs, draft_probs, accept_draws, token_draws))
-    tokens, emitted = torch.empty(R * (N + 2), dtype=torch.int32, device=target_probs.device).split_with_sizes((R * (N + 1), R))
-    tokens = tokens.view(R, N + 1)
-    if R == 0:
-        return tokens, emitted
-    with region("verify_drafts", 4 * R * V * (2 if guess else 1)):
-        _VERIFY((target_probs.data_ptr(), q_start.data_ptr(), draft_tokens.data_ptr(), draft_len.data_ptr() if draft_len is not None else 0,
-                 guess or 0, accept_draws.data_ptr(), token_draws.data_ptr(), tokens.data_ptr(), emitted.data_ptr(), err.data_ptr(), row,
-                 by_req, by_place, T, V, R, N), stream)
-    return tokens, emitted
-
-
-_VERIFY = Launcher("verify_drafts.cu", "aie_verify_drafts", "10P3q4i")
+    return draft_call("verify_drafts", 1, _nb(token_draws) * target_probs.shape[-1], target_probs, q_start, draft_tokens, draft_len,
+                      draft_probs, accept_draws, token_draws, err)

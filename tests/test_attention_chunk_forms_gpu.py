@@ -14,11 +14,7 @@ BF16 = torch.bfloat16
 def form(request, monkeypatch):
     from ai_engine_b200.kernels import ops
 
-    def choose(bf16, d, page, *_):
-        return {"tcgen05": (ops._CHUNKS_TC, (), 256, 1, d), "mma 16": (ops._CHUNKS_BF16, (16,), 16, 2, d),
-                "mma 32": (ops._CHUNKS_BF16, (32,), 32, 2, d), "float32": (ops._CHUNKS_F32, (1,), 32, 2 if d == 64 else 1, d)}[request.param]
-
-    monkeypatch.setattr(ops, "chunk_form", choose)
+    monkeypatch.setattr(ops, "CHUNK_FORM", {"float32": 0, "mma 16": 1, "mma 32": 2, "tcgen05": 3}[request.param])
     return request.param
 
 
