@@ -1,38 +1,42 @@
-// Attention of new tokens over a paged cache (see attention_chunks.cuh) in bfloat16, heads of 64 and 128, for items of up to 32 rows:
-// a few drafted tokens of a request times the query heads of a key head.
+// Attention of new tokens over a paged cache (see attention_chunks.cuh) in bfloat16, heads of 64 and 128, for items of 16, 32 or 64 rows:
+// a few drafted tokens of a request times the query heads of a key head; any page size.
 //   o = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m),   x_j = (q . k_j) * scale * log2 e
 //
-// What bounds it: reading keys and values once.  Products go through mma.sync, whose tiles of 16 rows fit 4 tokens of 4 heads: at 16 rows they
-// need a fifth of the time that the bytes take.  A block has four warps; of every key tile each warp takes CK keys of its own through a ring
-// of its own (cp.async, stages of 8 KB), so that warps meet only at an item's end, where their outputs are added up in shared memory.
-// Queries are read as fragments out of shared memory.  Scores, maxima and sums are float32; probabilities are rounded to bfloat16 for the
-// product with the values, as the values are, which the result's own rounding hides (2^-9 each on average).
+// Products go through mma.sync, whose tiles of 16 rows fit 4 tokens of 4 heads.  A block has four groups of warps; of every key
+// tile each group takes CK keys of its own through a ring of its own (cp.async, stages of 8 KB), and each warp of a group has 16 rows of
+// the item and reads the group's keys and values.  Groups meet only at an item's end, where their outputs are added up in shared memory.
+// What bounds it: with every 16 rows a warp of its own, reading keys and values once.  One warp for 32 rows (255 registers, eight
+// warps an SM) waited for its own instructions: 5.3 cycles each, at a quarter of the tensor pipe and half of the memory's rate.
+// Scores, maxima and sums are float32, a row's reference maximum moves by more than 8 (log2 units) or not at all; probabilities are rounded
+// to bfloat16 for the product with the values, as the values are, which the result's own rounding hides (2^-9 each on average).
 #include "attention_chunks.cuh"
 
-#define CB_WARPS 4
-#define CB_STAGES 3
+#define CB_GROUPS 4
+#define CB_RESCALE_STEP 8.0f
 
-template <int D, int MT> struct CbShape {
-    static constexpr int M = 16 * MT;                 // rows of an item
-    static constexpr int CK = D == 64 ? 32 : 16;      // keys of a warp's stage
-    static constexpr int KT = CB_WARPS * CK;          // keys of a tile
+// GW: warps of a group
+template <int D, int GW> struct CbShape {
+    static constexpr int M = 16 * GW;                 // rows of an item
+    static constexpr int threads = CB_GROUPS * GW * 32;
+    static constexpr int CK = D == 64 ? 32 : 16;      // keys of a group's stage
+    static constexpr int KT = CB_GROUPS * CK;         // keys of a tile
+    static constexpr int NST = 3;
     static constexpr int stage = 2 * CK * D;          // elements: keys, then values
-    static constexpr int ring_bytes = CB_WARPS * CB_STAGES * stage * 2;
-    static constexpr int q_off = ring_bytes, ml_off = q_off + M * D * 2, bytes = ml_off + CB_WARPS * M * 2 * 4;
-    static_assert(CB_WARPS * M * D * 4 <= ring_bytes, "the warps' outputs meet in the ring's memory");
+    static constexpr int TPK = 32 * GW / CK < 2 ? 2 : 32 * GW / CK;      // threads that copy a key: at least a 32-byte sector at a time
+    static constexpr int ring_bytes = CB_GROUPS * NST * stage * 2;
+    static constexpr int blocks = GW == 4 ? 1 : 2;    // an SM: 16 warps of 128 registers, or eight of 255
+    static constexpr int o_bytes = CB_GROUPS * M * D * 4;      // the groups' outputs meet in the ring's memory
+    static constexpr int q_off = ring_bytes > o_bytes ? ring_bytes : o_bytes, ml_off = q_off + M * D * 2, bytes = ml_off + CB_GROUPS * M * 2 * 4;
 };
 
-__device__ __forceinline__ void cb_fetch(void* dst, const void* src, bool there) {
-    const unsigned d = (unsigned)__cvta_generic_to_shared(dst);
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;\n" ::"r"(d), "l"(src), "r"(there ? 16 : 0));
+__device__ __forceinline__ void cb_fetch(unsigned dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 16 : 0));
 }
-__device__ __forceinline__ void cb_ldsm(unsigned (&r)[4], const void* p) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"((unsigned)__cvta_generic_to_shared(p)));
+__device__ __forceinline__ void cb_ldsm(unsigned (&r)[4], unsigned p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p));
 }
-__device__ __forceinline__ void cb_ldsm_t(unsigned (&r)[4], const void* p) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"((unsigned)__cvta_generic_to_shared(p)));
+__device__ __forceinline__ void cb_ldsm_t(unsigned (&r)[4], unsigned p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p));
 }
 __device__ __forceinline__ void cb_mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -48,29 +52,32 @@ __device__ __forceinline__ float cb_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// row r, 16-byte piece c of rows of D elements: pieces are permuted so that eight rows' pieces lie in different banks
-template <int D> __device__ __forceinline__ bf16* cb_at(bf16* base, int row, int piece) { return base + row * D + ((piece ^ (row & 7)) << 3); }
+// byte offset of row r, 16-byte piece c of rows of D elements: pieces are permuted so that eight rows' pieces lie in different banks
+template <int D> __device__ __forceinline__ unsigned cb_at(int row, int piece) { return (unsigned)(row * (D * 2) + ((piece ^ (row & 7)) << 4)); }
 
-template <int D, int MT>
-__global__ void __launch_bounds__(CB_WARPS * 32, 2) chunk_bf16_kernel(const ChArgs a) {
-    using S = CbShape<D, MT>;
-    constexpr int M = S::M, KT = S::KT, CK = S::CK, PC = D / 8, NST = CB_STAGES;
+template <int D, int GW>
+__global__ void __launch_bounds__(CbShape<D, GW>::threads, CbShape<D, GW>::blocks) chunk_bf16_kernel(const ChArgs a) {
+    using S = CbShape<D, GW>;
+    constexpr int M = S::M, KT = S::KT, CK = S::CK, PC = D / 8, NST = S::NST, THREADS = S::threads, TPK = S::TPK;
+    constexpr int KEYS = 32 * GW / TPK, ROUNDS = CK / KEYS;      // keys that the group's threads copy at a time, and how often
     extern __shared__ __align__(128) unsigned char cb_smem[];
     __shared__ ChShared sh;
     pdl_launch_dependents();
     pdl_wait();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = warp / GW, mt = warp % GW, gt = mt * 32 + lane;
     const int c = blockIdx.x, C = gridDim.x;
     if (tid == 0) a.meta[2 * c] = make_int4(0, 0, 0, 0);
     ChWalk w;
-    if (!ch_begin<CB_WARPS * 32, M, KT>(a, c, C, &sh, w)) return;
-    bf16* ring = reinterpret_cast<bf16*>(cb_smem) + warp * NST * S::stage;
-    bf16* q_s = reinterpret_cast<bf16*>(cb_smem + S::q_off);
-    float* ml = reinterpret_cast<float*>(cb_smem + S::ml_off);      // [warps][M][2]
+    if (!ch_begin<THREADS, M, KT>(a, c, C, &sh, w)) return;
+    const unsigned smem = (unsigned)__cvta_generic_to_shared(cb_smem);
+    const unsigned ring = smem + group * NST * S::stage * 2, q_s = smem + S::q_off;
+    float* ml = reinterpret_cast<float*>(cb_smem + S::ml_off);      // [groups][M][2]
     const bf16* kp = reinterpret_cast<const bf16*>(a.k_pages);
     const bf16* vp = reinterpret_cast<const bf16*>(a.v_pages);
     const int r0 = lane >> 2, col = (lane & 3) * 2;      // of a 16 x 8 accumulator: rows r0 and r0 + 8, columns col and col + 1
     const int lm = lane >> 3, l8 = lane & 7;             // ldmatrix: matrix and row that this lane points at
+    const bool plain = a.scale2 > 0.f;                   // else scores are scaled before they are masked
+    const float sl2 = plain ? a.scale2 : 1.f;
     unsigned bad = 0;
 
     for (;;) {
@@ -81,33 +88,43 @@ __global__ void __launch_bounds__(CB_WARPS * 32, 2) chunk_bf16_kernel(const ChAr
         const int kt0 = tl.first + w.k;
         const int low_all = a.window > 0 ? c0 + tl.i0 - a.window + 1 : 0;      // first key that any row sees
 
-        auto issue = [&](int i) {
-            if (i < n) {
-                bf16* ks = ring + (i % NST) * S::stage;
-                bf16* vs = ks + CK * D;
-                const int k_at = (kt0 + i) * KT + warp * CK + (lane & (CK - 1));
-                long long row_at = -1;
-                if (k_at < hi && k_at >= low_all) {
-                    const int pi = ch_over(k_at, a.by_p), page = __ldg(bt + pi);
-                    if (page >= 0 && page < a.num_pages) row_at = ((long long)page * a.K + w.kh) * a.P + (k_at - pi * a.P);
-                    else bad |= AIE_DEV_PAGE_OOB;
-                }
+        // this thread copies every TPK-th piece of its key of the stage; the page of the next stage's key is read a stage ahead
+        auto key_of = [&](int i, int round) { return (kt0 + i) * KT + group * CK + round * KEYS + gt / TPK; };
+        auto page_of = [&](int i, int round) {
+            const int key = key_of(i, round);
+            return i < n && key < hi && key >= low_all ? __ldg(bt + ch_over(key, a.by_p)) : -1;
+        };
+        int pages[ROUNDS];
 #pragma unroll
-                for (int x = 0; x < CK * PC / 32; ++x) {
-                    const int kk = (lane + 32 * x) / PC, pc = (lane + 32 * x) % PC;
-                    const long long ra = __shfl_sync(0xffffffffu, row_at, kk);
-                    const size_t off = ra >= 0 ? (size_t)ra * D + pc * 8 : 0;
-                    cb_fetch(cb_at<D>(ks, kk, pc), kp + off, ra >= 0);
-                    cb_fetch(cb_at<D>(vs, kk, pc), vp + off, ra >= 0);
+        for (int x = 0; x < ROUNDS; ++x) pages[x] = page_of(0, x);
+        auto issue = [&](int i, int slot) {
+            if (i < n) {
+                const unsigned st = ring + slot * S::stage * 2;
+#pragma unroll
+                for (int x = 0; x < ROUNDS; ++x) {
+                    const int key = key_of(i, x), kk = x * KEYS + gt / TPK, page = pages[x];
+                    bool there = key < hi && key >= low_all;
+                    if (there && (page < 0 || page >= a.num_pages)) {
+                        bad |= AIE_DEV_PAGE_OOB;
+                        there = false;
+                    }
+                    const size_t off = there ? (((size_t)page * a.K + w.kh) * a.P + (key - ch_over(key, a.by_p) * a.P)) * D + gt % TPK * 8 : 0;
+#pragma unroll
+                    for (int y = 0; y < PC / TPK; ++y) {
+                        const unsigned to = st + cb_at<D>(kk, gt % TPK + y * TPK);
+                        cb_fetch(to, kp + off + y * TPK * 8, there);
+                        cb_fetch(to + CK * D * 2, vp + off + y * TPK * 8, there);
+                    }
+                    pages[x] = page_of(i + 1, x);
                 }
             }
             asm volatile("cp.async.commit_group;\n" ::);
         };
 #pragma unroll
-        for (int i = 0; i < NST - 1; ++i) issue(i);
+        for (int i = 0; i < NST - 1; ++i) issue(i, i);
 
         // queries of the item
-        for (int i = tid; i < M * PC; i += CB_WARPS * 32) {
+        for (int i = tid; i < M * PC; i += THREADS) {
             const int row = i / PC, pc = i % PC;
             uint4 x = make_uint4(0u, 0u, 0u, 0u);
             if (row < tl.rows) {
@@ -115,155 +132,144 @@ __global__ void __launch_bounds__(CB_WARPS * 32, 2) chunk_bf16_kernel(const ChAr
                 x = *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.q) + (s0 + t) * a.q_token +
                                                     (long long)(w.kh * a.G + g) * a.q_head + pc * 8);
             }
-            *reinterpret_cast<uint4*>(cb_at<D>(q_s, row, pc)) = x;
+            *reinterpret_cast<uint4*>(cb_smem + S::q_off + cb_at<D>(row, pc)) = x;
         }
         __syncthreads();
 
-        float m_run[MT][2], l_run[MT][2], o[MT][D / 8][4];
-        int pos[MT][2];
+        const bool live = mt * 16 < tl.rows;             // any row of this warp
+        float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f}, o[D / 8][4];
+        const int pos0 = c0 + ch_over(tl.row0 + mt * 16 + r0, a.by_g), pos1 = c0 + ch_over(tl.row0 + mt * 16 + r0 + 8, a.by_g);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int x = 0; x < D / 8; ++x)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                m_run[mt][e] = -INFINITY;
-                l_run[mt][e] = 0.f;
-                pos[mt][e] = c0 + ch_over(tl.row0 + mt * 16 + r0 + 8 * e, a.by_g);
-            }
-#pragma unroll
-            for (int x = 0; x < D / 8; ++x)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[mt][x][e] = 0.f;
-        }
+            for (int e = 0; e < 4; ++e) o[x][e] = 0.f;
         const int last_low = a.window > 0 ? c0 + tl.i1 - a.window + 1 : 0;      // first key that the last row sees
 
+        int slot = 0;
         for (int i = 0; i < n; ++i) {
-            issue(i + NST - 1);
-            asm volatile("cp.async.wait_group %0;\n" ::"n"(NST - 1));
-            __syncwarp();
-            bf16* ks = ring + (i % NST) * S::stage;
-            bf16* vs = ks + CK * D;
-            const int k_at = (kt0 + i) * KT + warp * CK;
-            if (k_at < hi) {
-                float s[MT][CK / 8][4];
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(NST - 2));
+            // the stage is there for the whole group, and the group has read the one that the next copies go to
+            if (GW == 1) __syncwarp();
+            else asm volatile("bar.sync %0, %1;\n" ::"r"(1 + group), "n"(32 * GW) : "memory");
+            issue(i + NST - 1, slot == 0 ? NST - 1 : slot - 1);
+            const unsigned ks = ring + slot * S::stage * 2, vs = ks + CK * D * 2;
+            slot = slot + 1 == NST ? 0 : slot + 1;
+            const int k_at = (kt0 + i) * KT + group * CK;
+            if (k_at >= hi || !live) continue;
+            float s[CK / 8][4];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+            for (int x = 0; x < CK / 8; ++x)
 #pragma unroll
-                    for (int x = 0; x < CK / 8; ++x)
+                for (int e = 0; e < 4; ++e) s[x][e] = 0.f;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[mt][x][e] = 0.f;
+            for (int kk = 0; kk < D / 16; ++kk) {
+                unsigned qa[4];
+                cb_ldsm(qa, q_s + cb_at<D>(mt * 16 + (lm & 1) * 8 + l8, kk * 2 + (lm >> 1)));
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    unsigned qa[MT][4];
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) cb_ldsm(qa[mt], cb_at<D>(q_s, mt * 16 + (lm & 1) * 8 + l8, kk * 2 + (lm >> 1)));
-#pragma unroll
-                    for (int x = 0; x < CK / 16; ++x) {
-                        unsigned b[4];
-                        cb_ldsm(b, cb_at<D>(ks, x * 16 + (lm >> 1) * 8 + l8, kk * 2 + (lm & 1)));
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
-                            cb_mma(s[mt][2 * x], qa[mt], b[0], b[1]);
-                            cb_mma(s[mt][2 * x + 1], qa[mt], b[2], b[3]);
-                        }
-                    }
+                for (int x = 0; x < CK / 16; ++x) {
+                    unsigned b[4];
+                    cb_ldsm(b, ks + cb_at<D>(x * 16 + (lm >> 1) * 8 + l8, kk * 2 + (lm & 1)));
+                    cb_mma(s[2 * x], qa, b[0], b[1]);
+                    cb_mma(s[2 * x + 1], qa, b[2], b[3]);
                 }
-                const bool masked = k_at + CK - 1 > c0 + tl.i0 || k_at < last_low;
-                unsigned p[MT][CK / 16][4];
+            }
+            if (__builtin_expect(!plain, 0)) {
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    float top[2] = {-INFINITY, -INFINITY};
+                for (int x = 0; x < CK / 8; ++x)
 #pragma unroll
-                    for (int x = 0; x < CK / 8; ++x)
+                    for (int e = 0; e < 4; ++e) s[x][e] *= a.scale2;
+            }
+            if (k_at + CK - 1 > c0 + tl.i0 || k_at < last_low) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float v = s[mt][x][e] * a.scale2;
-                            if (masked) {
-                                const int key = k_at + x * 8 + col + (e & 1), q = pos[mt][e >> 1];
-                                if (key > q || (a.window > 0 && key <= q - a.window)) v = -INFINITY;
-                            }
-                            s[mt][x][e] = v;
-                            top[e >> 1] = fmaxf(top[e >> 1], v);
-                        }
-                    float corr[2], use[2];
+                for (int x = 0; x < CK / 8; ++x)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
-                        top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
-                        const float m_new = fmaxf(m_run[mt][e], top[e]);
-                        use[e] = m_new == -INFINITY ? 0.f : m_new;
-                        corr[e] = m_run[mt][e] == m_new ? 1.f : cb_exp2(m_run[mt][e] - use[e]);
-                        m_run[mt][e] = m_new;
-                        l_run[mt][e] *= corr[e];
-                    }
-#pragma unroll
-                    for (int x = 0; x < CK / 8; ++x) {
-                        float f[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) f[e] = cb_exp2(s[mt][x][e] - use[e >> 1]);
-                        l_run[mt][0] += f[0] + f[1];          // of this lane's keys
-                        l_run[mt][1] += f[2] + f[3];
-                        p[mt][x >> 1][(x & 1) * 2] = cb_pack(f[0], f[1]);
-                        p[mt][x >> 1][(x & 1) * 2 + 1] = cb_pack(f[2], f[3]);
-                    }
-                    if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
-#pragma unroll
-                        for (int x = 0; x < D / 8; ++x) {
-                            o[mt][x][0] *= corr[0], o[mt][x][1] *= corr[0];
-                            o[mt][x][2] *= corr[1], o[mt][x][3] *= corr[1];
-                        }
-                    }
-                }
-#pragma unroll
-                for (int y = 0; y < CK / 16; ++y)
-#pragma unroll
-                    for (int x = 0; x < D / 16; ++x) {
-                        unsigned b[4];
-                        cb_ldsm_t(b, cb_at<D>(vs, y * 16 + (lm & 1) * 8 + l8, x * 2 + (lm >> 1)));
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
-                            cb_mma(o[mt][2 * x], p[mt][y], b[0], b[1]);
-                            cb_mma(o[mt][2 * x + 1], p[mt][y], b[2], b[3]);
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = k_at + x * 8 + col + (e & 1), q = e < 2 ? pos0 : pos1;
+                        if (key > q || (a.window > 0 && key <= q - a.window)) s[x][e] = -INFINITY;
                     }
             }
-            __syncwarp();      // the stage is free again
+            float top[2] = {-INFINITY, -INFINITY}, corr[2] = {1.f, 1.f}, use[2];
+#pragma unroll
+            for (int x = 0; x < CK / 8; ++x) {
+                top[0] = fmaxf(top[0], fmaxf(s[x][0], s[x][1]));
+                top[1] = fmaxf(top[1], fmaxf(s[x][2], s[x][3]));
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2)) * sl2;
+                if (top[e] > m_run[e] + CB_RESCALE_STEP) {
+                    corr[e] = m_run[e] == -INFINITY ? 0.f : cb_exp2(m_run[e] - top[e]);
+                    m_run[e] = top[e];
+                }
+                use[e] = m_run[e] == -INFINITY ? 0.f : m_run[e];
+            }
+            if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+                l_run[0] *= corr[0];
+                l_run[1] *= corr[1];
+#pragma unroll
+                for (int x = 0; x < D / 8; ++x) {
+                    o[x][0] *= corr[0], o[x][1] *= corr[0];
+                    o[x][2] *= corr[1], o[x][3] *= corr[1];
+                }
+            }
+#pragma unroll
+            for (int y = 0; y < CK / 16; ++y) {
+                unsigned p[4];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    float f[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) f[e] = cb_exp2(fmaf(s[2 * y + x][e], sl2, -use[e >> 1]));
+                    l_run[0] += f[0] + f[1];          // of this lane's keys
+                    l_run[1] += f[2] + f[3];
+                    p[2 * x] = cb_pack(f[0], f[1]);
+                    p[2 * x + 1] = cb_pack(f[2], f[3]);
+                }
+#pragma unroll
+                for (int x = 0; x < D / 16; ++x) {
+                    unsigned b[4];
+                    cb_ldsm_t(b, vs + cb_at<D>(y * 16 + (lm & 1) * 8 + l8, x * 2 + (lm >> 1)));
+                    cb_mma(o[2 * x], p, b[0], b[1]);
+                    cb_mma(o[2 * x + 1], p, b[2], b[3]);
+                }
+            }
         }
         asm volatile("cp.async.wait_group 0;\n" ::);
         __syncthreads();
 
-        // the warps meet
-        float* o_s = reinterpret_cast<float*>(cb_smem);      // [warps][M][D]
+        // the groups meet
+        float* o_s = reinterpret_cast<float*>(cb_smem);      // [groups][M][D]
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int e = 0; e < 2; ++e) {
+            const int row = mt * 16 + r0 + 8 * e;
+            float l = l_run[e];
+            l += __shfl_xor_sync(0xffffffffu, l, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
+            if ((lane & 3) == 0) *reinterpret_cast<float2*>(ml + (group * M + row) * 2) = make_float2(m_run[e], l);
+            if (row < tl.rows)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int row = mt * 16 + r0 + 8 * e;
-                float l = l_run[mt][e];
-                l += __shfl_xor_sync(0xffffffffu, l, 1);
-                l += __shfl_xor_sync(0xffffffffu, l, 2);
-                if ((lane & 3) == 0) *reinterpret_cast<float2*>(ml + (warp * M + row) * 2) = make_float2(m_run[mt][e], l);
-                if (row < tl.rows)
-#pragma unroll
-                    for (int x = 0; x < D / 8; ++x)
-                        *reinterpret_cast<float2*>(o_s + (warp * M + row) * D + x * 8 + col) = make_float2(o[mt][x][2 * e], o[mt][x][2 * e + 1]);
-            }
+                for (int x = 0; x < D / 8; ++x)
+                    *reinterpret_cast<float2*>(o_s + (group * M + row) * D + ((x * 8 + col) ^ ((row & 3) << 3))) = make_float2(o[x][2 * e], o[x][2 * e + 1]);
+        }
         __syncthreads();
         const bool begins = w.k == 0, ends = w.k + n == tl.tiles;
-        const size_t slot = (size_t)2 * c + (begins ? 1 : 0);
-        for (int i = tid; i < tl.rows * (D / 4); i += CB_WARPS * 32) {
+        const size_t place = (size_t)2 * c + (begins ? 1 : 0);
+        for (int i = tid; i < tl.rows * (D / 4); i += THREADS) {
             const int row = i / (D / 4), e = (i % (D / 4)) * 4;
-            float2 g[CB_WARPS];
+            float2 g[CB_GROUPS];
             float m = -INFINITY, l = 0.f;
 #pragma unroll
-            for (int x = 0; x < CB_WARPS; ++x) {
+            for (int x = 0; x < CB_GROUPS; ++x) {
                 g[x] = *reinterpret_cast<const float2*>(ml + (x * M + row) * 2);
                 m = fmaxf(m, g[x].x);
             }
             float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int x = 0; x < CB_WARPS; ++x) {
+            for (int x = 0; x < CB_GROUPS; ++x) {
                 const float f = g[x].x == -INFINITY ? 0.f : cb_exp2(g[x].x - m);
-                const float4 z = *reinterpret_cast<const float4*>(o_s + (x * M + row) * D + e);
+                const float4 z = *reinterpret_cast<const float4*>(o_s + (x * M + row) * D + (e ^ ((row & 3) << 3)));
                 l += f * g[x].y;
                 y.x += f * z.x, y.y += f * z.y, y.z += f * z.z, y.w += f * z.w;
             }
@@ -273,8 +279,8 @@ __global__ void __launch_bounds__(CB_WARPS * 32, 2) chunk_bf16_kernel(const ChAr
                 store4<bf16>(reinterpret_cast<bf16*>(a.out) + ((size_t)(s0 + t) * a.H + h) * D + e,
                              make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
             } else {
-                *reinterpret_cast<float4*>(a.part_o + (slot * M + row) * D + e) = y;
-                if (e == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * M + row) * 2) = make_float2(m, l);
+                *reinterpret_cast<float4*>(a.part_o + (place * M + row) * D + e) = y;
+                if (e == 0) *reinterpret_cast<float2*>(a.part_ml + (place * M + row) * 2) = make_float2(m, l);
             }
         }
         if (begins && !ends && tid == 0) ch_leave(a, w, c, n);
@@ -284,29 +290,28 @@ __global__ void __launch_bounds__(CB_WARPS * 32, 2) chunk_bf16_kernel(const ChAr
     if (bad) atomicOr(a.err, bad);
 }
 
-template <int D, int MT> static int launch_chunk_bf16(const ChArgs& a, int C, cudaStream_t st) {
-    using S = CbShape<D, MT>;
-    auto kern = chunk_bf16_kernel<D, MT>;
+template <int D, int GW> static int launch_chunk_bf16(const ChArgs& a, cudaStream_t st) {
+    using S = CbShape<D, GW>;
+    auto kern = chunk_bf16_kernel<D, GW>;
+    const int C = S::blocks * aie_sm_count();
     static unsigned long long done = 0;
     ch_prepare(kern, S::bytes, &done);
-    const int rc = (int)launch_pdl(kern, dim3(C), dim3(CB_WARPS * 32), S::bytes, st, a);
+    const int rc = (int)launch_pdl(kern, dim3(C), dim3(S::threads), S::bytes, st, a);
     if (rc) return rc;
     return launch_chunk_join<bf16, S::M, D>(a, C, st);
 }
 
-// Blocks of the kernels: two an SM.  The scratch is [2 * blocks * rows * (d + 2)] floats and [2 * blocks] int4.
-extern "C" int aie_attention_chunks_bf16_blocks() { return 2 * aie_sm_count(); }
-
-// rows: 16 or 32 of an item
+// rows: 16, 32 or 64 of an item.  The scratch is [2 * blocks * rows * (d + 2)] floats and [2 * blocks] int4; blocks: two an SM, one for 64 rows.
 extern "C" int aie_attention_chunks_bf16(const ChCall* call, int rows, cudaStream_t stream) {
     if (call->R <= 0 || call->T <= 0) return 0;
     ChArgs a;
     const int rc = ch_args(call, 16, 64, &a);
     if (rc) return rc;
-    const int C = aie_attention_chunks_bf16_blocks();
-    if (a.d == 64 && rows == 16) return launch_chunk_bf16<64, 1>(a, C, stream);
-    if (a.d == 64 && rows == 32) return launch_chunk_bf16<64, 2>(a, C, stream);
-    if (a.d == 128 && rows == 16) return launch_chunk_bf16<128, 1>(a, C, stream);
-    if (a.d == 128 && rows == 32) return launch_chunk_bf16<128, 2>(a, C, stream);
+    if (a.d == 64 && rows == 16) return launch_chunk_bf16<64, 1>(a, stream);
+    if (a.d == 64 && rows == 32) return launch_chunk_bf16<64, 2>(a, stream);
+    if (a.d == 64 && rows == 64) return launch_chunk_bf16<64, 4>(a, stream);
+    if (a.d == 128 && rows == 16) return launch_chunk_bf16<128, 1>(a, stream);
+    if (a.d == 128 && rows == 32) return launch_chunk_bf16<128, 2>(a, stream);
+    if (a.d == 128 && rows == 64) return launch_chunk_bf16<128, 4>(a, stream);
     return AIE_UNSUPPORTED;
 }

@@ -269,7 +269,7 @@ PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// The forms of the attention: 0 float32 (and bfloat16 that the others do not take), 1 mma.sync, 16 rows an item, 2 the same with 32, 3 tcgen05.
+// The forms of the attention: 0 float32 (and bfloat16 that the others do not take), 1, 2, 4 mma.sync with 16, 32, 64 rows an item, 3 tcgen05.
 // Rows of queries that a request has for a key head, on average, decide between those that take a call.
 int chunk_form(int code, const Pools& p, double rows) {
     if (code != 1 || (p.d != 64 && p.d != 128)) return 0;
@@ -319,7 +319,7 @@ PyObject* paged_attention_chunks(PyObject*, PyObject* const* a, Py_ssize_t n) {
             if (!sm_count) sm_count = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
             if (form < 0) form = chunk_form(p.code, p, (double)T * G / R);
             const int64_t wide = form ? p.d : p.d <= 64 ? 64 : p.d <= 128 ? 128 : 256;
-            const int64_t M = form == 3 ? 256 : form == 1 || (form == 0 && wide == 256) ? 16 : 32;
+            const int64_t M = form == 3 ? 256 : form == 4 ? 64 : form == 1 || (form == 0 && wide == 256) ? 16 : 32;
             const int64_t blocks = sm_count * (form == 1 || form == 2 || (form == 0 && wide == 64) ? 2 : 1), parts = 2 * blocks * M;
             // parts [parts][wide], their maxima and sums [parts][2], what is to be joined [blocks][2] int4
             at::Tensor scratch = fresh({parts * (wide + 2) + 8 * blocks}, at::kFloat, q);
