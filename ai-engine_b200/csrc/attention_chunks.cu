@@ -88,15 +88,25 @@ __global__ void __launch_bounds__(CbShape<D, GW>::threads, CbShape<D, GW>::block
         const int kt0 = tl.first + w.k;
         const int low_all = a.window > 0 ? c0 + tl.i0 - a.window + 1 : 0;      // first key that any row sees
 
-        // this thread copies every TPK-th piece of its key of the stage; the page of the next stage's key is read a stage ahead
+        // this thread copies every TPK-th piece of its key of the stage; the pages of the next two stages' keys are read ahead
         auto key_of = [&](int i, int round) { return (kt0 + i) * KT + group * CK + round * KEYS + gt / TPK; };
         auto page_of = [&](int i, int round) {
             const int key = key_of(i, round);
             return i < n && key < hi && key >= low_all ? __ldg(bt + ch_over(key, a.by_p)) : -1;
         };
-        int pages[ROUNDS];
+        int pages[ROUNDS], pages_next[ROUNDS];
 #pragma unroll
-        for (int x = 0; x < ROUNDS; ++x) pages[x] = page_of(0, x);
+        for (int x = 0; x < ROUNDS; ++x) {
+            pages[x] = page_of(0, x);
+            pages_next[x] = page_of(1, x);
+        }
+        // queries of the item: they land with the first stage
+        for (int i = tid; i < M * PC; i += THREADS) {
+            const int row = i / PC, pc = i % PC;
+            const bool there = row < tl.rows;
+            const int full = tl.row0 + (there ? row : 0), t = ch_over(full, a.by_g), g = full - t * a.G;
+            cb_fetch(q_s + cb_at<D>(row, pc), reinterpret_cast<const bf16*>(a.q) + (s0 + t) * a.q_token + (long long)(w.kh * a.G + g) * a.q_head + pc * 8, there);
+        }
         auto issue = [&](int i, int slot) {
             if (i < n) {
                 const unsigned st = ring + slot * S::stage * 2;
@@ -115,7 +125,8 @@ __global__ void __launch_bounds__(CbShape<D, GW>::threads, CbShape<D, GW>::block
                         cb_fetch(to, kp + off + y * TPK * 8, there);
                         cb_fetch(to + CK * D * 2, vp + off + y * TPK * 8, there);
                     }
-                    pages[x] = page_of(i + 1, x);
+                    pages[x] = pages_next[x];
+                    pages_next[x] = page_of(i + 2, x);
                 }
             }
             asm volatile("cp.async.commit_group;\n" ::);
@@ -123,17 +134,7 @@ __global__ void __launch_bounds__(CbShape<D, GW>::threads, CbShape<D, GW>::block
 #pragma unroll
         for (int i = 0; i < NST - 1; ++i) issue(i, i);
 
-        // queries of the item
-        for (int i = tid; i < M * PC; i += THREADS) {
-            const int row = i / PC, pc = i % PC;
-            uint4 x = make_uint4(0u, 0u, 0u, 0u);
-            if (row < tl.rows) {
-                const int full = tl.row0 + row, t = ch_over(full, a.by_g), g = full - t * a.G;
-                x = *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.q) + (s0 + t) * a.q_token +
-                                                    (long long)(w.kh * a.G + g) * a.q_head + pc * 8);
-            }
-            *reinterpret_cast<uint4*>(cb_smem + S::q_off + cb_at<D>(row, pc)) = x;
-        }
+        asm volatile("cp.async.wait_group %0;\n" ::"n"(NST - 2));
         __syncthreads();
 
         const bool live = mt * 16 < tl.rows;             // any row of this warp

@@ -320,7 +320,7 @@ PyObject* paged_attention_chunks(PyObject*, PyObject* const* a, Py_ssize_t n) {
             if (form < 0) form = chunk_form(p.code, p, (double)T * G / R);
             const int64_t wide = form ? p.d : p.d <= 64 ? 64 : p.d <= 128 ? 128 : 256;
             const int64_t M = form == 3 ? 256 : form == 4 ? 64 : form == 1 || (form == 0 && wide == 256) ? 16 : 32;
-            const int64_t blocks = sm_count * (form == 1 || form == 2 || (form == 0 && wide == 64) ? 2 : 1), parts = 2 * blocks * M;
+            const int64_t blocks = sm_count * (form == 1 || form == 2 ? 2 : 1), parts = 2 * blocks * M;
             // parts [parts][wide], their maxima and sums [parts][2], what is to be joined [blocks][2] int4
             at::Tensor scratch = fresh({parts * (wide + 2) + 8 * blocks}, at::kFloat, q);
             float* s = scratch.data_ptr<float>();
