@@ -2,13 +2,14 @@
 // ones whose head size the tensor-core kernels do not take.
 //   o = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m),   x_j = (q . k_j) * scale * log2 e,   keys j <= position (and > position - window)
 //
-// A block has NG groups of two warps; of every key tile each group takes eight keys of its own through a ring of its own (cp.async), and
-// each warp of a group has every other four rows of the item.  Groups meet only at an item's end.  Scores: a lane has one key and
-// every fourth of the warp's rows, products and sums two at a time (fma.rn.f32x2) along the head; outputs: a lane has
-// D / 32 columns of all the warp's rows, two rows at a time.  The loop over key tiles exists for each number of fours of rows.
+// A block has NG groups of four warps; of every key tile each group takes sixteen keys of its own through a ring of its own (cp.async), and
+// each warp of a group has every fourth four of the item's rows.  Groups meet only at an item's end.  Scores: a lane has two keys and
+// one row of each of the warp's fours, products and sums two at a time (fma.rn.f32x2) along the head; outputs: a lane has
+// D / 32 columns of all the warp's rows, two rows at a time.  The loop over key tiles exists for each number of fours.
 // What bounds it: the multiply-adds of 5 tokens x 4 heads take as long as their keys' bytes (0.27 G of them, 58 MB: 9 us each), and reading
-// shared memory nearly as long (of a tile of 8 keys x 16 rows x 128: 160 reads of K and Q beside 256 packed multiply-adds, then 64
-// of V and P beside 256).  One warp for 32 rows of 8 keys (255 registers, eight warps an SM) took twice the time.
+// shared memory nearly as long (of 16 keys x 8 rows x 128: 128 reads of K and Q beside 256 packed multiply-adds, then 96 wavefronts
+// of V and P beside 256).  What a step costs beside that is its chain of waits (copies, reads, a row's maximum among eight lanes,
+// probabilities through shared memory): two warps of 16 rows and eight keys each, with twice the steps, took twice the time.
 #include "attention_chunks.cuh"
 
 typedef unsigned long long u64;
@@ -42,16 +43,16 @@ __device__ __forceinline__ float2 cf_both(u64 v) {
 template <int N> struct CfInt { static constexpr int value = N; };
 
 template <int D> struct CfShape {
-    static constexpr int MH = D > 128 ? 8 : 16;      // rows of a warp
-    static constexpr int M = 2 * MH;                 // ... of an item
-    static constexpr int NG = D > 128 ? 4 : 8;       // groups
-    static constexpr int threads = NG * 64;
-    static constexpr int NST = D > 64 ? 3 : 4;       // stages of a group's ring: 8 keys and their values each
-    static constexpr int KT = NG * 8;                // keys of a tile
+    static constexpr int FW = D > 128 ? 1 : 2;       // fours of rows of a warp
+    static constexpr int M = 16 * FW;                // rows of an item
+    static constexpr int NG = D > 128 ? 2 : 4;       // groups of four warps
+    static constexpr int threads = NG * 128;
+    static constexpr int NST = D > 64 ? 3 : 4;       // stages of a group's ring: 16 keys and their values each
+    static constexpr int KT = NG * 16;               // keys of a tile
     static constexpr int KS = D + 4;                 // distance of two rows of keys or queries: eight of them lie in different banks
-    static constexpr int stage = 8 * KS + 8 * D;     // floats
-    static constexpr int PS = MH + 4;                // distance of two keys' probabilities: eight keys' lie in different banks
-    static constexpr int q_off = NG * NST * stage, p_off = q_off + M * KS, ml_off = p_off + NG * 2 * 8 * PS, end = ml_off + NG * M * 2;
+    static constexpr int stage = 16 * KS + 16 * D;   // floats
+    static constexpr int PS = 4 * FW + 4;            // distance of two keys' probabilities
+    static constexpr int q_off = NG * NST * stage, p_off = q_off + M * KS, ml_off = p_off + NG * 4 * 16 * PS, end = ml_off + NG * M * 2;
     static constexpr int bytes = end * 4;
     static_assert(NG * M * D <= NG * NST * stage && bytes <= 227 * 1024 - 256, "the groups' outputs meet in the ring's memory");
 };
@@ -68,25 +69,25 @@ __device__ __forceinline__ void cf_fetch(float* dst, const bf16* src, bool there
 template <typename T, int D>
 __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const ChArgs a) {
     using S = CfShape<D>;
-    constexpr int M = S::M, MH = S::MH, NG = S::NG, NST = S::NST, KT = S::KT, CH = D / 4, RJ = MH / 4, CL = D / 32, THREADS = S::threads;      // CL: columns of a lane
+    constexpr int M = S::M, FW = S::FW, NG = S::NG, NST = S::NST, KT = S::KT, CH = D / 4, CL = D / 32, THREADS = S::threads;      // CL: columns of a lane
     extern __shared__ __align__(16) float cf_smem[];
     __shared__ ChShared sh;
     __shared__ ChWalk place_in_line;              // while the registers hold rows' outputs
     pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int group = warp % NG, half = warp / NG, gt = half * 32 + lane;
+    const int group = warp % NG, mt = warp / NG, gt = mt * 32 + lane;      // mt: which fours of rows
     const int c = blockIdx.x, C = gridDim.x;
     if (tid == 0) a.meta[2 * c] = make_int4(0, 0, 0, 0);
     ChWalk w;
     if (!ch_begin<THREADS, M, KT>(a, c, C, &sh, w)) return;
     float* ring = cf_smem + group * NST * S::stage;
     float* q_s = cf_smem + S::q_off;              // [M][KS]
-    float* p_s = cf_smem + S::p_off + warp * 8 * S::PS;      // this warp's [8 keys][MH]
+    float* p_s = cf_smem + S::p_off + warp * 16 * S::PS;      // this warp's [16 keys][4 FW]
     float* ml = cf_smem + S::ml_off;              // [NG][M][2]
     const T* kp = reinterpret_cast<const T*>(a.k_pages);
     const T* vp = reinterpret_cast<const T*>(a.v_pages);
-    const int key = lane & 7, rg = lane >> 3;     // for the scores: this lane's key; of every four rows of the warp it has row rg
+    const int key = lane & 7, rg = lane >> 3;     // for the scores: this lane's keys are `key` and `key` + 8, of every four rows it has row rg
     unsigned bad = 0;
 
     for (;;) {
@@ -96,7 +97,7 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
         const int* bt = a.table + (size_t)w.r * a.W;
 
         // eight threads copy a key: each every eighth piece; the pages of the next two stages' keys are read ahead
-        const int my_key = group * 8 + (gt >> 3);
+        const int my_key = group * 16 + (gt >> 3);
         auto page_of = [&](int i) {
             const int k_at = (kt0 + i) * KT + my_key;
             return i < n && k_at < hi && k_at >= low_all ? __ldg(bt + ch_over(k_at, a.by_p)) : -1;
@@ -125,7 +126,7 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
                     const bool in = there && ch * 4 < a.d;
                     const size_t off = in ? row_at + ch * 4 : 0;
                     cf_fetch(to + (gt >> 3) * S::KS + ch * 4, kp + off, in);
-                    cf_fetch(to + 8 * S::KS + (gt >> 3) * D + ch * 4, vp + off, in);
+                    cf_fetch(to + 16 * S::KS + (gt >> 3) * D + ch * 4, vp + off, in);
                 }
                 page = page_next;
                 page_next = page_of(i + 2);
@@ -138,15 +139,15 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
         asm volatile("cp.async.wait_group %0;\n" ::"n"(NST - 2));
         __syncthreads();
 
-        float m_run[RJ], l_run[RJ];
-        int lim[RJ];                              // last key that a row sees, -1 for a row that is not there
-        u64 o[RJ][2][CL];                         // rows 4 j + 2 e and the next, column lane * CL + x (CL 8: 4 lane + x % 4, 128 further from x 4 on)
+        float m_run[FW], l_run[FW];
+        int lim[FW];                              // last key that a row sees, -1 for a row that is not there
+        u64 o[FW][2][CL];                         // rows 4 (mt + 4 j) + 2 e and the next, columns CL lane .. (128 further from the fifth on)
         const int reach = a.window > 0 ? a.window : 0x7fffffff;
 #pragma unroll
-        for (int j = 0; j < RJ; ++j) {
+        for (int j = 0; j < FW; ++j) {
             m_run[j] = -INFINITY;
             l_run[j] = 0.f;
-            const int row = (2 * j + half) * 4 + rg;
+            const int row = (mt + 4 * j) * 4 + rg;
             lim[j] = row < rows ? c0 + ch_over(row0 + row, a.by_g) : -1;
 #pragma unroll
             for (int x = 0; x < CL; ++x) o[j][0][x] = o[j][1][x] = 0ull;
@@ -157,34 +158,41 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
             int slot = 0;
             for (int i = 0; i < n; ++i) {
                 asm volatile("cp.async.wait_group %0;\n" ::"n"(NST - 2));
-                // the stage is there for both warps, and both have read the one that the next copies go to
-                asm volatile("bar.sync %0, 64;\n" ::"r"(1 + group) : "memory");
+                // the stage is there for the whole group, and the group has read the one that the next copies go to
+                asm volatile("bar.sync %0, 128;\n" ::"r"(1 + group) : "memory");
                 issue(i + NST - 1, slot == 0 ? NST - 1 : slot - 1);
                 const float* ks = ring + slot * S::stage;
-                const float* vs = ks + 8 * S::KS;
+                const float* vs = ks + 16 * S::KS;
                 slot = slot + 1 == NST ? 0 : slot + 1;
                 if constexpr (JN > 0) {
-                    const int k_at = (kt0 + i) * KT + group * 8 + key;
+                    const int k_at = (kt0 + i) * KT + group * 16 + key;
                     if (k_at - key >= hi) continue;
-                    u64 s2[JN];
+                    u64 s2[JN][2];
 #pragma unroll
-                    for (int j = 0; j < JN; ++j) s2[j] = 0ull;
+                    for (int j = 0; j < JN; ++j) s2[j][0] = s2[j][1] = 0ull;
+                    const float *k0 = ks + key * S::KS, *q0 = q_s + (mt * 4 + rg) * S::KS;
 #pragma unroll 8
                     for (int ch = 0; ch < CH; ++ch) {
-                        const ulonglong2 k2 = *reinterpret_cast<const ulonglong2*>(ks + key * S::KS + ch * 4);
+                        const ulonglong2 ka = *reinterpret_cast<const ulonglong2*>(k0 + ch * 4), kb = *reinterpret_cast<const ulonglong2*>(k0 + 8 * S::KS + ch * 4);
 #pragma unroll
                         for (int j = 0; j < JN; ++j) {
-                            const int row = (2 * j + half) * 4 + rg;
-                            const ulonglong2 q2 = *reinterpret_cast<const ulonglong2*>(q_s + row * S::KS + ch * 4);
-                            s2[j] = cf_fma2(k2.x, q2.x, s2[j]);
-                            s2[j] = cf_fma2(k2.y, q2.y, s2[j]);
+                            const ulonglong2 q2 = *reinterpret_cast<const ulonglong2*>(q0 + j * 16 * S::KS + ch * 4);
+                            s2[j][0] = cf_fma2(ka.x, q2.x, s2[j][0]);
+                            s2[j][1] = cf_fma2(kb.x, q2.x, s2[j][1]);
+                            s2[j][0] = cf_fma2(ka.y, q2.y, s2[j][0]);
+                            s2[j][1] = cf_fma2(kb.y, q2.y, s2[j][1]);
                         }
                     }
-                    float x[JN], top[JN], corr[JN];
+                    float x[JN][2], top[JN], corr[JN];
 #pragma unroll
                     for (int j = 0; j < JN; ++j) {
-                        const float2 f = cf_both(s2[j]);
-                        x[j] = top[j] = k_at <= lim[j] && lim[j] - k_at < reach ? (f.x + f.y) * a.scale2 : -INFINITY;
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float2 f = cf_both(s2[j][e]);
+                            const int at = k_at + 8 * e;
+                            x[j][e] = at <= lim[j] && lim[j] - at < reach ? (f.x + f.y) * a.scale2 : -INFINITY;
+                        }
+                        top[j] = fmaxf(x[j][0], x[j][1]);
                     }
 #pragma unroll
                     for (int b = 1; b < 8; b <<= 1)
@@ -200,9 +208,13 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
                             m_run[j] = top[j];
                             moved = true;
                         }
-                        const float p = x[j] == -INFINITY ? 0.f : cf_exp2(x[j] - m_run[j]);
-                        l_run[j] = l_run[j] * corr[j] + p;          // of this lane's keys
-                        p_s[key * S::PS + j * 4 + rg] = p;
+                        l_run[j] *= corr[j];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float p = x[j][e] == -INFINITY ? 0.f : cf_exp2(x[j][e] - m_run[j]);
+                            l_run[j] += p;                          // of this lane's keys
+                            p_s[(key + 8 * e) * S::PS + j * 4 + rg] = p;
+                        }
                     }
                     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -216,8 +228,8 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
                             }
                     }
                     __syncwarp();
-#pragma unroll 4
-                    for (int kk = 0; kk < 8; ++kk) {
+#pragma unroll 8
+                    for (int kk = 0; kk < 16; ++kk) {
                         float v[CL];
                         if constexpr (CL == 2) {
                             const float2 t = *reinterpret_cast<const float2*>(vs + kk * D + lane * 2);
@@ -246,30 +258,28 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
                 }
             }
         };
-        const int fours = (((rows + 3) >> 2) + 1 - half) >> 1;      // of this warp: every other four of the item's
+        const int fours = (((rows + 3) >> 2) + 3 - mt) >> 2;      // of this warp: every fourth four of the item's
         if (fours <= 0) walk(CfInt<0>());
         else if (fours == 1) walk(CfInt<1>());
-        else if (fours == 2 || RJ == 2) walk(CfInt<2>());
-        else if (fours == 3) walk(CfInt<RJ < 3 ? RJ : 3>());
-        else walk(CfInt<RJ>());
+        else walk(CfInt<FW>());
         asm volatile("cp.async.wait_group 0;\n" ::);
 
         // the groups meet: every row's maximum, then outputs and sums
 #pragma unroll
-        for (int j = 0; j < RJ; ++j) {
+        for (int j = 0; j < FW; ++j) {
             float l = l_run[j];
 #pragma unroll
             for (int b = 1; b < 8; b <<= 1) l += __shfl_xor_sync(0xffffffffu, l, b);
-            if (key == 0) *reinterpret_cast<float2*>(ml + (group * M + (2 * j + half) * 4 + rg) * 2) = make_float2(m_run[j], l);
+            if (key == 0) *reinterpret_cast<float2*>(ml + (group * M + (mt + 4 * j) * 4 + rg) * 2) = make_float2(m_run[j], l);
         }
         __syncthreads();
         w = place_in_line;
         float* o_s = cf_smem;                     // [NG][M][D]
 #pragma unroll
-        for (int j = 0; j < RJ; ++j)
+        for (int j = 0; j < FW; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int row = (2 * j + half) * 4 + e;
+                const int row = (mt + 4 * j) * 4 + e;
                 if (row >= w.tile.rows) continue;
                 float f[CL];
 #pragma unroll
