@@ -9,7 +9,16 @@
 // warps an SM) waited for its own instructions: 5.3 cycles each, at a quarter of the tensor pipe and half of the memory's rate.
 // Scores, maxima and sums are float32, a row's reference maximum moves by more than 8 (log2 units) or not at all; probabilities are rounded
 // to bfloat16 for the product with the values, as the values are, which the result's own rounding hides (2^-9 each on average).
+//
+// Two ways to share the work out.  The line of attention_chunks.cuh balances any lengths, at the price of a second kernel.  For few requests
+// with few keys that is a third of the call, so there a cluster of S blocks takes a (request, key head), each block a part of every item's
+// key tiles, and the parts are joined in the cluster's shared memory (one request of 5 tokens behind 1,000, 32 heads of 128: LINE us
+// by the line, CLUSTER by clusters; eight requests behind 500 to 2,000: LINE8 and CLUSTER8).
+#include <cooperative_groups.h>
+
 #include "attention_chunks.cuh"
+
+namespace cg = cooperative_groups;
 
 #define CB_GROUPS 4
 #define CB_RESCALE_STEP 8.0f
@@ -26,7 +35,8 @@ template <int D, int GW> struct CbShape {
     static constexpr int ring_bytes = CB_GROUPS * NST * stage * 2;
     static constexpr int blocks = GW == 4 ? 1 : 2;    // an SM: 16 warps of 128 registers, or eight of 255
     static constexpr int o_bytes = CB_GROUPS * M * D * 4;      // the groups' outputs meet in the ring's memory
-    static constexpr int q_off = ring_bytes > o_bytes ? ring_bytes : o_bytes, ml_off = q_off + M * D * 2, bytes = ml_off + CB_GROUPS * M * 2 * 4;
+    static constexpr int q_off = ring_bytes > o_bytes ? ring_bytes : o_bytes, ml_off = q_off + M * D * 2;
+    static constexpr int block_ml_off = ml_off + CB_GROUPS * M * 2 * 4, bytes = block_ml_off + M * 2 * 4;      // the block's own maxima and sums, for its cluster
 };
 
 __device__ __forceinline__ void cb_fetch(unsigned dst, const void* src, bool there) {
@@ -55,20 +65,42 @@ __device__ __forceinline__ float cb_exp2(float x) {
 // byte offset of row r, 16-byte piece c of rows of D elements: pieces are permuted so that eight rows' pieces lie in different banks
 template <int D> __device__ __forceinline__ unsigned cb_at(int row, int piece) { return (unsigned)(row * (D * 2) + ((piece ^ (row & 7)) << 4)); }
 
-template <int D, int GW>
-__global__ void __launch_bounds__(CbShape<D, GW>::threads, CbShape<D, GW>::blocks) chunk_bf16_kernel(const ChArgs a) {
+// The walk of a block in a cluster: its part of the tiles of row tile `m` (maybe none).
+template <int M, int KT> __device__ __forceinline__ void cb_part(const ChArgs& a, ChWalk& w, int m, int rank, int S) {
+    w.m = m;
+    w.tile = ch_tile<M, KT>(a, w.req, m);
+    w.per = (w.tile.tiles + S - 1) / S;
+    w.k = rank * w.per;
+    w.left = max(0, min(w.per, w.tile.tiles - w.k));
+}
+
+template <int D, int GW, bool CLUSTER>
+__global__ void __launch_bounds__(CbShape<D, GW>::threads, CbShape<D, GW>::blocks) chunk_bf16_kernel(const ChArgs a, int S_blocks) {
     using S = CbShape<D, GW>;
     constexpr int M = S::M, KT = S::KT, CK = S::CK, PC = D / 8, NST = S::NST, THREADS = S::threads, TPK = S::TPK;
     constexpr int KEYS = 32 * GW / TPK, ROUNDS = CK / KEYS;      // keys that the group's threads copy at a time, and how often
     extern __shared__ __align__(128) unsigned char cb_smem[];
     __shared__ ChShared sh;
+    __shared__ ChWalk place_in_line;      // while the registers hold rows' outputs
     pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = warp / GW, mt = warp % GW, gt = mt * 32 + lane;
-    const int c = blockIdx.x, C = gridDim.x;
-    if (tid == 0) a.meta[2 * c] = make_int4(0, 0, 0, 0);
+    const int c = blockIdx.x, C = gridDim.x, rank = CLUSTER ? c % S_blocks : 0;
     ChWalk w;
-    if (!ch_begin<THREADS, M, KT>(a, c, C, &sh, w)) return;
+    if constexpr (CLUSTER) {
+        const int item = c / S_blocks;
+        unsigned bad_lengths = 0;
+        w.r = item / a.K;
+        w.kh = item - w.r * a.K;
+        w.req = ch_req(a, w.r, &bad_lengths);
+        w.s0 = a.q_start[w.r];
+        if (bad_lengths && tid == 0 && rank == 0 && w.kh == 0) atomicOr(a.err, bad_lengths);
+        if (w.req.n == 0) return;                 // the whole cluster
+        cb_part<M, KT>(a, w, 0, rank, S_blocks);
+    } else {
+        if (tid == 0) a.meta[2 * c] = make_int4(0, 0, 0, 0);
+        if (!ch_begin<THREADS, M, KT>(a, c, C, &sh, w)) return;
+    }
     const unsigned smem = (unsigned)__cvta_generic_to_shared(cb_smem);
     const unsigned ring = smem + group * NST * S::stage * 2, q_s = smem + S::q_off;
     float* ml = reinterpret_cast<float*>(cb_smem + S::ml_off);      // [groups][M][2]
@@ -81,7 +113,7 @@ __global__ void __launch_bounds__(CbShape<D, GW>::threads, CbShape<D, GW>::block
     unsigned bad = 0;
 
     for (;;) {
-        const int n = ch_share(w);
+        const int n = CLUSTER ? w.left : ch_share(w);
         const ChTile tl = w.tile;
         const int c0 = w.req.c, s0 = w.s0, hi = c0 + tl.i1 + 1;
         const int* bt = a.table + (size_t)w.r * a.W;
@@ -146,6 +178,7 @@ __global__ void __launch_bounds__(CbShape<D, GW>::threads, CbShape<D, GW>::block
             for (int e = 0; e < 4; ++e) o[x][e] = 0.f;
         const int last_low = a.window > 0 ? c0 + tl.i1 - a.window + 1 : 0;      // first key that the last row sees
 
+        if (tid == 0) place_in_line = w;
         int slot = 0;
         for (int i = 0; i < n; ++i) {
             asm volatile("cp.async.wait_group %0;\n" ::"n"(NST - 2));
@@ -241,6 +274,7 @@ __global__ void __launch_bounds__(CbShape<D, GW>::threads, CbShape<D, GW>::block
         __syncthreads();
 
         // the groups meet
+        w = place_in_line;
         float* o_s = reinterpret_cast<float*>(cb_smem);      // [groups][M][D]
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -249,15 +283,15 @@ __global__ void __launch_bounds__(CbShape<D, GW>::threads, CbShape<D, GW>::block
             l += __shfl_xor_sync(0xffffffffu, l, 1);
             l += __shfl_xor_sync(0xffffffffu, l, 2);
             if ((lane & 3) == 0) *reinterpret_cast<float2*>(ml + (group * M + row) * 2) = make_float2(m_run[e], l);
-            if (row < tl.rows)
+            if (row < w.tile.rows)
 #pragma unroll
                 for (int x = 0; x < D / 8; ++x)
                     *reinterpret_cast<float2*>(o_s + (group * M + row) * D + ((x * 8 + col) ^ ((row & 3) << 3))) = make_float2(o[x][2 * e], o[x][2 * e + 1]);
         }
         __syncthreads();
-        const bool begins = w.k == 0, ends = w.k + n == tl.tiles;
+        const bool begins = w.k == 0, ends = w.k + n == w.tile.tiles;
         const size_t place = (size_t)2 * c + (begins ? 1 : 0);
-        for (int i = tid; i < tl.rows * (D / 4); i += THREADS) {
+        for (int i = tid; i < w.tile.rows * (D / 4); i += THREADS) {
             const int row = i / (D / 4), e = (i % (D / 4)) * 4;
             float2 g[CB_GROUPS];
             float m = -INFINITY, l = 0.f;
@@ -274,40 +308,114 @@ __global__ void __launch_bounds__(CbShape<D, GW>::threads, CbShape<D, GW>::block
                 l += f * g[x].y;
                 y.x += f * z.x, y.y += f * z.y, y.z += f * z.z, y.w += f * z.w;
             }
-            if (begins && ends) {
+            if constexpr (CLUSTER) {              // for the other blocks, where group 0's outputs were (this thread's alone to read)
+                *reinterpret_cast<float4*>(o_s + row * D + (e ^ ((row & 3) << 3))) = y;
+                if (e == 0) *reinterpret_cast<float2*>(cb_smem + S::block_ml_off + row * 8) = make_float2(m, l);
+            } else if (begins && ends) {
                 const float inv = ch_inverse(l);
-                const int full = tl.row0 + row, t = ch_over(full, a.by_g), h = w.kh * a.G + full - t * a.G;
-                store4<bf16>(reinterpret_cast<bf16*>(a.out) + ((size_t)(s0 + t) * a.H + h) * D + e,
+                const int full = w.tile.row0 + row, t = ch_over(full, a.by_g), h = w.kh * a.G + full - t * a.G;
+                store4<bf16>(reinterpret_cast<bf16*>(a.out) + ((size_t)(w.s0 + t) * a.H + h) * D + e,
                              make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
             } else {
                 *reinterpret_cast<float4*>(a.part_o + (place * M + row) * D + e) = y;
                 if (e == 0) *reinterpret_cast<float2*>(a.part_ml + (place * M + row) * 2) = make_float2(m, l);
             }
         }
-        if (begins && !ends && tid == 0) ch_leave(a, w, c, n);
-        if (!ch_next<M, KT>(a, w, n)) break;
-        __syncthreads();                      // the ring's memory is the next item's
+        if constexpr (CLUSTER) {
+            cg::cluster_group cluster = cg::this_cluster();
+            cluster.sync();
+            for (int i = rank * THREADS + tid; i < w.tile.rows * (D / 4); i += S_blocks * THREADS) {
+                const int row = i / (D / 4), e = (i % (D / 4)) * 4;
+                float m = -INFINITY, l = 0.f;
+                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+                for (int b0 = 0; b0 < S_blocks; b0 += 4) {      // four blocks at a time, so that their reads are under way together
+                    float2 g[4];
+                    float4 z[4];
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const unsigned char* at = cluster.map_shared_rank(cb_smem, min(b0 + b, S_blocks - 1));
+                        g[b] = *reinterpret_cast<const float2*>(at + S::block_ml_off + row * 8);
+                        z[b] = *reinterpret_cast<const float4*>(at + (row * D + (e ^ ((row & 3) << 3))) * 4);
+                        if (b0 + b >= S_blocks) g[b].x = -INFINITY;
+                    }
+                    const float top = fmaxf(m, fmaxf(fmaxf(g[0].x, g[1].x), fmaxf(g[2].x, g[3].x)));
+                    const float was = m == -INFINITY ? 0.f : cb_exp2(m - top);
+                    l *= was;
+                    y.x *= was, y.y *= was, y.z *= was, y.w *= was;
+#pragma unroll
+                    for (int b = 0; b < 4; ++b)
+                        if (g[b].x != -INFINITY) {
+                            const float f = cb_exp2(g[b].x - top);
+                            l += f * g[b].y;
+                            y.x += f * z[b].x, y.y += f * z[b].y, y.z += f * z[b].z, y.w += f * z[b].w;
+                        }
+                    m = top;
+                }
+                const float inv = ch_inverse(l);
+                const int full = w.tile.row0 + row, t = ch_over(full, a.by_g), h = w.kh * a.G + full - t * a.G;
+                store4<bf16>(reinterpret_cast<bf16*>(a.out) + ((size_t)(w.s0 + t) * a.H + h) * D + e,
+                             make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
+            }
+            cluster.sync();                   // the others have read this block's memory
+            if ((w.m + 1) * M >= w.req.n * a.G) break;
+            cb_part<M, KT>(a, w, w.m + 1, rank, S_blocks);
+        } else {
+            if (begins && !ends && tid == 0) ch_leave(a, w, c, n);
+            if (!ch_next<M, KT>(a, w, n)) break;
+            __syncthreads();                  // the ring's memory is the next item's
+        }
     }
     if (bad) atomicOr(a.err, bad);
 }
 
 template <int D, int GW> static int launch_chunk_bf16(const ChArgs& a, cudaStream_t st) {
     using S = CbShape<D, GW>;
-    auto kern = chunk_bf16_kernel<D, GW>;
+    auto kern = chunk_bf16_kernel<D, GW, false>;
     const int C = S::blocks * aie_sm_count();
     static unsigned long long done = 0;
     ch_prepare(kern, S::bytes, &done);
-    const int rc = (int)launch_pdl(kern, dim3(C), dim3(S::threads), S::bytes, st, a);
+    const int rc = (int)launch_pdl(kern, dim3(C), dim3(S::threads), S::bytes, st, a, 1);
     if (rc) return rc;
     return launch_chunk_join<bf16, S::M, D>(a, C, st);
 }
 
-// rows: 16, 32 or 64 of an item.  The scratch is [2 * blocks * rows * (d + 2)] floats and [2 * blocks] int4; blocks: two an SM, one for 64 rows.
-extern "C" int aie_attention_chunks_bf16(const ChCall* call, int rows, cudaStream_t stream) {
+template <int D, int GW> static int launch_chunk_clusters(const ChArgs& a, int blocks, cudaStream_t st) {
+    using S = CbShape<D, GW>;
+    auto kern = chunk_bf16_kernel<D, GW, true>;
+    static unsigned long long done = 0;
+    ch_prepare(kern, S::bytes, &done);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.R * a.K * blocks));
+    cfg.blockDim = dim3(S::threads);
+    cfg.dynamicSmemBytes = S::bytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)blocks;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return (int)cudaLaunchKernelEx(&cfg, kern, a, blocks);
+}
+
+// rows: 16, 32 or 64 of an item.  clusters 0: by the line, with a scratch of [2 * blocks * rows * (d + 2)] floats and [2 * blocks] int4, blocks:
+// two an SM, one for 64 rows.  clusters 2 .. 8: blocks of a cluster for every request and key head (16 or 32 rows, no scratch).
+extern "C" int aie_attention_chunks_bf16(const ChCall* call, int rows, int clusters, cudaStream_t stream) {
     if (call->R <= 0 || call->T <= 0) return 0;
     ChArgs a;
     const int rc = ch_args(call, 16, 64, &a);
     if (rc) return rc;
+    if (clusters) {
+        if (clusters < 2 || clusters > 8 || (long long)a.R * a.K * clusters > 0x7fffffff) return AIE_UNSUPPORTED;
+        if (a.d == 64 && rows == 16) return launch_chunk_clusters<64, 1>(a, clusters, stream);
+        if (a.d == 64 && rows == 32) return launch_chunk_clusters<64, 2>(a, clusters, stream);
+        if (a.d == 128 && rows == 16) return launch_chunk_clusters<128, 1>(a, clusters, stream);
+        if (a.d == 128 && rows == 32) return launch_chunk_clusters<128, 2>(a, clusters, stream);
+        return AIE_UNSUPPORTED;
+    }
     if (a.d == 64 && rows == 16) return launch_chunk_bf16<64, 1>(a, stream);
     if (a.d == 64 && rows == 32) return launch_chunk_bf16<64, 2>(a, stream);
     if (a.d == 64 && rows == 64) return launch_chunk_bf16<64, 4>(a, stream);

@@ -137,7 +137,7 @@ int (*step_tables_fn)(const StArgs*, cudaStream_t) = nullptr;
 int (*write_fn)(const CwArgs*, cudaStream_t) = nullptr;
 int (*verify_fn)(const VdArgs*, cudaStream_t) = nullptr;
 int (*chunks_f32_fn)(const ChCall*, int, cudaStream_t) = nullptr;
-int (*chunks_mma_fn)(const ChCall*, int, cudaStream_t) = nullptr;
+int (*chunks_mma_fn)(const ChCall*, int, int, cudaStream_t) = nullptr;
 int (*chunks_tc_fn)(const ChCall*, cudaStream_t) = nullptr;
 int sm_count = 0;
 
@@ -269,9 +269,10 @@ PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// The forms of the attention: 0 float32 (and bfloat16 that the others do not take), 1, 2, 4 mma.sync with 16, 32, 64 rows an item, 3 tcgen05.
+// The forms of the attention: 0 float32 (and bfloat16 that the others do not take); 1, 2, 4 mma.sync with 16, 32, 64 rows an item; 3 tcgen05;
+// 16 * S + 1, 16 * S + 2 mma.sync with 16, 32 rows an item and clusters of S blocks.
 // Rows of queries that a request has for a key head, on average, decide between those that take a call.
-int chunk_form(int code, const Pools& p, double rows) {
+int chunk_form(int code, const Pools& p, int64_t R, int64_t W, double rows) {
     if (code != 1 || (p.d != 64 && p.d != 128)) return 0;
     if (rows > 32 && p.P % 8 == 0 && (128 % p.P == 0 || p.P % 128 == 0) && p.N * p.K * p.P / 8 < 0x7fffffff) return 3;
     return rows <= 16 ? 1 : 2;
@@ -317,19 +318,22 @@ PyObject* paged_attention_chunks(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (T && R) {
             const int64_t G = H / p.K;
             if (!sm_count) sm_count = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-            if (form < 0) form = chunk_form(p.code, p, (double)T * G / R);
+            if (form < 0) form = chunk_form(p.code, p, R, W, (double)T * G / R);
             const int64_t wide = form ? p.d : p.d <= 64 ? 64 : p.d <= 128 ? 128 : 256;
+            const int clusters = (int)(form >> 4);
+            form &= 15;
             const int64_t M = form == 3 ? 256 : form == 4 ? 64 : form == 1 || (form == 0 && wide == 256) ? 16 : 32;
             const int64_t blocks = sm_count * (form == 1 || form == 2 ? 2 : 1), parts = 2 * blocks * M;
             // parts [parts][wide], their maxima and sums [parts][2], what is to be joined [blocks][2] int4
-            at::Tensor scratch = fresh({parts * (wide + 2) + 8 * blocks}, at::kFloat, q);
-            float* s = scratch.data_ptr<float>();
+            at::Tensor scratch;
+            if (!clusters) scratch = fresh({parts * (wide + 2) + 8 * blocks}, at::kFloat, q);
+            float* s = clusters ? nullptr : scratch.data_ptr<float>();
             const ChCall call = {q.data_ptr(), kp.data_ptr(), vp.data_ptr(), out.data_ptr(), start.data_ptr(), len.data_ptr(), ctx.data_ptr(),
                                  table.data_ptr(), s, s + parts * wide, s + parts * (wide + 2), q.stride(0), q.stride(1), (int)R, (int)W, (int)T,
                                  (int)p.N, (int)p.P, (int)H, (int)p.K, (int)G, (int)p.d, (int)window, (float)(scale * 1.4426950408889634), err.data_ptr()};
             launched(w, form == 3   ? loaded(chunks_tc_fn, "aie_attention_chunks_tc")(&call, st)
                         : form == 0 ? loaded(chunks_f32_fn, "aie_attention_chunks_f32")(&call, p.code, st)
-                                    : loaded(chunks_mma_fn, "aie_attention_chunks_bf16")(&call, (int)M, st));
+                                    : loaded(chunks_mma_fn, "aie_attention_chunks_bf16")(&call, (int)M, clusters, st));
         }
         return THPVariable_Wrap(std::move(out));
     });
