@@ -203,53 +203,64 @@ __device__ __forceinline__ void ch_leave(const ChArgs& a, const ChWalk& w, int c
 }
 __device__ __forceinline__ float ch_inverse(float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); }      // of a row's sum; a row that sees nothing is zero
 
-// Joins the parts of the item that block c began: out = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p.  A thread has four columns of a row.
-template <typename T, int M, int D>
-__global__ void __launch_bounds__(256) chunk_join_kernel(const ChArgs a) {
+// Joins the parts of the items that blocks c .. c + PER - 1 began: out = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p, four columns of a row a
+// thread.  Items of 256 rows take 32 blocks, so that one in sixty parts does not take eight of them 30 us, and a block looks at
+// four of them, so that there are no more blocks than the machine holds at once (a list of the items with parts, made by every
+// block, cost 4 us).
+template <typename T, int M, int D, int PER>
+__global__ void __launch_bounds__(256) chunk_join_kernel(const ChArgs a, int C) {
     pdl_launch_dependents();
     pdl_wait();
-    const int c = blockIdx.x;
-    const int4 it = a.meta[2 * c], more = a.meta[2 * c + 1];
-    if (it.w == 0) return;
     constexpr int CH = D / 4;
-    for (int i = blockIdx.y * 256 + threadIdx.x; i < it.z * CH; i += gridDim.y * 256) {
-        const int row = i / CH, e = (i - row * CH) * 4;
-        if (e >= a.d) continue;
-        // part 0 lies in block c's place for items begun, part p in block c + p's for items continued
-        const float* ml = a.part_ml + ((size_t)2 * c * M + row) * 2;
-        const float* po = a.part_o + ((size_t)2 * c * M + row) * D + e;
-        float m = -INFINITY, l = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        // eight parts at a time, so that their loads are under way together
-        for (int p0 = 0; p0 < it.w; p0 += 8) {
-            float2 g[8];
-            float4 x[8];
+    int4 its[PER];
 #pragma unroll
-            for (int p = 0; p < 8; ++p) {
-                const bool there = p0 + p < it.w;
-                const size_t place = there ? (p0 + p == 0 ? 1 : 2 * (p0 + p)) : 1;
-                g[p] = there ? *reinterpret_cast<const float2*>(ml + place * (M * 2)) : make_float2(-INFINITY, 0.f);
-                x[p] = *reinterpret_cast<const float4*>(po + place * ((size_t)M * D));
+    for (int x = 0; x < PER; ++x) its[x] = blockIdx.x * PER + x < C ? a.meta[2 * (blockIdx.x * PER + x)] : make_int4(0, 0, 0, 0);
+#pragma unroll 1
+    for (int x = 0; x < PER; ++x) {
+        int4 it = its[0];
+#pragma unroll
+        for (int y = 1; y < PER; ++y)
+            if (y == x) it = its[y];
+        if (it.w == 0) continue;
+        const int c = blockIdx.x * PER + x, s0 = a.meta[2 * c + 1].x;
+        for (int i = blockIdx.y * 256 + threadIdx.x; i < it.z * CH; i += gridDim.y * 256) {
+            const int row = i / CH, e = (i - row * CH) * 4;
+            if (e >= a.d) continue;
+            // part 0 lies in block c's place for items begun, part p in block c + p's for items continued
+            const float* ml = a.part_ml + ((size_t)2 * c * M + row) * 2;
+            const float* po = a.part_o + ((size_t)2 * c * M + row) * D + e;
+            float m = -INFINITY, l = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int p0 = 0; p0 < it.w; p0 += 8) {       // eight parts at a time, so that their loads are under way together
+                float2 g[8];
+                float4 z[8];
+#pragma unroll
+                for (int p = 0; p < 8; ++p) {
+                    const bool there = p0 + p < it.w;
+                    const size_t place = there ? (p0 + p == 0 ? 1 : 2 * (p0 + p)) : 1;
+                    g[p] = there ? *reinterpret_cast<const float2*>(ml + place * (M * 2)) : make_float2(-INFINITY, 0.f);
+                    if (there) z[p] = *reinterpret_cast<const float4*>(po + place * ((size_t)M * D));
+                }
+                float top = m;
+#pragma unroll
+                for (int p = 0; p < 8; ++p) top = fmaxf(top, g[p].x);
+                const float was = m == -INFINITY ? 0.f : exp2f(m - top);
+                l *= was;
+                o.x *= was, o.y *= was, o.z *= was, o.w *= was;
+#pragma unroll
+                for (int p = 0; p < 8; ++p) {
+                    if (g[p].x == -INFINITY) continue;
+                    const float f = exp2f(g[p].x - top);
+                    l += f * g[p].y;
+                    o.x += f * z[p].x, o.y += f * z[p].y, o.z += f * z[p].z, o.w += f * z[p].w;
+                }
+                m = top;
             }
-            float top = m;
-#pragma unroll
-            for (int p = 0; p < 8; ++p) top = fmaxf(top, g[p].x);
-            const float was = m == -INFINITY ? 0.f : exp2f(m - top);
-            l *= was;
-            o.x *= was, o.y *= was, o.z *= was, o.w *= was;
-#pragma unroll
-            for (int p = 0; p < 8; ++p) {
-                if (g[p].x == -INFINITY) continue;
-                const float f = exp2f(g[p].x - top);
-                l += f * g[p].y;
-                o.x += f * x[p].x, o.y += f * x[p].y, o.z += f * x[p].z, o.w += f * x[p].w;
-            }
-            m = top;
+            const float inv = ch_inverse(l);
+            const int full = it.y + row, tok = ch_over(full, a.by_g), h = it.x * a.G + full - tok * a.G;
+            store4<T>(reinterpret_cast<T*>(a.out) + ((size_t)(s0 + tok) * a.H + h) * a.d + e,
+                      make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
         }
-        const float inv = ch_inverse(l);
-        const int full = it.y + row, tok = ch_over(full, a.by_g), h = it.x * a.G + full - tok * a.G;
-        store4<T>(reinterpret_cast<T*>(a.out) + ((size_t)(more.x + tok) * a.H + h) * a.d + e,
-                  make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
     }
 }
 // What a kernel is told once on each device: the shared memory it takes (0: none), and that it wants as much of it an SM as there is.
@@ -262,9 +273,9 @@ template <typename F> static void ch_prepare(F kern, int bytes, unsigned long lo
 }
 // ... with as much shared memory an SM as the kernel before it, which would otherwise have to leave the SM before it changes
 template <typename T, int M, int D> static int launch_chunk_join(const ChArgs& a, int C, cudaStream_t st) {
-    auto kern = chunk_join_kernel<T, M, D>;
+    constexpr int PER = M > 32 ? 4 : 1;
+    auto kern = chunk_join_kernel<T, M, D, PER>;
     static unsigned long long done = 0;
     ch_prepare(kern, 0, &done);
-    constexpr int blocks = M * D / 4 / 256;
-    return (int)launch_pdl(kern, dim3(C, blocks > 8 ? 8 : blocks), dim3(256), 0, st, a);
+    return (int)launch_pdl(kern, dim3((C + PER - 1) / PER, M * D / 4 / 256), dim3(256), 0, st, a, C);
 }
