@@ -1,19 +1,20 @@
-// Attention of new tokens over a paged cache (see attention_chunks.cuh) in bfloat16, heads of 64 and 128, for items of 16, 32 or 64 rows:
+// Attention of new tokens over a paged cache (see attention_chunks.cuh) in bfloat16, heads of 64 and 128, for items of 32 rows:
 // a few drafted tokens of a request times the query heads of a key head; any page size.
 //   o = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m),   x_j = (q . k_j) * scale * log2 e
 //
-// Products go through mma.sync, whose tiles of 16 rows fit 4 tokens of 4 heads.  A block has four groups of warps; of every key
+// Products go through mma.sync, whose tiles of 16 rows fit 4 tokens of 4 heads.  A block has four groups of two warps; of every key
 // tile each group takes CK keys of its own through a ring of its own (cp.async, stages of 8 KB), and each warp of a group has 16 rows of
 // the item and reads the group's keys and values.  Groups meet only at an item's end, where their outputs are added up in shared memory.
-// What bounds it: with every 16 rows a warp of its own, reading keys and values once.  One warp for 32 rows (255 registers, eight
-// warps an SM) waited for its own instructions: 5.3 cycles each, at a quarter of the tensor pipe and half of the memory's rate.
+// What bounds it: reading keys and values once, and 10 us of a small call's chain of waits (lengths, pages, rows, outputs that meet).  One
+// warp for 32 rows (255 registers, eight warps an SM) waited for its own instructions, 5.3 cycles each, at half of the memory's rate
+// (56 requests of heads of 64: 84 us, now 71); items of 16 rows or of 64 were at most a twentieth better anywhere.
 // Scores, maxima and sums are float32, a row's reference maximum moves by more than 8 (log2 units) or not at all; probabilities are rounded
 // to bfloat16 for the product with the values, as the values are, which the result's own rounding hides (2^-9 each on average).
 //
 // Two ways to share the work out.  The line of attention_chunks.cuh balances any lengths, at the price of a second kernel.  For few requests
 // with few keys that is a third of the call, so there a cluster of S blocks takes a (request, key head), each block a part of every item's
-// key tiles, and the parts are joined in the cluster's shared memory (one request of 5 tokens behind 1,000, 32 heads of 128: LINE us
-// by the line, CLUSTER by clusters; eight requests behind 500 to 2,000: LINE8 and CLUSTER8).
+// key tiles, and the parts are joined in the cluster's shared memory (one request of 5 tokens behind 1,000, 32 heads of 128: 10.3 us
+// by the line, 7.3 by clusters of eight; eight requests behind 500 to 2,000: 20.0, and 18.5 by clusters of four).
 #include <cooperative_groups.h>
 
 #include "attention_chunks.cuh"
@@ -21,19 +22,20 @@
 namespace cg = cooperative_groups;
 
 #define CB_GROUPS 4
+#define CB_GW 2                // warps of a group
 #define CB_RESCALE_STEP 8.0f
 
-// GW: warps of a group
-template <int D, int GW> struct CbShape {
+template <int D> struct CbShape {
+    static constexpr int GW = CB_GW;
     static constexpr int M = 16 * GW;                 // rows of an item
     static constexpr int threads = CB_GROUPS * GW * 32;
     static constexpr int CK = D == 64 ? 32 : 16;      // keys of a group's stage
     static constexpr int KT = CB_GROUPS * CK;         // keys of a tile
     static constexpr int NST = 3;
     static constexpr int stage = 2 * CK * D;          // elements: keys, then values
-    static constexpr int TPK = 32 * GW / CK < 2 ? 2 : 32 * GW / CK;      // threads that copy a key: at least a 32-byte sector at a time
+    static constexpr int TPK = 32 * GW / CK;          // threads that copy a key
     static constexpr int ring_bytes = CB_GROUPS * NST * stage * 2;
-    static constexpr int blocks = GW == 4 ? 1 : 2;    // an SM: 16 warps of 128 registers, or eight of 255
+    static constexpr int blocks = 2;                  // an SM: 16 warps of 128 registers
     static constexpr int o_bytes = CB_GROUPS * M * D * 4;      // the groups' outputs meet in the ring's memory
     static constexpr int q_off = ring_bytes > o_bytes ? ring_bytes : o_bytes, ml_off = q_off + M * D * 2;
     static constexpr int block_ml_off = ml_off + CB_GROUPS * M * 2 * 4, bytes = block_ml_off + M * 2 * 4;      // the block's own maxima and sums, for its cluster
@@ -74,11 +76,10 @@ template <int M, int KT> __device__ __forceinline__ void cb_part(const ChArgs& a
     w.left = max(0, min(w.per, w.tile.tiles - w.k));
 }
 
-template <int D, int GW, bool CLUSTER>
-__global__ void __launch_bounds__(CbShape<D, GW>::threads, CbShape<D, GW>::blocks) chunk_bf16_kernel(const ChArgs a, int S_blocks) {
-    using S = CbShape<D, GW>;
-    constexpr int M = S::M, KT = S::KT, CK = S::CK, PC = D / 8, NST = S::NST, THREADS = S::threads, TPK = S::TPK;
-    constexpr int KEYS = 32 * GW / TPK, ROUNDS = CK / KEYS;      // keys that the group's threads copy at a time, and how often
+template <int D, bool CLUSTER>
+__global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk_bf16_kernel(const ChArgs a, int S_blocks) {
+    using S = CbShape<D>;
+    constexpr int GW = CB_GW, M = S::M, KT = S::KT, CK = S::CK, PC = D / 8, NST = S::NST, THREADS = S::threads, TPK = S::TPK;
     extern __shared__ __align__(128) unsigned char cb_smem[];
     __shared__ ChShared sh;
     __shared__ ChWalk place_in_line;      // while the registers hold rows' outputs
@@ -121,17 +122,12 @@ __global__ void __launch_bounds__(CbShape<D, GW>::threads, CbShape<D, GW>::block
         const int low_all = a.window > 0 ? c0 + tl.i0 - a.window + 1 : 0;      // first key that any row sees
 
         // this thread copies every TPK-th piece of its key of the stage; the pages of the next two stages' keys are read ahead
-        auto key_of = [&](int i, int round) { return (kt0 + i) * KT + group * CK + round * KEYS + gt / TPK; };
-        auto page_of = [&](int i, int round) {
-            const int key = key_of(i, round);
+        auto key_of = [&](int i) { return (kt0 + i) * KT + group * CK + gt / TPK; };
+        auto page_of = [&](int i) {
+            const int key = key_of(i);
             return i < n && key < hi && key >= low_all ? __ldg(bt + ch_over(key, a.by_p)) : -1;
         };
-        int pages[ROUNDS], pages_next[ROUNDS];
-#pragma unroll
-        for (int x = 0; x < ROUNDS; ++x) {
-            pages[x] = page_of(0, x);
-            pages_next[x] = page_of(1, x);
-        }
+        int page = page_of(0), page_next = page_of(1);
         // queries of the item: they land with the first stage
         for (int i = tid; i < M * PC; i += THREADS) {
             const int row = i / PC, pc = i % PC;
@@ -142,24 +138,21 @@ __global__ void __launch_bounds__(CbShape<D, GW>::threads, CbShape<D, GW>::block
         auto issue = [&](int i, int slot) {
             if (i < n) {
                 const unsigned st = ring + slot * S::stage * 2;
-#pragma unroll
-                for (int x = 0; x < ROUNDS; ++x) {
-                    const int key = key_of(i, x), kk = x * KEYS + gt / TPK, page = pages[x];
-                    bool there = key < hi && key >= low_all;
-                    if (there && (page < 0 || page >= a.num_pages)) {
-                        bad |= AIE_DEV_PAGE_OOB;
-                        there = false;
-                    }
-                    const size_t off = there ? (((size_t)page * a.K + w.kh) * a.P + (key - ch_over(key, a.by_p) * a.P)) * D + gt % TPK * 8 : 0;
-#pragma unroll
-                    for (int y = 0; y < PC / TPK; ++y) {
-                        const unsigned to = st + cb_at<D>(kk, gt % TPK + y * TPK);
-                        cb_fetch(to, kp + off + y * TPK * 8, there);
-                        cb_fetch(to + CK * D * 2, vp + off + y * TPK * 8, there);
-                    }
-                    pages[x] = pages_next[x];
-                    pages_next[x] = page_of(i + 2, x);
+                const int key = key_of(i);
+                bool there = key < hi && key >= low_all;
+                if (there && (page < 0 || page >= a.num_pages)) {
+                    bad |= AIE_DEV_PAGE_OOB;
+                    there = false;
                 }
+                const size_t off = there ? (((size_t)page * a.K + w.kh) * a.P + (key - ch_over(key, a.by_p) * a.P)) * D + gt % TPK * 8 : 0;
+#pragma unroll
+                for (int y = 0; y < PC / TPK; ++y) {
+                    const unsigned to = st + cb_at<D>(gt / TPK, gt % TPK + y * TPK);
+                    cb_fetch(to, kp + off + y * TPK * 8, there);
+                    cb_fetch(to + CK * D * 2, vp + off + y * TPK * 8, there);
+                }
+                page = page_next;
+                page_next = page_of(i + 2);
             }
             asm volatile("cp.async.commit_group;\n" ::);
         };
@@ -183,8 +176,7 @@ __global__ void __launch_bounds__(CbShape<D, GW>::threads, CbShape<D, GW>::block
         for (int i = 0; i < n; ++i) {
             asm volatile("cp.async.wait_group %0;\n" ::"n"(NST - 2));
             // the stage is there for the whole group, and the group has read the one that the next copies go to
-            if (GW == 1) __syncwarp();
-            else asm volatile("bar.sync %0, %1;\n" ::"r"(1 + group), "n"(32 * GW) : "memory");
+            asm volatile("bar.sync %0, %1;\n" ::"r"(1 + group), "n"(32 * GW) : "memory");
             issue(i + NST - 1, slot == 0 ? NST - 1 : slot - 1);
             const unsigned ks = ring + slot * S::stage * 2, vs = ks + CK * D * 2;
             slot = slot + 1 == NST ? 0 : slot + 1;
@@ -369,9 +361,9 @@ __global__ void __launch_bounds__(CbShape<D, GW>::threads, CbShape<D, GW>::block
     if (bad) atomicOr(a.err, bad);
 }
 
-template <int D, int GW> static int launch_chunk_bf16(const ChArgs& a, cudaStream_t st) {
-    using S = CbShape<D, GW>;
-    auto kern = chunk_bf16_kernel<D, GW, false>;
+template <int D> static int launch_chunk_bf16(const ChArgs& a, cudaStream_t st) {
+    using S = CbShape<D>;
+    auto kern = chunk_bf16_kernel<D, false>;
     const int C = S::blocks * aie_sm_count();
     static unsigned long long done = 0;
     ch_prepare(kern, S::bytes, &done);
@@ -380,9 +372,9 @@ template <int D, int GW> static int launch_chunk_bf16(const ChArgs& a, cudaStrea
     return launch_chunk_join<bf16, S::M, D>(a, C, st);
 }
 
-template <int D, int GW> static int launch_chunk_clusters(const ChArgs& a, int blocks, cudaStream_t st) {
-    using S = CbShape<D, GW>;
-    auto kern = chunk_bf16_kernel<D, GW, true>;
+template <int D> static int launch_chunk_clusters(const ChArgs& a, int blocks, cudaStream_t st) {
+    using S = CbShape<D>;
+    auto kern = chunk_bf16_kernel<D, true>;
     static unsigned long long done = 0;
     ch_prepare(kern, S::bytes, &done);
     cudaLaunchConfig_t cfg = {};
@@ -401,26 +393,15 @@ template <int D, int GW> static int launch_chunk_clusters(const ChArgs& a, int b
     return (int)cudaLaunchKernelEx(&cfg, kern, a, blocks);
 }
 
-// rows: 16, 32 or 64 of an item.  clusters 0: by the line, with a scratch of [2 * blocks * rows * (d + 2)] floats and [2 * blocks] int4, blocks:
-// two an SM, one for 64 rows.  clusters 2 .. 8: blocks of a cluster for every request and key head (16 or 32 rows, no scratch).
-extern "C" int aie_attention_chunks_bf16(const ChCall* call, int rows, int clusters, cudaStream_t stream) {
+// clusters 0: by the line, with a scratch of [2 * blocks * 32 * (d + 2)] floats and [2 * blocks] int4, two blocks an SM.  clusters 2 .. 8: blocks of
+// a cluster for every request and key head, no scratch.
+extern "C" int aie_attention_chunks_bf16(const ChCall* call, int clusters, cudaStream_t stream) {
     if (call->R <= 0 || call->T <= 0) return 0;
     ChArgs a;
-    const int rc = ch_args(call, 16, 64, &a);
+    const int rc = ch_args(call, 32, 64, &a);
     if (rc) return rc;
-    if (clusters) {
-        if (clusters < 2 || clusters > 8 || (long long)a.R * a.K * clusters > 0x7fffffff) return AIE_UNSUPPORTED;
-        if (a.d == 64 && rows == 16) return launch_chunk_clusters<64, 1>(a, clusters, stream);
-        if (a.d == 64 && rows == 32) return launch_chunk_clusters<64, 2>(a, clusters, stream);
-        if (a.d == 128 && rows == 16) return launch_chunk_clusters<128, 1>(a, clusters, stream);
-        if (a.d == 128 && rows == 32) return launch_chunk_clusters<128, 2>(a, clusters, stream);
-        return AIE_UNSUPPORTED;
-    }
-    if (a.d == 64 && rows == 16) return launch_chunk_bf16<64, 1>(a, stream);
-    if (a.d == 64 && rows == 32) return launch_chunk_bf16<64, 2>(a, stream);
-    if (a.d == 64 && rows == 64) return launch_chunk_bf16<64, 4>(a, stream);
-    if (a.d == 128 && rows == 16) return launch_chunk_bf16<128, 1>(a, stream);
-    if (a.d == 128 && rows == 32) return launch_chunk_bf16<128, 2>(a, stream);
-    if (a.d == 128 && rows == 64) return launch_chunk_bf16<128, 4>(a, stream);
-    return AIE_UNSUPPORTED;
+    if (a.d != 64 && a.d != 128) return AIE_UNSUPPORTED;
+    if (!clusters) return a.d == 64 ? launch_chunk_bf16<64>(a, stream) : launch_chunk_bf16<128>(a, stream);
+    if (clusters < 2 || clusters > 8 || (long long)a.R * a.K * clusters > 0x7fffffff) return AIE_UNSUPPORTED;
+    return a.d == 64 ? launch_chunk_clusters<64>(a, clusters, stream) : launch_chunk_clusters<128>(a, clusters, stream);
 }

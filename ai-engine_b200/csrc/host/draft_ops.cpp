@@ -12,7 +12,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
-#include <cstdio>
+#include <algorithm>
 #include <initializer_list>
 #include <string>
 
@@ -137,7 +137,7 @@ int (*step_tables_fn)(const StArgs*, cudaStream_t) = nullptr;
 int (*write_fn)(const CwArgs*, cudaStream_t) = nullptr;
 int (*verify_fn)(const VdArgs*, cudaStream_t) = nullptr;
 int (*chunks_f32_fn)(const ChCall*, int, cudaStream_t) = nullptr;
-int (*chunks_mma_fn)(const ChCall*, int, int, cudaStream_t) = nullptr;
+int (*chunks_mma_fn)(const ChCall*, int, cudaStream_t) = nullptr;
 int (*chunks_tc_fn)(const ChCall*, cudaStream_t) = nullptr;
 int sm_count = 0;
 
@@ -269,13 +269,43 @@ PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// The forms of the attention: 0 float32 (and bfloat16 that the others do not take); 1, 2, 4 mma.sync with 16, 32, 64 rows an item; 3 tcgen05;
-// 16 * S + 1, 16 * S + 2 mma.sync with 16, 32 rows an item and clusters of S blocks.
-// Rows of queries that a request has for a key head, on average, decide between those that take a call.
-int chunk_form(int code, const Pools& p, int64_t R, int64_t W, double rows) {
-    if (code != 1 || (p.d != 64 && p.d != 128)) return 0;
-    if (rows > 32 && p.P % 8 == 0 && (128 % p.P == 0 || p.P % 128 == 0) && p.N * p.K * p.P / 8 < 0x7fffffff) return 3;
-    return rows <= 16 ? 1 : 2;
+// The forms of the attention: FLOAT32 (and bfloat16 that the others do not take); MMA, items of 32 rows by the line; TCGEN05, items of 256 rows by the
+// line; MMA + S, items of 32 rows, a cluster of S blocks for every request and key head.
+enum { FLOAT32 = 0, MMA = 16, TCGEN05 = 1 };
+
+// Which of them takes a call, by what the host knows: tokens, requests, and how many keys a request can have (the table's width; a
+// window).  The least of the times that each would take, in us, fitted to 643 calls (1 to 64 requests of 1 to 200 tokens behind 40 to 20,000, four head
+// layouts; the choice is 4 % above the best form of each call on average): a fixed part, and one for every key tile of the
+// busiest block.  Only these proportions count, so the machine's numbers are no promise.
+int chunk_form(int code, const Pools& p, int64_t R, int64_t W, int64_t T, int64_t G, int64_t window) {
+    if (code != 1 || (p.d != 64 && p.d != 128)) return FLOAT32;
+    auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    const int64_t items = R * p.K, rows = up(T * G, R), tile = p.d == 128 ? 64 : 128;
+    int64_t keys = W * p.P;
+    if (window > 0) keys = std::min(keys, window + up(T, R));
+    const int64_t tiles = up(keys, tile);
+    int form = MMA;
+    double least = 6.5 + 1.5 * up(items * up(rows, 32) * tiles, 2 * sm_count);
+    if (p.P % 8 == 0 && (128 % p.P == 0 || p.P % 128 == 0) && p.N * p.K * p.P / 8 < 0x7fffffff) {
+        // a tile of more than 128 rows takes both streams of a block for every key tile, one of fewer rows takes one of them
+        const int64_t rest = rows % 256, pairs = rows / 256 + (rest > 128), lone = rest > 0 && rest <= 128;
+        const double t = 12.5 + (p.d == 128 ? 1.6 : 1.0) * up(items * (pairs + lone) * up(keys, 128), sm_count) * (2 * pairs + lone) / (pairs + lone);
+        if (t < least) {
+            least = t;
+            form = TCGEN05;
+        }
+    }
+    // clusters: every block there at once, a row tile or little more each, and few key tiles, since nothing evens out unequal lengths
+    for (int S = 8; S >= 2 && rows <= 32; S /= 2) {
+        const int64_t each = up(tiles, S);
+        if (items * S > 2 * sm_count || each > 8) continue;
+        const double t = 5.0 + 0.9 * each;
+        if (t < least) {
+            least = t;
+            form = MMA + S;
+        }
+    }
+    return form;
 }
 
 PyObject* paged_attention_chunks(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -318,22 +348,20 @@ PyObject* paged_attention_chunks(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (T && R) {
             const int64_t G = H / p.K;
             if (!sm_count) sm_count = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-            if (form < 0) form = chunk_form(p.code, p, R, W, (double)T * G / R);
-            const int64_t wide = form ? p.d : p.d <= 64 ? 64 : p.d <= 128 ? 128 : 256;
-            const int clusters = (int)(form >> 4);
-            form &= 15;
-            const int64_t M = form == 3 ? 256 : form == 4 ? 64 : form == 1 || (form == 0 && wide == 256) ? 16 : 32;
-            const int64_t blocks = sm_count * (form == 1 || form == 2 ? 2 : 1), parts = 2 * blocks * M;
+            if (form < 0) form = chunk_form(p.code, p, R, W, T, G, window);
+            const int64_t wide = form == FLOAT32 ? (p.d <= 64 ? 64 : p.d <= 128 ? 128 : 256) : p.d;
+            const int64_t M = form == TCGEN05 ? 256 : form == FLOAT32 && wide == 256 ? 16 : 32;
+            const int64_t blocks = form > MMA ? 0 : sm_count * (form == MMA ? 2 : 1), parts = 2 * blocks * M;
             // parts [parts][wide], their maxima and sums [parts][2], what is to be joined [blocks][2] int4
             at::Tensor scratch;
-            if (!clusters) scratch = fresh({parts * (wide + 2) + 8 * blocks}, at::kFloat, q);
-            float* s = clusters ? nullptr : scratch.data_ptr<float>();
+            if (blocks) scratch = fresh({parts * (wide + 2) + 8 * blocks}, at::kFloat, q);
+            float* s = blocks ? scratch.data_ptr<float>() : nullptr;
             const ChCall call = {q.data_ptr(), kp.data_ptr(), vp.data_ptr(), out.data_ptr(), start.data_ptr(), len.data_ptr(), ctx.data_ptr(),
                                  table.data_ptr(), s, s + parts * wide, s + parts * (wide + 2), q.stride(0), q.stride(1), (int)R, (int)W, (int)T,
                                  (int)p.N, (int)p.P, (int)H, (int)p.K, (int)G, (int)p.d, (int)window, (float)(scale * 1.4426950408889634), err.data_ptr()};
-            launched(w, form == 3   ? loaded(chunks_tc_fn, "aie_attention_chunks_tc")(&call, st)
-                        : form == 0 ? loaded(chunks_f32_fn, "aie_attention_chunks_f32")(&call, p.code, st)
-                                    : loaded(chunks_mma_fn, "aie_attention_chunks_bf16")(&call, (int)M, clusters, st));
+            launched(w, form == TCGEN05   ? loaded(chunks_tc_fn, "aie_attention_chunks_tc")(&call, st)
+                        : form == FLOAT32 ? loaded(chunks_f32_fn, "aie_attention_chunks_f32")(&call, p.code, st)
+                                          : loaded(chunks_mma_fn, "aie_attention_chunks_bf16")(&call, (int)form - MMA, st));
         }
         return THPVariable_Wrap(std::move(out));
     });

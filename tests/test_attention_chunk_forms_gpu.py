@@ -10,12 +10,14 @@ pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
 
 
-@pytest.fixture(params=["tcgen05", "mma 16", "mma 32", "mma 64", "float32", "16 in clusters of 2", "32 in clusters of 8", "32 in clusters of 3"])
+FORMS = {"float32": 0, "tcgen05": 1, "mma": 16, "clusters of 2": 18, "clusters of 3": 19, "clusters of 8": 24}
+
+
+@pytest.fixture(params=list(FORMS))
 def form(request, monkeypatch):
     from ai_engine_b200.kernels import ops
 
-    monkeypatch.setattr(ops, "CHUNK_FORM", {"float32": 0, "mma 16": 1, "mma 32": 2, "tcgen05": 3, "mma 64": 4, "16 in clusters of 2": 33,
-                                            "32 in clusters of 8": 130, "32 in clusters of 3": 50}[request.param])
+    monkeypatch.setattr(ops, "CHUNK_FORM", FORMS[request.param])
     return request.param
 
 
