@@ -3,13 +3,13 @@
 //   o = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m),   x_j = (q . k_j) * scale * log2 e,   keys j <= position (and > position - window)
 //
 // A block has NG groups of four warps; of every key tile each group takes sixteen keys of its own through a ring of its own (cp.async), and
-// each warp of a group has every fourth four of the item's rows.  Groups meet only at an item's end.  Scores: a lane has two keys and
-// one row of each of the warp's fours, products and sums two at a time (fma.rn.f32x2) along the head; outputs: a lane has
-// D / 32 columns of all the warp's rows, two rows at a time.  The loop over key tiles exists for each number of fours.
-// What bounds it: the multiply-adds of 5 tokens x 4 heads take as long as their keys' bytes (0.27 G of them, 58 MB: 9 us each), and reading
-// shared memory nearly as long (of 16 keys x 8 rows x 128: 128 reads of K and Q beside 256 packed multiply-adds, then 96 wavefronts
-// of V and P beside 256).  What a step costs beside that is its chain of waits (copies, reads, a row's maximum among eight lanes,
-// probabilities through shared memory): two warps of 16 rows and eight keys each, with twice the steps, took twice the time.
+// each warp of a group has eight of the item's rows.  Groups meet only at an item's end.
+// Scores: a 16-byte read of shared memory takes four cycles of the SM whatever lanes share, so a lane multiplies 4 keys x 4 rows: the lanes
+// are 4 (keys) x 2 (rows) x 4 (parts of the head).  The parts' sums are then exchanged so that every lane ends with one key and four rows:
+// its i-th key is the (i ^ part)-th of its four, and what a lane gives away lies in the same registers in all lanes.  (Two keys x two
+// rows a lane: 512 cycles of reads a warp's step against 128 of multiply-adds, 47 us for the case below.)
+// Outputs: a lane has D / 32 columns of the warp's rows, two rows an instruction (fma.rn.f32x2).
+// What bounds it: these reads; the multiply-adds of 5 tokens x 4 heads behind 500 to 3,000 keys, 8 requests, take 9 us, as do their bytes.
 #include "attention_chunks.cuh"
 
 typedef unsigned long long u64;
@@ -40,18 +40,17 @@ __device__ __forceinline__ float2 cf_both(u64 v) {
     return f;
 }
 
-template <int N> struct CfInt { static constexpr int value = N; };
+#define CF_ROWS 32      // of an item: four warps' eight
 
 template <int D> struct CfShape {
-    static constexpr int FW = D > 128 ? 1 : 2;       // fours of rows of a warp
-    static constexpr int M = 16 * FW;                // rows of an item
+    static constexpr int M = CF_ROWS;
     static constexpr int NG = D > 128 ? 2 : 4;       // groups of four warps
     static constexpr int threads = NG * 128;
-    static constexpr int NST = D > 64 ? 3 : 4;       // stages of a group's ring: 16 keys and their values each
+    static constexpr int NST = D > 128 ? 2 : D > 64 ? 3 : 4;      // stages of a group's ring: 16 keys and their values each
     static constexpr int KT = NG * 16;               // keys of a tile
     static constexpr int KS = D + 4;                 // distance of two rows of keys or queries: eight of them lie in different banks
     static constexpr int stage = 16 * KS + 16 * D;   // floats
-    static constexpr int PS = 4 * FW + 4;            // distance of two keys' probabilities
+    static constexpr int PS = 12;                    // distance of two keys' probabilities
     static constexpr int q_off = NG * NST * stage, p_off = q_off + M * KS, ml_off = p_off + NG * 4 * 16 * PS, end = ml_off + NG * M * 2;
     static constexpr int bytes = end * 4;
     static_assert(NG * M * D <= NG * NST * stage && bytes <= 227 * 1024 - 256, "the groups' outputs meet in the ring's memory");
@@ -69,25 +68,26 @@ __device__ __forceinline__ void cf_fetch(float* dst, const bf16* src, bool there
 template <typename T, int D>
 __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const ChArgs a) {
     using S = CfShape<D>;
-    constexpr int M = S::M, FW = S::FW, NG = S::NG, NST = S::NST, KT = S::KT, CH = D / 4, CL = D / 32, THREADS = S::threads;      // CL: columns of a lane
+    constexpr int M = S::M, NG = S::NG, NST = S::NST, KT = S::KT, CH = D / 4, CL = D / 32, THREADS = S::threads;      // CL: columns of a lane
     extern __shared__ __align__(16) float cf_smem[];
     __shared__ ChShared sh;
     __shared__ ChWalk place_in_line;              // while the registers hold rows' outputs
     pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int group = warp % NG, mt = warp / NG, gt = mt * 32 + lane;      // mt: which fours of rows
+    const int group = warp % NG, mt = warp / NG, gt = mt * 32 + lane;      // mt: which eight rows
     const int c = blockIdx.x, C = gridDim.x;
     if (tid == 0) a.meta[2 * c] = make_int4(0, 0, 0, 0);
     ChWalk w;
     if (!ch_begin<THREADS, M, KT>(a, c, C, &sh, w)) return;
     float* ring = cf_smem + group * NST * S::stage;
     float* q_s = cf_smem + S::q_off;              // [M][KS]
-    float* p_s = cf_smem + S::p_off + warp * 16 * S::PS;      // this warp's [16 keys][4 FW]
+    float* p_s = cf_smem + S::p_off + warp * 16 * S::PS;      // this warp's [16 keys][8]
     float* ml = cf_smem + S::ml_off;              // [NG][M][2]
     const T* kp = reinterpret_cast<const T*>(a.k_pages);
     const T* vp = reinterpret_cast<const T*>(a.v_pages);
-    const int key = lane & 7, rg = lane >> 3;     // for the scores: this lane's keys are `key` and `key` + 8, of every four rows it has row rg
+    const int kq = lane & 3, rq = (lane >> 2) & 1, ds = lane >> 3;      // for the scores: keys kq + 4 i, rows 4 rq + r of the warp, part of the head
+    const int key = kq + 4 * ds;                  // the one that this lane has in the end
     unsigned bad = 0;
 
     for (;;) {
@@ -139,147 +139,152 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
         asm volatile("cp.async.wait_group %0;\n" ::"n"(NST - 2));
         __syncthreads();
 
-        float m_run[FW], l_run[FW];
-        int lim[FW];                              // last key that a row sees, -1 for a row that is not there
-        u64 o[FW][2][CL];                         // rows 4 (mt + 4 j) + 2 e and the next, columns CL lane .. (128 further from the fifth on)
+        const bool live = mt * 8 < rows;          // any row of this warp
+        float m_run[4], l_run[4];                 // of rows 8 mt + 4 rq + r
+        int lim[4];                               // last key that a row sees, -1 for a row that is not there
+        u64 o[2][2][CL];                          // rows 8 mt + 4 j + 2 e and the next, columns CL lane .. (128 further from the fifth on)
         const int reach = a.window > 0 ? a.window : 0x7fffffff;
 #pragma unroll
-        for (int j = 0; j < FW; ++j) {
-            m_run[j] = -INFINITY;
-            l_run[j] = 0.f;
-            const int row = (mt + 4 * j) * 4 + rg;
-            lim[j] = row < rows ? c0 + ch_over(row0 + row, a.by_g) : -1;
+        for (int r = 0; r < 4; ++r) {
+            m_run[r] = -INFINITY;
+            l_run[r] = 0.f;
+            const int row = mt * 8 + rq * 4 + r;
+            lim[r] = row < rows ? c0 + ch_over(row0 + row, a.by_g) : -1;
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int x = 0; x < CL; ++x) o[j][0][x] = o[j][1][x] = 0ull;
-        }
 
-        auto walk = [&](auto fours) {
-            constexpr int JN = decltype(fours)::value;
-            int slot = 0;
-            for (int i = 0; i < n; ++i) {
-                asm volatile("cp.async.wait_group %0;\n" ::"n"(NST - 2));
-                // the stage is there for the whole group, and the group has read the one that the next copies go to
-                asm volatile("bar.sync %0, 128;\n" ::"r"(1 + group) : "memory");
-                issue(i + NST - 1, slot == 0 ? NST - 1 : slot - 1);
-                const float* ks = ring + slot * S::stage;
-                const float* vs = ks + 16 * S::KS;
-                slot = slot + 1 == NST ? 0 : slot + 1;
-                if constexpr (JN > 0) {
-                    const int k_at = (kt0 + i) * KT + group * 16 + key;
-                    if (k_at - key >= hi) continue;
-                    u64 s2[JN][2];
+        int slot = 0;
+        for (int i = 0; i < n; ++i) {
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(NST - 2));
+            // the stage is there for the whole group, and the group has read the one that the next copies go to
+            asm volatile("bar.sync %0, 128;\n" ::"r"(1 + group) : "memory");
+            issue(i + NST - 1, slot == 0 ? NST - 1 : slot - 1);
+            const float* ks = ring + slot * S::stage;
+            const float* vs = ks + 16 * S::KS;
+            slot = slot + 1 == NST ? 0 : slot + 1;
+            const int k_at = (kt0 + i) * KT + group * 16;
+            if (k_at >= hi || !live) continue;
+            float x[4];
+            {
+                u64 s2[4][4];
 #pragma unroll
-                    for (int j = 0; j < JN; ++j) s2[j][0] = s2[j][1] = 0ull;
-                    const float *k0 = ks + key * S::KS, *q0 = q_s + (mt * 4 + rg) * S::KS;
-#pragma unroll 8
-                    for (int ch = 0; ch < CH; ++ch) {
-                        const ulonglong2 ka = *reinterpret_cast<const ulonglong2*>(k0 + ch * 4), kb = *reinterpret_cast<const ulonglong2*>(k0 + 8 * S::KS + ch * 4);
+                for (int y = 0; y < 4; ++y)
 #pragma unroll
-                        for (int j = 0; j < JN; ++j) {
-                            const ulonglong2 q2 = *reinterpret_cast<const ulonglong2*>(q0 + j * 16 * S::KS + ch * 4);
-                            s2[j][0] = cf_fma2(ka.x, q2.x, s2[j][0]);
-                            s2[j][1] = cf_fma2(kb.x, q2.x, s2[j][1]);
-                            s2[j][0] = cf_fma2(ka.y, q2.y, s2[j][0]);
-                            s2[j][1] = cf_fma2(kb.y, q2.y, s2[j][1]);
+                    for (int r = 0; r < 4; ++r) s2[y][r] = 0ull;
+                const float *k0 = ks + (kq + 4 * ds) * S::KS + ds * 4, *k1 = ks + (kq + 4 * (ds ^ 1)) * S::KS + ds * 4;
+                const float *k2 = ks + (kq + 4 * (ds ^ 2)) * S::KS + ds * 4, *k3 = ks + (kq + 4 * (ds ^ 3)) * S::KS + ds * 4;
+                const float* q0 = q_s + (mt * 8 + rq * 4) * S::KS + ds * 4;
+#pragma unroll 2
+                for (int ch = 0; ch < CH / 4; ++ch) {
+                    const ulonglong2 kv[4] = {*reinterpret_cast<const ulonglong2*>(k0 + ch * 16), *reinterpret_cast<const ulonglong2*>(k1 + ch * 16),
+                                              *reinterpret_cast<const ulonglong2*>(k2 + ch * 16), *reinterpret_cast<const ulonglong2*>(k3 + ch * 16)};
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const ulonglong2 q2 = *reinterpret_cast<const ulonglong2*>(q0 + r * S::KS + ch * 16);
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            s2[y][r] = cf_fma2(kv[y].x, q2.x, s2[y][r]);
+                            s2[y][r] = cf_fma2(kv[y].y, q2.y, s2[y][r]);
                         }
                     }
-                    float x[JN][2], top[JN], corr[JN];
+                }
+                float f[4][4];
 #pragma unroll
-                    for (int j = 0; j < JN; ++j) {
+                for (int y = 0; y < 4; ++y)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float2 f = cf_both(s2[j][e]);
-                            const int at = k_at + 8 * e;
-                            x[j][e] = at <= lim[j] && lim[j] - at < reach ? (f.x + f.y) * a.scale2 : -INFINITY;
-                        }
-                        top[j] = fmaxf(x[j][0], x[j][1]);
+                    for (int r = 0; r < 4; ++r) {
+                        const float2 t = cf_both(s2[y][r]);
+                        f[y][r] = t.x + t.y;
                     }
 #pragma unroll
-                    for (int b = 1; b < 8; b <<= 1)
+                for (int r = 0; r < 4; ++r) {
+                    f[0][r] += __shfl_xor_sync(0xffffffffu, f[2][r], 16);
+                    f[1][r] += __shfl_xor_sync(0xffffffffu, f[3][r], 16);
+                }
 #pragma unroll
-                        for (int j = 0; j < JN; ++j) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], b));
-                    bool moved = false;
+                for (int r = 0; r < 4; ++r) x[r] = f[0][r] + __shfl_xor_sync(0xffffffffu, f[1][r], 8);
+            }
+            const int at = k_at + key;
+            float top[4], corr[4];
 #pragma unroll
-                    for (int j = 0; j < JN; ++j) {
-                        // the reference moves by more than 8 or not at all: weights stay below 2^8, outputs are rarely rescaled
-                        corr[j] = 1.f;
-                        if (top[j] > m_run[j] + 8.f) {
-                            corr[j] = m_run[j] == -INFINITY ? 0.f : cf_exp2(m_run[j] - top[j]);
-                            m_run[j] = top[j];
-                            moved = true;
-                        }
-                        l_run[j] *= corr[j];
+            for (int r = 0; r < 4; ++r) top[r] = x[r] = at <= lim[r] && lim[r] - at < reach ? x[r] * a.scale2 : -INFINITY;
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float p = x[j][e] == -INFINITY ? 0.f : cf_exp2(x[j][e] - m_run[j]);
-                            l_run[j] += p;                          // of this lane's keys
-                            p_s[(key + 8 * e) * S::PS + j * 4 + rg] = p;
-                        }
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], b < 2 ? 1 << b : 2 << b));
+            bool moved = false;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                // the reference moves by more than 8 or not at all: weights stay below 2^8, outputs are rarely rescaled
+                corr[r] = 1.f;
+                if (top[r] > m_run[r] + 8.f) {
+                    corr[r] = m_run[r] == -INFINITY ? 0.f : cf_exp2(m_run[r] - top[r]);
+                    m_run[r] = top[r];
+                    moved = true;
+                }
+                x[r] = x[r] == -INFINITY ? 0.f : cf_exp2(x[r] - m_run[r]);
+                l_run[r] = l_run[r] * corr[r] + x[r];          // of this lane's keys
+            }
+            *reinterpret_cast<float4*>(p_s + key * S::PS + rq * 4) = make_float4(x[0], x[1], x[2], x[3]);
+            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float f0 = __shfl_sync(0xffffffffu, corr[2 * e], 4 * j), f1 = __shfl_sync(0xffffffffu, corr[2 * e + 1], 4 * j);
+                        const u64 ff = cf_pack(f0, f1);
+#pragma unroll
+                        for (int y = 0; y < CL; ++y) o[j][e][y] = cf_mul2(o[j][e][y], ff);
                     }
-                    if (__any_sync(0xffffffffu, moved)) {
+            }
+            __syncwarp();
+#pragma unroll 4
+            for (int kk = 0; kk < 16; ++kk) {
+                float v[CL];
+                if constexpr (CL == 2) {
+                    const float2 t = *reinterpret_cast<const float2*>(vs + kk * D + lane * 2);
+                    v[0] = t.x, v[1] = t.y;
+                } else {
 #pragma unroll
-                        for (int j = 0; j < JN; ++j)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const float f0 = __shfl_sync(0xffffffffu, corr[j], 16 * e), f1 = __shfl_sync(0xffffffffu, corr[j], 16 * e + 8);
-                                const u64 ff = cf_pack(f0, f1);
-#pragma unroll
-                                for (int y = 0; y < CL; ++y) o[j][e][y] = cf_mul2(o[j][e][y], ff);
-                            }
+                    for (int y = 0; y < CL / 4; ++y) {
+                        const float4 t = *reinterpret_cast<const float4*>(vs + kk * D + (lane + 32 * y) * 4);
+                        v[4 * y] = t.x, v[4 * y + 1] = t.y, v[4 * y + 2] = t.z, v[4 * y + 3] = t.w;
                     }
-                    __syncwarp();
-#pragma unroll 8
-                    for (int kk = 0; kk < 16; ++kk) {
-                        float v[CL];
-                        if constexpr (CL == 2) {
-                            const float2 t = *reinterpret_cast<const float2*>(vs + kk * D + lane * 2);
-                            v[0] = t.x, v[1] = t.y;
-                        } else {
+                }
 #pragma unroll
-                            for (int y = 0; y < CL / 4; ++y) {
-                                const float4 t = *reinterpret_cast<const float4*>(vs + kk * D + (lane + 32 * y) * 4);
-                                v[4 * y] = t.x, v[4 * y + 1] = t.y, v[4 * y + 2] = t.z, v[4 * y + 3] = t.w;
-                            }
-                        }
-                        u64 vv[CL];
+                for (int j = 0; j < 2; ++j) {
+                    const ulonglong2 p2 = *reinterpret_cast<const ulonglong2*>(p_s + kk * S::PS + j * 4);
 #pragma unroll
-                        for (int y = 0; y < CL; ++y) vv[y] = cf_pack(v[y], v[y]);
-#pragma unroll
-                        for (int j = 0; j < JN; ++j) {
-                            const ulonglong2 p2 = *reinterpret_cast<const ulonglong2*>(p_s + kk * S::PS + j * 4);
-#pragma unroll
-                            for (int y = 0; y < CL; ++y) {
-                                o[j][0][y] = cf_fma2(p2.x, vv[y], o[j][0][y]);
-                                o[j][1][y] = cf_fma2(p2.y, vv[y], o[j][1][y]);
-                            }
-                        }
+                    for (int y = 0; y < CL; ++y) {
+                        const u64 vv = cf_pack(v[y], v[y]);
+                        o[j][0][y] = cf_fma2(p2.x, vv, o[j][0][y]);
+                        o[j][1][y] = cf_fma2(p2.y, vv, o[j][1][y]);
                     }
-                    __syncwarp();
                 }
             }
-        };
-        const int fours = (((rows + 3) >> 2) + 3 - mt) >> 2;      // of this warp: every fourth four of the item's
-        if (fours <= 0) walk(CfInt<0>());
-        else if (fours == 1) walk(CfInt<1>());
-        else walk(CfInt<FW>());
+            __syncwarp();
+        }
         asm volatile("cp.async.wait_group 0;\n" ::);
 
         // the groups meet: every row's maximum, then outputs and sums
 #pragma unroll
-        for (int j = 0; j < FW; ++j) {
-            float l = l_run[j];
+        for (int r = 0; r < 4; ++r) {
+            float l = l_run[r];
 #pragma unroll
-            for (int b = 1; b < 8; b <<= 1) l += __shfl_xor_sync(0xffffffffu, l, b);
-            if (key == 0) *reinterpret_cast<float2*>(ml + (group * M + (mt + 4 * j) * 4 + rg) * 2) = make_float2(m_run[j], l);
+            for (int b = 0; b < 4; ++b) l += __shfl_xor_sync(0xffffffffu, l, b < 2 ? 1 << b : 2 << b);
+            if (key == 0) *reinterpret_cast<float2*>(ml + (group * M + mt * 8 + rq * 4 + r) * 2) = make_float2(m_run[r], l);
         }
         __syncthreads();
         w = place_in_line;
         float* o_s = cf_smem;                     // [NG][M][D]
 #pragma unroll
-        for (int j = 0; j < FW; ++j)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int row = (mt + 4 * j) * 4 + e;
+                const int row = mt * 8 + j * 4 + e;
                 if (row >= w.tile.rows) continue;
                 float f[CL];
 #pragma unroll
@@ -295,7 +300,7 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
             }
         __syncthreads();
         const bool begins = w.k == 0, ends = w.k + n == w.tile.tiles;
-        const size_t slot = (size_t)2 * c + (begins ? 1 : 0);
+        const size_t place = (size_t)2 * c + (begins ? 1 : 0);
         for (int i = tid; i < w.tile.rows * CH; i += THREADS) {
             const int row = i / CH, e = (i - row * CH) * 4;
             float m = -INFINITY, l = 0.f;
@@ -320,8 +325,8 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
                     store4<T>(reinterpret_cast<T*>(a.out) + ((size_t)(w.s0 + t) * a.H + h) * a.d + e,
                               make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
             } else {
-                *reinterpret_cast<float4*>(a.part_o + (slot * M + row) * D + e) = y;
-                if (e == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * M + row) * 2) = make_float2(m, l);
+                *reinterpret_cast<float4*>(a.part_o + (place * M + row) * D + e) = y;
+                if (e == 0) *reinterpret_cast<float2*>(a.part_ml + (place * M + row) * 2) = make_float2(m, l);
             }
         }
         if (begins && !ends && tid == 0) ch_leave(a, w, c, n);
@@ -342,13 +347,13 @@ template <typename T, int D> static int launch_chunk_f32(const ChArgs& a, cudaSt
     return launch_chunk_join<T, S::M, D>(a, C, st);
 }
 
-// Items have 32 rows, 16 at heads above 128; a block an SM.  The scratch is [2 * blocks * rows * (D + 2)] floats and [2 * blocks] int4, D
+// A block an SM.  The scratch is [2 * blocks * 32 * (D + 2)] floats and [2 * blocks] int4, D
 // the head size rounded up to 64, 128 or 256.
 extern "C" int aie_attention_chunks_f32(const ChCall* call, int dtype, cudaStream_t stream) {
     if (call->R <= 0 || call->T <= 0) return 0;
     if (call->d <= 0 || call->d > 256 || call->d % 8) return AIE_UNSUPPORTED;
     ChArgs a;
-    const int rc = ch_args(call, 16, 32, &a);
+    const int rc = ch_args(call, 32, 32, &a);
     if (rc) return rc;
     const int w = a.d <= 64 ? 0 : a.d <= 128 ? 1 : 2;
     if (dtype == AIE_F32) return w == 0 ? launch_chunk_f32<float, 64>(a, stream) : w == 1 ? launch_chunk_f32<float, 128>(a, stream) : launch_chunk_f32<float, 256>(a, stream);

@@ -350,7 +350,7 @@ PyObject* paged_attention_chunks(PyObject*, PyObject* const* a, Py_ssize_t n) {
             if (!sm_count) sm_count = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
             if (form < 0) form = chunk_form(p.code, p, R, W, T, G, window);
             const int64_t wide = form == FLOAT32 ? (p.d <= 64 ? 64 : p.d <= 128 ? 128 : 256) : p.d;
-            const int64_t M = form == TCGEN05 ? 256 : form == FLOAT32 && wide == 256 ? 16 : 32;
+            const int64_t M = form == TCGEN05 ? 256 : 32;
             const int64_t blocks = form > MMA ? 0 : sm_count * (form == MMA ? 2 : 1), parts = 2 * blocks * M;
             // parts [parts][wide], their maxima and sums [parts][2], what is to be joined [blocks][2] int4
             at::Tensor scratch;
