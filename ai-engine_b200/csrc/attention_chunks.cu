@@ -31,6 +31,8 @@ template <int D> struct CbShape {
     static constexpr int threads = CB_GROUPS * GW * 32;
     static constexpr int CK = D == 64 ? 32 : 16;      // keys of a group's stage
     static constexpr int KT = CB_GROUPS * CK;         // keys of a tile
+    static constexpr int MAX_WEIGHT = 1;
+    static __device__ __forceinline__ int weight(int) { return 1; }
     static constexpr int NST = 3;
     static constexpr int stage = 2 * CK * D;          // elements: keys, then values
     static constexpr int TPK = 32 * GW / CK;          // threads that copy a key
@@ -68,9 +70,9 @@ __device__ __forceinline__ float cb_exp2(float x) {
 template <int D> __device__ __forceinline__ unsigned cb_at(int row, int piece) { return (unsigned)(row * (D * 2) + ((piece ^ (row & 7)) << 4)); }
 
 // The walk of a block in a cluster: its part of the tiles of row tile `m` (maybe none).
-template <int M, int KT> __device__ __forceinline__ void cb_part(const ChArgs& a, ChWalk& w, int m, int rank, int S) {
+template <typename Sh> __device__ __forceinline__ void cb_part(const ChArgs& a, ChWalk& w, int m, int rank, int S) {
     w.m = m;
-    w.tile = ch_tile<M, KT>(a, w.req, m);
+    w.tile = ch_tile<Sh>(a, w.req, m);
     w.per = (w.tile.tiles + S - 1) / S;
     w.k = rank * w.per;
     w.left = max(0, min(w.per, w.tile.tiles - w.k));
@@ -97,10 +99,10 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
         w.s0 = a.q_start[w.r];
         if (bad_lengths && tid == 0 && rank == 0 && w.kh == 0) atomicOr(a.err, bad_lengths);
         if (w.req.n == 0) return;                 // the whole cluster
-        cb_part<M, KT>(a, w, 0, rank, S_blocks);
+        cb_part<S>(a, w, 0, rank, S_blocks);
     } else {
         if (tid == 0) a.meta[2 * c] = make_int4(0, 0, 0, 0);
-        if (!ch_begin<THREADS, M, KT>(a, c, C, &sh, w)) return;
+        if (!ch_begin<THREADS, S>(a, c, C, &sh, w)) return;
     }
     const unsigned smem = (unsigned)__cvta_generic_to_shared(cb_smem);
     const unsigned ring = smem + group * NST * S::stage * 2, q_s = smem + S::q_off;
@@ -114,7 +116,7 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
     unsigned bad = 0;
 
     for (;;) {
-        const int n = CLUSTER ? w.left : ch_share(w);
+        const int n = CLUSTER ? w.left : ch_share<S>(w);
         const ChTile tl = w.tile;
         const int c0 = w.req.c, s0 = w.s0, hi = c0 + tl.i1 + 1;
         const int* bt = a.table + (size_t)w.r * a.W;
@@ -351,10 +353,10 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
             }
             cluster.sync();                   // the others have read this block's memory
             if ((w.m + 1) * M >= w.req.n * a.G) break;
-            cb_part<M, KT>(a, w, w.m + 1, rank, S_blocks);
+            cb_part<S>(a, w, w.m + 1, rank, S_blocks);
         } else {
-            if (begins && !ends && tid == 0) ch_leave(a, w, c, n);
-            if (!ch_next<M, KT>(a, w, n)) break;
+            if (begins && !ends && tid == 0) ch_leave<S>(a, w, c);
+            if (!ch_next<S>(a, w, n)) break;
             __syncthreads();                  // the ring's memory is the next item's
         }
     }
@@ -398,7 +400,7 @@ template <int D> static int launch_chunk_clusters(const ChArgs& a, int blocks, c
 extern "C" int aie_attention_chunks_bf16(const ChCall* call, int clusters, cudaStream_t stream) {
     if (call->R <= 0 || call->T <= 0) return 0;
     ChArgs a;
-    const int rc = ch_args(call, 32, 64, &a);
+    const int rc = ch_args(call, 32, 64, 1, &a);
     if (rc) return rc;
     if (a.d != 64 && a.d != 128) return AIE_UNSUPPORTED;
     if (!clusters) return a.d == 64 ? launch_chunk_bf16<64>(a, stream) : launch_chunk_bf16<128>(a, stream);

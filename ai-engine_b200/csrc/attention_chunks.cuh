@@ -5,9 +5,9 @@
 // are rows: row = i * G + g.  An item is (request, key head, tile of M rows); it walks key tiles of KT keys, from the one that holds the
 // first key any of its rows sees to the one of its last row's own key.
 //
-// All items' key tiles stand in one line, in the order of requests, key heads and row tiles; block c of C takes those from c * per to
-// (c + 1) * per - 1, per = ceil(all / C), so every block has the same number of tiles whatever the requests' lengths.  Every
-// block works out the line from the lengths by itself (sums over the requests), so nothing comes from the host and a
+// All items' key tiles stand in one line, in the order of requests, key heads and row tiles, each as long as it takes (a weight by the
+// item's rows); block c of C takes those that begin in [c * per, (c + 1) * per), per = ceil(all / C), so every block has the same work
+// whatever the requests' lengths.  Every block works out the line from the lengths by itself (sums over the requests), so nothing comes from the host and a
 // captured call follows the lengths.  An item that a block does not finish is left as a part: sums of exp2(x - m) v without
 // division, m and l, in a place of the block's own (one for an item that it began, one for an item that it continued), and a second,
 // small kernel joins the parts of every item in their order.  The split depends on all requests' lengths: the sums of a token
@@ -45,13 +45,13 @@ struct ChArgs : ChCall {
     ChDiv by_g, by_p;
 };
 
-// Checks a call and completes it; `tiles`: rows of an item and keys of a tile of the kernel that takes it.
-static inline int ch_args(const ChCall* call, int M, int KT, ChArgs* a) {
+// Checks a call and completes it; M, KT, weight: rows of an item, keys of a tile and its largest weight in the kernel that takes it.
+static inline int ch_args(const ChCall* call, int M, int KT, int weight, ChArgs* a) {
     *static_cast<ChCall*>(a) = *call;
     if (a->W <= 0 || a->num_pages <= 0 || a->P <= 0 || a->K <= 0 || a->H <= 0 || a->H % a->K || a->G != a->H / a->K) return AIE_BAD_ARG;
     // the line's length has to fit 31 bits: every request at least one row tile a key head, each over all the table's keys
     const double items = (double)a->T * a->H / M + (double)a->R * a->K, keys = (double)a->W * a->P / KT + 2;
-    if (items * keys > 2147000000.0) return -3;
+    if (items * keys * weight > 2147000000.0) return -3;
     a->by_g = ch_div((unsigned)a->G);
     a->by_p = ch_div((unsigned)a->P);
     return 0;
@@ -66,27 +66,31 @@ __device__ __forceinline__ ChReq ch_req(const ChArgs& a, int r, unsigned* bad = 
     return {fits ? n : 0, c};
 }
 
+// A kernel's shape Sh: M rows of an item, KT keys of a tile, weight(rows) of a key tile (at most MAX_WEIGHT).
 struct ChTile { int row0, rows, i0, i1, first, tiles; };      // rows of the tile, its first and last token, first key tile, key tiles
-template <int M, int KT> __device__ __forceinline__ ChTile ch_tile(const ChArgs& a, const ChReq& q, int m) {
+template <typename Sh> __device__ __forceinline__ ChTile ch_tile(const ChArgs& a, const ChReq& q, int m) {
     ChTile t;
-    t.row0 = m * M;
-    t.rows = min(M, q.n * a.G - t.row0);
+    t.row0 = m * Sh::M;
+    t.rows = min(Sh::M, q.n * a.G - t.row0);
     t.i0 = ch_over(t.row0, a.by_g);
     t.i1 = ch_over(t.row0 + t.rows - 1, a.by_g);
     const int lo = a.window > 0 ? max(0, q.c + t.i0 - a.window + 1) : 0;
-    t.first = lo / KT;
-    t.tiles = (q.c + t.i1) / KT - t.first + 1;
+    t.first = lo / Sh::KT;
+    t.tiles = (q.c + t.i1) / Sh::KT - t.first + 1;
     return t;
 }
-template <int M, int KT> __device__ __forceinline__ int ch_tiles(const ChArgs& a, const ChReq& q) {      // of one key head
+template <typename Sh> __device__ __forceinline__ int ch_length(const ChArgs& a, const ChReq& q) {      // of the line of one key head
     int s = 0;
-    for (int m = 0; m * M < q.n * a.G; ++m) s += ch_tile<M, KT>(a, q, m).tiles;
+    for (int m = 0; m * Sh::M < q.n * a.G; ++m) {
+        const ChTile t = ch_tile<Sh>(a, q, m);
+        s += t.tiles * Sh::weight(t.rows);
+    }
     return s;
 }
 
 // Where a block is in the line.
 struct ChWalk {
-    int left, per;           // key tiles that are left of this block's share, tiles of a share
+    int left, per;           // of the line, from the beginning of tile k to the end of this block's share; length of a share
     int r, kh, m, k, s0;     // item, key tile within it, the request's first token
     ChReq req;
     ChTile tile;
@@ -118,8 +122,26 @@ template <int THREADS> __device__ __forceinline__ int ch_scan(int v, ChShared* s
     return before + x - v;
 }
 
+// ... on to the next item; false: there is none
+template <typename Sh> __device__ __forceinline__ bool ch_item(const ChArgs& a, ChWalk& w) {
+    w.k = 0;
+    ++w.m;
+    if (w.m * Sh::M >= w.req.n * a.G) {
+        w.m = 0;
+        if (++w.kh == a.K) {
+            w.kh = 0;
+            do {
+                if (++w.r >= a.R) return false;
+                w.req = ch_req(a, w.r);
+            } while (w.req.n == 0);
+            w.s0 = a.q_start[w.r];
+        }
+    }
+    w.tile = ch_tile<Sh>(a, w.req, w.m);
+    return true;
+}
 // This block's share of the line; false: none.  All threads of the block call it.
-template <int THREADS, int M, int KT>
+template <int THREADS, typename Sh>
 __device__ __forceinline__ bool ch_begin(const ChArgs& a, int c, int C, ChShared* s, ChWalk& w) {
     const int tid = threadIdx.x;
     int all = 0, mine = 0, before = 0;
@@ -130,18 +152,18 @@ __device__ __forceinline__ bool ch_begin(const ChArgs& a, int c, int C, ChShared
         mine = 0;
         if (r < a.R) {
             q = ch_req(a, r, &bad);
-            mine = a.K * ch_tiles<M, KT>(a, q);
+            mine = a.K * ch_length<Sh>(a, q);
             if (bad && c == 0) atomicOr(a.err, bad);
         }
         int sum;
         before = all + ch_scan<THREADS>(mine, s, &sum);
         all += sum;
     }
-    w.per = (int)(((unsigned)all + C - 1) / (unsigned)C);
+    // at least the weight of a tile: a tile then begins in every share that lies within one item
+    w.per = max((int)(((unsigned)all + C - 1) / (unsigned)C), Sh::MAX_WEIGHT);
     const long long first = (long long)c * w.per;
     if (first >= all) return false;
     const int at = (int)first;
-    w.left = min(w.per, all - at);
     auto leave = [&](int r, const ChReq& x, int off) {
         s->r = r;
         s->off = off;
@@ -156,7 +178,7 @@ __device__ __forceinline__ bool ch_begin(const ChArgs& a, int c, int C, ChShared
         for (int base = 0; base < a.R; base += THREADS) {
             const int r = base + tid;
             q = r < a.R ? ch_req(a, r) : ChReq{0, 0};
-            const int here = r < a.R ? a.K * ch_tiles<M, KT>(a, q) : 0;
+            const int here = r < a.R ? a.K * ch_length<Sh>(a, q) : 0;
             int sum;
             const int b = upto + ch_scan<THREADS>(here, s, &sum);
             if (at >= b && at < b + here) leave(r, q, at - b);
@@ -167,38 +189,33 @@ __device__ __forceinline__ bool ch_begin(const ChArgs& a, int c, int C, ChShared
     w.r = s->r;
     w.s0 = s->s0;
     w.req = {s->n, s->c};
-    const unsigned one = (unsigned)ch_tiles<M, KT>(a, w.req), off = (unsigned)s->off;
+    const unsigned one = (unsigned)ch_length<Sh>(a, w.req), off = (unsigned)s->off;
     w.kh = (int)(off / one);
-    w.k = (int)(off - w.kh * one);
+    int rest = (int)(off - w.kh * one), weight;
     for (w.m = 0;; ++w.m) {
-        w.tile = ch_tile<M, KT>(a, w.req, w.m);
-        if (w.k < w.tile.tiles) break;
-        w.k -= w.tile.tiles;
+        w.tile = ch_tile<Sh>(a, w.req, w.m);
+        weight = Sh::weight(w.tile.rows);
+        if (rest < w.tile.tiles * weight) break;
+        rest -= w.tile.tiles * weight;
     }
-    return true;
+    w.k = (rest + weight - 1) / weight;                  // the first tile that begins in the share
+    w.left = w.per - (w.k * weight - rest);
+    if (w.k == w.tile.tiles) return w.left > 0 && ch_item<Sh>(a, w);
+    return w.left > 0;
 }
-__device__ __forceinline__ int ch_share(const ChWalk& w) { return min(w.tile.tiles - w.k, w.left); }      // key tiles of the item that are this block's
+template <typename Sh> __device__ __forceinline__ int ch_share(const ChWalk& w) {      // key tiles of the item that are this block's
+    const int weight = Sh::weight(w.tile.rows);
+    return min(w.tile.tiles - w.k, (w.left + weight - 1) / weight);
+}
 // ... the next item behind the `n` tiles of this one; false: the share is done
-template <int M, int KT> __device__ __forceinline__ bool ch_next(const ChArgs& a, ChWalk& w, int n) {
-    w.left -= n;
-    if (w.left <= 0) return false;
-    w.k = 0;
-    ++w.m;
-    if (w.m * M >= w.req.n * a.G) {
-        w.m = 0;
-        if (++w.kh == a.K) {
-            w.kh = 0;
-            do { w.req = ch_req(a, ++w.r); } while (w.req.n == 0);
-            w.s0 = a.q_start[w.r];
-        }
-    }
-    w.tile = ch_tile<M, KT>(a, w.req, w.m);
-    return true;
+template <typename Sh> __device__ __forceinline__ bool ch_next(const ChArgs& a, ChWalk& w, int n) {
+    w.left -= n * Sh::weight(w.tile.rows);
+    return w.left > 0 && ch_item<Sh>(a, w);
 }
-// What the joining kernel has to know of the item that block c begins here and does not finish with its `n` tiles.
-__device__ __forceinline__ void ch_leave(const ChArgs& a, const ChWalk& w, int c, int n) {
-    const int rest = w.tile.tiles - w.k - n;
-    a.meta[2 * c] = make_int4(w.kh, w.tile.row0, w.tile.rows, 1 + (rest + w.per - 1) / w.per);
+// What the joining kernel has to know of the item that block c begins here and does not finish.
+template <typename Sh> __device__ __forceinline__ void ch_leave(const ChArgs& a, const ChWalk& w, int c) {
+    const int last = (w.tile.tiles - 1) * Sh::weight(w.tile.rows);      // where its last tile begins, from the item's beginning
+    a.meta[2 * c] = make_int4(w.kh, w.tile.row0, w.tile.rows, last < w.left ? 1 : 2 + (last - w.left) / w.per);
     a.meta[2 * c + 1] = make_int4(w.s0, 0, 0, 0);
 }
 __device__ __forceinline__ float ch_inverse(float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); }      // of a row's sum; a row that sees nothing is zero

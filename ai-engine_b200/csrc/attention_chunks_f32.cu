@@ -48,6 +48,9 @@ template <int D> struct CfShape {
     static constexpr int threads = NG * 128;
     static constexpr int NST = D > 128 ? 2 : D > 64 ? 3 : 4;      // stages of a group's ring: 16 keys and their values each
     static constexpr int KT = NG * 16;               // keys of a tile
+    // a tile takes as long as its warps with rows, and a part that does not depend on them
+    static constexpr int MAX_WEIGHT = 8;
+    static __device__ __forceinline__ int weight(int rows) { return 4 + (rows + 7) / 8; }
     static constexpr int KS = D + 4;                 // distance of two rows of keys or queries: eight of them lie in different banks
     static constexpr int stage = 16 * KS + 16 * D;   // floats
     static constexpr int PS = 12;                    // distance of two keys' probabilities
@@ -79,7 +82,7 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
     const int c = blockIdx.x, C = gridDim.x;
     if (tid == 0) a.meta[2 * c] = make_int4(0, 0, 0, 0);
     ChWalk w;
-    if (!ch_begin<THREADS, M, KT>(a, c, C, &sh, w)) return;
+    if (!ch_begin<THREADS, S>(a, c, C, &sh, w)) return;
     float* ring = cf_smem + group * NST * S::stage;
     float* q_s = cf_smem + S::q_off;              // [M][KS]
     float* p_s = cf_smem + S::p_off + warp * 16 * S::PS;      // this warp's [16 keys][8]
@@ -91,7 +94,7 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
     unsigned bad = 0;
 
     for (;;) {
-        const int n = ch_share(w);
+        const int n = ch_share<S>(w);
         const int c0 = w.req.c, hi = c0 + w.tile.i1 + 1, low_all = a.window > 0 ? c0 + w.tile.i0 - a.window + 1 : 0;
         const int rows = w.tile.rows, row0 = w.tile.row0, kt0 = w.tile.first + w.k, kh = w.kh;
         const int* bt = a.table + (size_t)w.r * a.W;
@@ -329,8 +332,8 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
                 if (e == 0) *reinterpret_cast<float2*>(a.part_ml + (place * M + row) * 2) = make_float2(m, l);
             }
         }
-        if (begins && !ends && tid == 0) ch_leave(a, w, c, n);
-        if (!ch_next<M, KT>(a, w, n)) break;
+        if (begins && !ends && tid == 0) ch_leave<S>(a, w, c);
+        if (!ch_next<S>(a, w, n)) break;
         __syncthreads();                          // the ring's memory is the next item's
     }
     if (bad) atomicOr(a.err, bad);
@@ -353,7 +356,7 @@ extern "C" int aie_attention_chunks_f32(const ChCall* call, int dtype, cudaStrea
     if (call->R <= 0 || call->T <= 0) return 0;
     if (call->d <= 0 || call->d > 256 || call->d % 8) return AIE_UNSUPPORTED;
     ChArgs a;
-    const int rc = ch_args(call, 32, 32, &a);
+    const int rc = ch_args(call, 32, 32, 8, &a);
     if (rc) return rc;
     const int w = a.d <= 64 ? 0 : a.d <= 128 ? 1 : 2;
     if (dtype == AIE_F32) return w == 0 ? launch_chunk_f32<float, 64>(a, stream) : w == 1 ? launch_chunk_f32<float, 128>(a, stream) : launch_chunk_f32<float, 256>(a, stream);

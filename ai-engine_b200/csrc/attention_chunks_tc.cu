@@ -33,7 +33,10 @@
 #define CT_RESCALE_STEP 8.0f
 
 template <int D> struct CtShape {
-    static constexpr int M = 2 * CT_M;                 // rows of an item
+    static constexpr int M = 2 * CT_M, KT = CT_KT;     // rows of an item, keys of a tile
+    // both streams take every key tile of an item of more than 128 rows, one of them that of a smaller one
+    static constexpr int MAX_WEIGHT = 2;
+    static __device__ __forceinline__ int weight(int rows) { return rows > CT_M ? 2 : 1; }
     static constexpr int tile = 128 * D * 2;           // bytes of 128 rows
     static constexpr int NS = D == 128 ? 5 : 10;       // tiles of keys or values in the ring
     // [3 KB: barriers, what the walk and the streams tell one another | queries x 2 | ring], 227 KB at heads of 128: nothing is left
@@ -95,7 +98,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         return;
     }
     ChWalk w;
-    if (!ch_begin<CT_THREADS, M, CT_KT>(a, c, C, sh, w)) return;
+    if (!ch_begin<CT_THREADS, S>(a, c, C, sh, w)) return;
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc_smem(tmem_slot)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
@@ -126,7 +129,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                 }
             };
             for (;;) {
-                const int n = ch_share(w), L = min(ct_ahead(w.tile), n), kt0 = w.tile.first + w.k;
+                const int n = ch_share<S>(w), L = min(ct_ahead(w.tile), n), kt0 = w.tile.first + w.k;
                 const int hi = w.req.c + w.tile.i1 + 1, low = a.window > 0 ? w.req.c + w.tile.i0 - a.window + 1 : 0;
                 const int* bt = a.table + (size_t)w.r * a.W;
                 // the page of this lane's box of tile j (read some tiles ahead of its use), and its first group of 8 rows
@@ -165,7 +168,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                 }
                 if (!ok) break;
                 if (!values) skip(L);
-                if (!ch_next<M, CT_KT>(a, w, n)) break;
+                if (!ch_next<S>(a, w, n)) break;
             }
             if (lane == 0) {
                 armed[2 * values] = mine;
@@ -201,7 +204,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                 }
             };
             for (;;) {
-                const int n = ch_share(w), L = ct_ahead(w.tile);
+                const int n = ch_share<S>(w), L = ct_ahead(w.tile);
                 const bool pair = L == 1, ends = w.k + n == w.tile.tiles;
                 const int past = w.req.c + w.tile.i1 + 1 - (w.tile.first + w.tile.tiles - 1) * CT_KT;      // keys of the item's last tile
                 const int q0 = nq & 1, q1 = pair ? q0 ^ 1 : q0, qp0 = (nq >> 1) & 1, qp1 = ((nq + 1) >> 1) & 1;
@@ -271,14 +274,14 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                         }
                     }
                 }
-                if (!ch_next<M, CT_KT>(a, w, n)) break;
+                if (!ch_next<S>(a, w, n)) break;
             }
         } else {
             // queries: every lane has four rows (token, head) of an item's tile; rows beyond the item's are zeros
             int nq = 0;
             bool ok = true;
             for (; ok;) {
-                const int n = ch_share(w), tiles = w.tile.rows > CT_M ? 2 : 1;
+                const int n = ch_share<S>(w), tiles = w.tile.rows > CT_M ? 2 : 1;
                 for (int t = 0; t < tiles && ok; ++t, ++nq) {
                     if (lane == 0) ok = mbar_wait(&q_empty[nq & 1], (unsigned)(((nq >> 1) & 1) ^ 1), abort_flag, a.err);
                     ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
@@ -301,7 +304,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                     __syncwarp();
                     if (lane == 0) mbar_arrive_plain(&q_full[nq & 1]);
                 }
-                if (!ok || !ch_next<M, CT_KT>(a, w, n)) break;
+                if (!ok || !ch_next<S>(a, w, n)) break;
             }
         }
     } else {
@@ -314,7 +317,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         unsigned s_ph = 0, o_ph = 0;
         bool ok = true;
         for (;;) {
-            const int n = ch_share(w), kt0 = w.tile.first + w.k;
+            const int n = ch_share<S>(w), kt0 = w.tile.first + w.k;
             const bool pair = w.tile.rows > CT_M;
             const int at = pair ? t * CT_M + row : row;                // row of the item
             const bool live = at - lane < w.tile.rows;                 // any row of this warp
@@ -472,10 +475,10 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                 }
                 if (there && !whole && (pair || t == 0)) *reinterpret_cast<float2*>(a.part_ml + place * 2) = make_float2(m_run, l_run);
             }
-            if (begins && !ends && tid == 0 && ok) ch_leave(a, w, c, n);
+            if (begins && !ends && tid == 0 && ok) ch_leave<S>(a, w, c);
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
             if (!pair) asm volatile("bar.sync %0, %1;\n" ::"r"(CT_BAR_MEET + 1), "r"(2 * CT_M) : "memory");      // both have read the outputs
-            if (!ch_next<M, CT_KT>(a, w, n)) break;
+            if (!ch_next<S>(a, w, n)) break;
         }
     }
 
@@ -515,7 +518,7 @@ template <int D> static int launch_chunk_tc(const ChArgs& a, int C, cudaStream_t
 extern "C" int aie_attention_chunks_tc(const ChCall* call, cudaStream_t stream) {
     if (call->R <= 0 || call->T <= 0) return 0;
     ChArgs a;
-    const int rc = ch_args(call, 128, CT_KT, &a);
+    const int rc = ch_args(call, 128, CT_KT, 2, &a);
     if (rc) return rc;
     if (a.P % 8 || (CT_KT % a.P && a.P % CT_KT) || (long long)a.num_pages * a.K * a.P / 8 > 0x7ffffffe) return AIE_UNSUPPORTED;
     if (a.d == 64) return launch_chunk_tc<64>(a, aie_sm_count(), stream);
