@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
         auto key_of = [&](int i) { return (kt0 + i) * KT + group * CK + gt / TPK; };
         auto page_of = [&](int i) {
             const int key = key_of(i);
-            return i < n && key < hi && key >= low_all ? __ldg(bt + ch_over(key, a.by_p)) : -1;
+            return i < n && key < hi && key >= low_all ? bt[ch_over(key, a.by_p)] : -1;
         };
         int page = page_of(0), page_next = page_of(1);
         // queries of the item: they land with the first stage

@@ -49,7 +49,8 @@ struct ChArgs : ChCall {
 static inline int ch_args(const ChCall* call, int M, int KT, int weight, ChArgs* a) {
     *static_cast<ChCall*>(a) = *call;
     if (a->W <= 0 || a->num_pages <= 0 || a->P <= 0 || a->K <= 0 || a->H <= 0 || a->H % a->K || a->G != a->H / a->K) return AIE_BAD_ARG;
-    // the line's length has to fit 31 bits: every request at least one row tile a key head, each over all the table's keys
+    // the line's length has to fit 31 bits: every request at least one row tile a key head, each over all the table's keys (where
+    // requests name the same rows more than once, ch_begin finds what this does not)
     const double items = (double)a->T * a->H / M + (double)a->R * a->K, keys = (double)a->W * a->P / KT + 2;
     if (items * keys * weight > 2147000000.0) return -3;
     a->by_g = ch_div((unsigned)a->G);
@@ -96,23 +97,23 @@ struct ChWalk {
     ChTile tile;
 };
 struct ChShared {
-    int sums[32];
+    long long sums[16];     // of a block's warps
     int r, off, n, c, s0;    // request in which the share begins, how far behind the request's first tile, its lengths
 };
 
 // Adds up `v` over the block in the order of threads; the result is what comes before this thread's, `all` the sum.
-template <int THREADS> __device__ __forceinline__ int ch_scan(int v, ChShared* s, int* all) {
+template <int THREADS> __device__ __forceinline__ long long ch_scan(int v, ChShared* s, long long* all) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int x = v;
+    long long x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
     __syncthreads();
     if (lane == 31) s->sums[warp] = x;
     __syncthreads();
-    int before = 0, total = 0;
+    long long before = 0, total = 0;
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) {
         if (w == warp) before = total;
@@ -144,7 +145,8 @@ template <typename Sh> __device__ __forceinline__ bool ch_item(const ChArgs& a, 
 template <int THREADS, typename Sh>
 __device__ __forceinline__ bool ch_begin(const ChArgs& a, int c, int C, ChShared* s, ChWalk& w) {
     const int tid = threadIdx.x;
-    int all = 0, mine = 0, before = 0;
+    int mine = 0;
+    long long all = 0, before = 0;
     ChReq q = {0, 0};
     for (int base = 0; base < a.R; base += THREADS) {
         const int r = base + tid;
@@ -155,9 +157,13 @@ __device__ __forceinline__ bool ch_begin(const ChArgs& a, int c, int C, ChShared
             mine = a.K * ch_length<Sh>(a, q);
             if (bad && c == 0) atomicOr(a.err, bad);
         }
-        int sum;
+        long long sum;
         before = all + ch_scan<THREADS>(mine, s, &sum);
         all += sum;
+    }
+    if (all > 0x7fffffff) {          // only where requests name the same rows again and again: their lengths do not fit q together
+        if (c == 0 && tid == 0) atomicOr(a.err, AIE_DEV_SLOT_OOB);
+        return false;
     }
     // at least the weight of a tile: a tile then begins in every share that lies within one item
     w.per = max((int)(((unsigned)all + C - 1) / (unsigned)C), Sh::MAX_WEIGHT);
@@ -172,16 +178,16 @@ __device__ __forceinline__ bool ch_begin(const ChArgs& a, int c, int C, ChShared
         s->s0 = a.q_start[r];
     };
     if (a.R <= THREADS) {
-        if (at >= before && at < before + mine) leave(tid, q, at - before);
+        if (at >= before && at < before + mine) leave(tid, q, (int)(at - before));
     } else {
-        int upto = 0;
+        long long upto = 0;
         for (int base = 0; base < a.R; base += THREADS) {
             const int r = base + tid;
             q = r < a.R ? ch_req(a, r) : ChReq{0, 0};
             const int here = r < a.R ? a.K * ch_length<Sh>(a, q) : 0;
-            int sum;
-            const int b = upto + ch_scan<THREADS>(here, s, &sum);
-            if (at >= b && at < b + here) leave(r, q, at - b);
+            long long sum;
+            const long long b = upto + ch_scan<THREADS>(here, s, &sum);
+            if (at >= b && at < b + here) leave(r, q, (int)(at - b));
             upto += sum;
         }
     }

@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
         const int my_key = group * 16 + (gt >> 3);
         auto page_of = [&](int i) {
             const int k_at = (kt0 + i) * KT + my_key;
-            return i < n && k_at < hi && k_at >= low_all ? __ldg(bt + ch_over(k_at, a.by_p)) : -1;
+            return i < n && k_at < hi && k_at >= low_all ? bt[ch_over(k_at, a.by_p)] : -1;
         };
         int page = page_of(0), page_next = page_of(1);
         // queries of the item: they land with the first stage

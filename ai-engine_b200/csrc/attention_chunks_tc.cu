@@ -118,6 +118,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             const bool values = warp == 10;
             const CUtensorMap* map = values ? &map_v : &map_k;
             const int BP = min(a.P, CT_KT), boxes = CT_KT / BP;      // rows of a box; lane i asks for box i of a tile
+            asm volatile("fence.proxy.async.global;\n" ::: "memory");      // the pages were written through the other proxy, by the kernels before
             int slot = 0, ph = 1;
             unsigned bad = 0, mine = 0, phase = 0;
             bool ok = true;
@@ -137,7 +138,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                     const int key = (kt0 + j) * CT_KT + lane * BP;
                     return j < n && lane < boxes && key < hi && key + BP > low;
                 };
-                auto page_of = [&](int j) { return wanted(j) ? __ldg(bt + ch_over((kt0 + j) * CT_KT + lane * BP, a.by_p)) : -1; };
+                auto page_of = [&](int j) { return wanted(j) ? bt[ch_over((kt0 + j) * CT_KT + lane * BP, a.by_p)] : -1; };
                 auto group_of = [&](int j, int page) {
                     if (!wanted(j)) return end_group;
                     if (page >= 0 && page < a.num_pages) {

@@ -35,8 +35,8 @@ template <typename T, int V> __device__ __forceinline__ void cw_load(CwVec<T, V>
 
 template <typename I, typename C, int V>
 __global__ void __launch_bounds__(CW_THREADS)
-write_kv_slots_kernel(const I* __restrict__ k, const I* __restrict__ v, long long k_token, long long k_head, long long v_token,
-                      long long v_head, C* __restrict__ k_pages, C* __restrict__ v_pages, const int* __restrict__ slots,
+write_kv_slots_kernel(const I* k, const I* v, long long k_token, long long k_head, long long v_token,
+                      long long v_head, C* k_pages, C* v_pages, const int* slots,
                       unsigned total, unsigned per_plane, CwDiv by_token, CwDiv by_head, CwDiv by_p, int P, int K, int d, int n_slots,
                       unsigned* err) {
     pdl_launch_dependents();
@@ -53,7 +53,7 @@ write_kv_slots_kernel(const I* __restrict__ k, const I* __restrict__ v, long lon
             head[u] = (int)h;
             at[u] = (int)(unit - h * per_head) * V;
             const bool is_v = (int)h >= K;
-            slot[u] = __ldg(slots + t);
+            slot[u] = slots[t];
             cw_load<I, V>(x[u], is_v ? v + t * v_token + (long long)(h - K) * v_head + at[u] : k + t * k_token + (long long)h * k_head + at[u]);
         }
     }

@@ -29,11 +29,11 @@ __device__ __forceinline__ long long st_shfl_up(long long v, int o) { return __s
 
 template <bool VEC>
 __global__ void __launch_bounds__(ST_THREADS, 2)
-step_tables_kernel(const int* __restrict__ cached, const int* __restrict__ counts, const int* __restrict__ held_in,
-                   const int* __restrict__ tables_in, const int* __restrict__ free_pages, const int* __restrict__ free_count, int R, int W,
-                   int F, int P, int num_pages, int capacity, int table_blocks, int* __restrict__ tables, int* __restrict__ held,
-                   int* __restrict__ free_left, int* __restrict__ q_start, int* __restrict__ q_len, int* __restrict__ positions,
-                   int* __restrict__ token_req, int* __restrict__ slots, unsigned* err) {
+step_tables_kernel(const int* cached, const int* counts, const int* held_in,
+                   const int* tables_in, const int* free_pages, const int* free_count, int R, int W,
+                   int F, int P, int num_pages, int capacity, int table_blocks, int* tables, int* held,
+                   int* free_left, int* q_start, int* q_len, int* positions,
+                   int* token_req, int* slots, unsigned* err) {
     extern __shared__ StRow rows[];
     __shared__ long long w_tokens[ST_THREADS / 32], w_pages[ST_THREADS / 32];
     __shared__ long long s_taken;
@@ -125,8 +125,8 @@ step_tables_kernel(const int* __restrict__ cached, const int* __restrict__ count
                 const int w = w0 + u * 32 * V;
                 e[u] = make_int4(-1, -1, -1, -1);
                 if (VEC ? w + V <= s.held : w < s.held) {
-                    if (VEC) e[u] = __ldg(reinterpret_cast<const int4*>(from + w));
-                    else e[u].x = __ldg(from + w);
+                    if (VEC) e[u] = *reinterpret_cast<const int4*>(from + w);
+                    else e[u].x = from[w];
                 }
             }
 #pragma unroll

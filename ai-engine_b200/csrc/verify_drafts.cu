@@ -48,11 +48,11 @@ struct VdMinus {
 // weights of the four tokens t .. t + 3; tokens from `V` on weigh nothing
 template <bool VEC> __device__ __forceinline__ void vd_load(float (&x)[4], const float* row, int t, int V) {
     if (VEC && t + 4 <= V) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(row + t));
+        const float4 a = *reinterpret_cast<const float4*>(row + t);
         x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = t + k < V ? __ldg(row + t + k) : 0.f;
+        for (int k = 0; k < 4; ++k) x[k] = t + k < V ? row[t + k] : 0.f;
     }
 }
 // the weights of a warp's segment: lane l has tokens 128 j + 4 l .. + 3 of it
@@ -74,10 +74,10 @@ template <bool VEC> __device__ __forceinline__ void vd_segment(u64 (&w)[4][4], c
 
 template <bool VEC, int VD_THREADS>
 __global__ void __cluster_dims__(VD_CLUSTER, 1, 1) __launch_bounds__(VD_THREADS, 1024 / VD_THREADS)
-verify_drafts_kernel(const float* __restrict__ target, long long target_row, int T, int V, const int* __restrict__ q_start,
-                     const int* __restrict__ draft_tokens, const int* __restrict__ draft_len, const float* __restrict__ draft_probs,
-                     long long draft_req, long long draft_place, int N, const float* __restrict__ accept_draws,
-                     const float* __restrict__ token_draws, int* __restrict__ tokens, int* __restrict__ emitted, unsigned* err) {
+verify_drafts_kernel(const float* target, long long target_row, int T, int V, const int* q_start,
+                     const int* draft_tokens, const int* draft_len, const float* draft_probs,
+                     long long draft_req, long long draft_place, int N, const float* accept_draws,
+                     const float* token_draws, int* tokens, int* emitted, unsigned* err) {
     __shared__ u64 seg_sum[VD_MAX_SEGMENTS];
     __shared__ u64 warp_sum[VD_THREADS / 32];
     __shared__ u64 sums[2][VD_CLUSTER];     // of every block: of w, of p alone

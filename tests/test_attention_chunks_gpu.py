@@ -197,3 +197,33 @@ def test_rows_whose_offset_passes_32_bits():
         b[name] = big
     b["table"] = torch.where(b["table"] >= 0, b["table"] + far, b["table"]).int()
     assert torch.equal(call(b)[0], want)
+
+
+def test_rows_named_again_and_again(monkeypatch):
+    """Requests may name the same rows.  So many of them that their work does not fit 31 bits bring nothing and are flagged."""
+    from ai_engine_b200.kernels import ops
+
+    b = paged_batch([70], [3], 8, 2, 64, 16, BF16, 15)
+    want = check(b, BF16)
+    twice = dict(b, **{k: torch.cat([b[k], b[k]]) for k in ("q_start", "q_len", "ctx_len", "table")})
+    out, word = call(twice)
+    assert word == 0 and torch.equal(out, want)
+    monkeypatch.setattr(ops, "CHUNK_FORM", 16)
+    R, n, W = 12000, 2000, 1024               # 12,000 x 8 key heads x 250 row tiles x 110 key tiles and more: 2.6e9
+    ints = lambda x, *s: torch.full(s, x, dtype=torch.int32, device=DEV)
+    q = torch.full((n, 32, 64), 2.0, dtype=BF16, device=DEV)
+    pool = torch.zeros(4, 8, 16, 64, dtype=BF16, device=DEV)
+    out, e = torch.full_like(q, 7.0), ints(0, 1)
+    ops.paged_attention_chunks(q, pool, pool, ints(0, R), ints(n, R), ints(14000, R), ints(0, R, W), 0.1, 0, e, out=out)
+    assert int(e.item()) == 8 and (out == 7).all()
+
+
+def test_sizes_whose_work_does_not_fit():
+    """A table so wide and so many rows that the work could not be counted: refused before anything runs."""
+    from ai_engine_b200.kernels import ops
+    from ai_engine_b200.kernels.loader import KernelError
+
+    pool = torch.zeros(1, 1, 128, 64, dtype=F32, device=DEV)
+    ints = lambda *s: torch.zeros(s, dtype=torch.int32, device=DEV)
+    with pytest.raises(KernelError):
+        ops.paged_attention_chunks(torch.zeros(4096, 64, 64, device=DEV), pool, pool, ints(1), ints(1), ints(1), ints(1, 1 << 19), 0.1, 0, ints(1))
