@@ -55,7 +55,7 @@ step_tables_kernel(const int* cached, const int* counts, const int* held_in,
             n = counts[r];
             h = held_in[r];
             c = cached[r];
-            if (n < 0 || c < 0 || h < 0 || h > W) {
+            if (n < 0 || c < 0 || h < 0 || h > W || c + n > 0x7fffffffll) {      // (n is 64 bits wide)
                 bad |= AIE_DEV_SLOT_OOB;
                 n = 0;
                 c = 0;

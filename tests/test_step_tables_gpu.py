@@ -83,7 +83,7 @@ def test_lengths_that_do_not_fit_wait_and_are_flagged():
     assert word == 8 and got.q_len.tolist() == [1, 1, 0, 1, 2] and got.held.tolist() == [3, 2, 4, 2, 1]
     assert got.q_start.tolist() == [0, 1, 2, 4, 5] and got.slots.tolist()[2:4] == [-1, -1] and got.free_count.tolist() == [3]
     # negative lengths
-    for key, values in (("cached", [16, -8, 31, 8, 3]), ("held", [2, -1, 4, 1, 1]), ("counts", [1, -1, 1, 1, 2]), ("held", [2, 5, 4, 1, 1])):
+    for key, values in (("cached", [16, 0x7fffffff, 31, 8, 3]), ("cached", [16, -8, 31, 8, 3]), ("held", [2, -1, 4, 1, 1]), ("counts", [1, -1, 1, 1, 2]), ("held", [2, 5, 4, 1, 1])):
         a = dict(good)
         a[key] = values
         got, word = call(a["cached"], a["counts"], a["held"], table, free, 6, P, 30, 10)
