@@ -323,6 +323,8 @@ PyObject* paged_attention_chunks(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor* given = maybe(w, "out", a[10]);
         long long form = integer(w, "form", a[11]);
         const Pools p = pools(w, kp, vp);
+        // (the launchers check the rest of what a form takes; the types of the operands they do not see)
+        if (form > FLOAT32 && p.code != 1) refuse(w, "form " + std::to_string(form) + " takes bfloat16 pools only");
         if (q.dim() != 3 || q.size(2) != p.d || q.size(1) == 0 || q.size(1) % p.K || q.scalar_type() != kp.scalar_type())
             refuse(w, "queries " + type_text(q) + " must be [T, a multiple of " + std::to_string(p.K) + ", " + std::to_string(p.d) + "] in the pools' dtype");
         const int64_t T = q.size(0), H = q.size(1);

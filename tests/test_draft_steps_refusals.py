@@ -49,6 +49,13 @@ def test_attention_refuses(change):
         attend(**change)
 
 
+@pytest.mark.parametrize("form", [1, 16, 18, 24])
+def test_attention_refuses_forms_of_another_type(form, monkeypatch):
+    monkeypatch.setattr(ops, "CHUNK_FORM", form)
+    with pytest.raises(ops.KernelError, match="bfloat16 pools only"):
+        attend(q=torch.zeros(6, 8, 64), k_pages=torch.zeros(5, 2, 16, 64), v_pages=torch.zeros(5, 2, 16, 64))
+
+
 def write(**change):
     a = dict(k=torch.zeros(6, 2, 64), v=torch.zeros(6, 2, 64), k_pages=torch.zeros(5, 2, 16, 64, dtype=BF16),
              v_pages=torch.zeros(5, 2, 16, 64, dtype=BF16), slots=ints(6), err=ints(1))
