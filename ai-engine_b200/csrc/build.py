@@ -155,19 +155,17 @@ def draft_module_path() -> str:
     """Path of the extension module of csrc/host/draft_ops.cpp, compiled against the installed torch."""
     import torch
 
-    folder = os.path.join(CSRC, "host")
-    src = os.path.join(folder, "draft_ops.cpp")
-    root = os.path.dirname(os.path.abspath(torch.__file__))
-    cuda = os.path.dirname(os.path.dirname(find_nvcc()))
+    src = os.path.join(CSRC, "host", "draft_ops.cpp")
     flags = CXX_FLAGS + [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
-    places = [f"-I{p}" for p in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
-                                 os.path.join(cuda, "include"), sysconfig.get_paths()["include"])]
-    lib = os.path.join(root, "lib")
-    libs = [f"-L{lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", f"-Wl,-rpath,{lib}"]
     key = _hash([src], flags + [torch.__version__, sysconfig.get_config_var("SOABI") or sys.version])
     target = os.path.join(build_dir(), f"_aie_draft_ops-{key}.so")
     if os.path.exists(target):
         return target
+    root, cuda = os.path.dirname(os.path.abspath(torch.__file__)), os.path.dirname(os.path.dirname(find_nvcc()))
+    places = [f"-I{p}" for p in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                                 os.path.join(cuda, "include"), sysconfig.get_paths()["include"])]
+    lib = os.path.join(root, "lib")
+    libs = [f"-L{lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", f"-Wl,-rpath,{lib}"]
     cxx = os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++")
     if not cxx:
         raise BuildError("no C++ compiler found (g++): the host side of the draft operators cannot be built")
