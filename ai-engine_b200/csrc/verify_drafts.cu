@@ -26,6 +26,7 @@ typedef unsigned long long u64;
 #define VD_CLUSTER 8
 #define VD_SEGMENT 512          // tokens a warp adds up at a time: four of 16 bytes a lane, of each row
 #define VD_MAX_SEGMENTS 256     // a block's: 1,048,576 tokens of vocabulary
+#define VD_TOO_MUCH (~0ull)     // a sum that does not fit
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory"); }
@@ -165,19 +166,26 @@ verify_drafts_kernel(const float* target, long long target_row, int T, int V, co
         __syncthreads();
         if (round == 0) cluster_wait();
         if (tid < VD_CLUSTER) {                    // to block `tid`
-            u64 a = 0;
+            // a warp's sum is below 2^62; a block's from 2^60 on is that of no distribution, and would not fit when the blocks' are added
+            u64 a = 0, high = 0;
 #pragma unroll
-            for (int w = 0; w < VD_THREADS / 32; ++w) a += warp_sum[w];
-            *cluster.map_shared_rank(&sums[round][rank], tid) = a;
+            for (int w = 0; w < VD_THREADS / 32; ++w) {
+                a += warp_sum[w];
+                high += warp_sum[w] >> 32;
+            }
+            *cluster.map_shared_rank(&sums[round][rank], tid) = high >> 28 ? VD_TOO_MUCH : a;
         }
         cluster.sync();
         before = total = 0;
+        bool fits = true;
 #pragma unroll
         for (int b = 0; b < VD_CLUSTER; ++b) {
             const u64 a = sums[round][b];
             if (b < rank) before += a;
             total += a;
+            fits = fits && a != VD_TOO_MUCH;
         }
+        if (!fits) total = 0;
         if (total > 0 || round == 1 || kept == n) break;      // the same in all blocks
         minus.row = nullptr;
         minus.token = -1;
@@ -188,7 +196,7 @@ verify_drafts_kernel(const float* target, long long target_row, int T, int V, co
             if (i != kept) out[i] = i < kept ? draft_tokens[(size_t)r * N + i] : -1;
         if (tid == 0) {
             emitted[r] = kept + 1;
-            if (total == 0) {                      // a row of zeros: no token can be drawn from it
+            if (total == 0) {                      // a row of zeros, or of no probabilities: no token can be drawn from it
                 out[kept] = 0;
                 atomicOr(err, AIE_DEV_NO_MASS);
             }

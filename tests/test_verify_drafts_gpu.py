@@ -112,6 +112,17 @@ def test_rows_that_are_not_distributions():
         assert call(row, [0], [[0]], [0], None, [[0.5]], [u])[0] == [[t, -1]]
 
 
+@pytest.mark.parametrize("R", [1, 20, 40])
+def test_rows_whose_sums_do_not_fit(R):
+    """Entries that are no probabilities: 70,000 ones weigh more than 64 bits hold; 20,000 still fit and are drawn from."""
+    ask = lambda row: call(row.expand(2, -1), [0] * R, [[-1]] * R, [1] * R, None, [[0.5]] * R, [0.5] * R)
+    for V, first in ((70000, 0), (100000, 12800), (1048576, 0)):
+        row = torch.ones(1, V)
+        row[:, :first] = 0
+        assert ask(row) == ([[0, -1]] * R, [1] * R, 1 | 16)
+    assert ask(torch.ones(1, 20000)) == ([[10000, -1]] * R, [1] * R, 1)
+
+
 def test_rows_and_tokens_that_are_not_there():
     target = torch.softmax(torch.randn(3, 600, generator=torch.Generator().manual_seed(2)), -1)
     for start, n in ((2, 1), (-1, 0), (3, 0), (0, 3), (2 ** 31 - 1, 1)):
