@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
         if (w.req.n == 0) return;                 // the whole cluster
         cb_part<S>(a, w, 0, rank, S_blocks);
     } else {
-        if (tid == 0) a.meta[2 * c] = make_int4(0, 0, 0, 0);
+        if (tid == 0) a.meta[c] = make_int4(0, 0, 0, 0);
         if (!ch_begin<THREADS, S>(a, c, C, &sh, w)) return;
     }
     const unsigned smem = (unsigned)__cvta_generic_to_shared(cb_smem);

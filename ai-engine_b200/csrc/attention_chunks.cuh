@@ -7,8 +7,8 @@
 //
 // All items' key tiles stand in one line, in the order of requests, key heads and row tiles, each as long as it takes (a weight by the
 // item's rows); block c of C takes those that begin in [c * per, (c + 1) * per), per = ceil(all / C), so every block has the same work
-// whatever the requests' lengths.  Every block works out the line from the lengths by itself (sums over the requests), so nothing comes from the host and a
-// captured call follows the lengths.  An item that a block does not finish is left as a part: sums of exp2(x - m) v without
+// whatever the requests' lengths.  Every block works out the line from the lengths by itself (sums over the requests), so nothing comes from
+// the host and a captured call follows the lengths.  An item that a block does not finish is left as a part: sums of exp2(x - m) v without
 // division, m and l, in a place of the block's own (one for an item that it began, one for an item that it continued), and a second,
 // small kernel joins the parts of every item in their order.  The split depends on all requests' lengths: the sums of a token
 // are taken in another order in another batch.
@@ -35,7 +35,7 @@ struct ChCall {                       // what a caller packs, in this order
     const int *q_start, *q_len, *ctx_len, *table;
     float* part_o;                    // [2 * C][M][D]
     float* part_ml;                   // [2 * C][M][2]
-    int4* meta;                       // [C][2] of the item that block c began and did not finish: key head, first row, rows, parts; first token
+    int4* meta;                       // [C] of the item that block c began and did not finish: key head, first row, rows and 2^16 parts (0: none), first token
     long long q_token, q_head;
     int R, W, T, num_pages, P, H, K, G, d, window;
     float scale2;                     // scale * log2 e: exponentials are powers of two
@@ -221,32 +221,33 @@ template <typename Sh> __device__ __forceinline__ bool ch_next(const ChArgs& a, 
 // What the joining kernel has to know of the item that block c begins here and does not finish.
 template <typename Sh> __device__ __forceinline__ void ch_leave(const ChArgs& a, const ChWalk& w, int c) {
     const int last = (w.tile.tiles - 1) * Sh::weight(w.tile.rows);      // where its last tile begins, from the item's beginning
-    a.meta[2 * c] = make_int4(w.kh, w.tile.row0, w.tile.rows, last < w.left ? 1 : 2 + (last - w.left) / w.per);
-    a.meta[2 * c + 1] = make_int4(w.s0, 0, 0, 0);
+    const int parts = last < w.left ? 1 : 2 + (last - w.left) / w.per;      // at most as many as there are blocks
+    a.meta[c] = make_int4(w.kh, w.tile.row0, w.tile.rows | parts << 16, w.s0);
 }
 __device__ __forceinline__ float ch_inverse(float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); }      // of a row's sum; a row that sees nothing is zero
 
 // Joins the parts of the items that blocks c .. c + PER - 1 began: out = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p, four columns of a row a
-// thread.  Items of 256 rows take 32 blocks, so that one in sixty parts does not take eight of them 30 us, and a block looks at
-// four of them, so that there are no more blocks than the machine holds at once (a list of the items with parts, made by every
-// block, cost 4 us).
+// thread.  What bounds it is the way to memory, twice: what there is to join, then its parts.  Four parts' loads are under way together:
+// 60 registers, so that four blocks stay on an SM (eight parts and 80: 300 to 500 new tokens of four requests behind 6,000 to 9,000 228 us in
+// all instead of 223, calls of 20 to 100 us 6 % more).  Items of 256 rows take 32 blocks, so that one in sixty parts does not take eight
+// of them 30 us, and a block looks at two of them (at four or at one: 2 and 4 % more; a list of the items with parts, made by every block, cost 4 us).
 template <typename T, int M, int D, int PER>
 __global__ void __launch_bounds__(256) chunk_join_kernel(const ChArgs a, int C) {
     pdl_launch_dependents();
     pdl_wait();
-    constexpr int CH = D / 4;
+    constexpr int CH = D / 4, AT = 4;
     int4 its[PER];
 #pragma unroll
-    for (int x = 0; x < PER; ++x) its[x] = blockIdx.x * PER + x < C ? a.meta[2 * (blockIdx.x * PER + x)] : make_int4(0, 0, 0, 0);
+    for (int x = 0; x < PER; ++x) its[x] = blockIdx.x * PER + x < C ? a.meta[blockIdx.x * PER + x] : make_int4(0, 0, 0, 0);
 #pragma unroll 1
     for (int x = 0; x < PER; ++x) {
         int4 it = its[0];
 #pragma unroll
         for (int y = 1; y < PER; ++y)
             if (y == x) it = its[y];
-        if (it.w == 0) continue;
-        const int c = blockIdx.x * PER + x, s0 = a.meta[2 * c + 1].x;
-        for (int i = blockIdx.y * 256 + threadIdx.x; i < it.z * CH; i += gridDim.y * 256) {
+        const int c = blockIdx.x * PER + x, rows = it.z & 0xffff, parts = it.z >> 16;
+        if (parts == 0) continue;
+        for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * CH; i += gridDim.y * 256) {
             const int row = i / CH, e = (i - row * CH) * 4;
             if (e >= a.d) continue;
             // part 0 lies in block c's place for items begun, part p in block c + p's for items continued
@@ -254,24 +255,24 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const ChArgs a, int C) 
             const float* po = a.part_o + ((size_t)2 * c * M + row) * D + e;
             float m = -INFINITY, l = 0.f;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int p0 = 0; p0 < it.w; p0 += 8) {       // eight parts at a time, so that their loads are under way together
-                float2 g[8];
-                float4 z[8];
+            for (int p0 = 0; p0 < parts; p0 += AT) {
+                float2 g[AT];
+                float4 z[AT];
 #pragma unroll
-                for (int p = 0; p < 8; ++p) {
-                    const bool there = p0 + p < it.w;
+                for (int p = 0; p < AT; ++p) {
+                    const bool there = p0 + p < parts;
                     const size_t place = there ? (p0 + p == 0 ? 1 : 2 * (p0 + p)) : 1;
                     g[p] = there ? *reinterpret_cast<const float2*>(ml + place * (M * 2)) : make_float2(-INFINITY, 0.f);
                     if (there) z[p] = *reinterpret_cast<const float4*>(po + place * ((size_t)M * D));
                 }
                 float top = m;
 #pragma unroll
-                for (int p = 0; p < 8; ++p) top = fmaxf(top, g[p].x);
+                for (int p = 0; p < AT; ++p) top = fmaxf(top, g[p].x);
                 const float was = m == -INFINITY ? 0.f : exp2f(m - top);
                 l *= was;
                 o.x *= was, o.y *= was, o.z *= was, o.w *= was;
 #pragma unroll
-                for (int p = 0; p < 8; ++p) {
+                for (int p = 0; p < AT; ++p) {
                     if (g[p].x == -INFINITY) continue;
                     const float f = exp2f(g[p].x - top);
                     l += f * g[p].y;
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const ChArgs a, int C) 
             }
             const float inv = ch_inverse(l);
             const int full = it.y + row, tok = ch_over(full, a.by_g), h = it.x * a.G + full - tok * a.G;
-            store4<T>(reinterpret_cast<T*>(a.out) + ((size_t)(s0 + tok) * a.H + h) * a.d + e,
+            store4<T>(reinterpret_cast<T*>(a.out) + ((size_t)(it.w + tok) * a.H + h) * a.d + e,
                       make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
         }
     }
@@ -296,7 +297,7 @@ template <typename F> static void ch_prepare(F kern, int bytes, unsigned long lo
 }
 // ... with as much shared memory an SM as the kernel before it, which would otherwise have to leave the SM before it changes
 template <typename T, int M, int D> static int launch_chunk_join(const ChArgs& a, int C, cudaStream_t st) {
-    constexpr int PER = M > 32 ? 4 : 1;
+    constexpr int PER = M > 32 ? 2 : 1;
     auto kern = chunk_join_kernel<T, M, D, PER>;
     static unsigned long long done = 0;
     ch_prepare(kern, 0, &done);

@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int group = warp % NG, mt = warp / NG, gt = mt * 32 + lane;      // mt: which eight rows
     const int c = blockIdx.x, C = gridDim.x;
-    if (tid == 0) a.meta[2 * c] = make_int4(0, 0, 0, 0);
+    if (tid == 0) a.meta[c] = make_int4(0, 0, 0, 0);
     ChWalk w;
     if (!ch_begin<THREADS, S>(a, c, C, &sh, w)) return;
     float* ring = cf_smem + group * NST * S::stage;

@@ -92,7 +92,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         tma_prefetch_map(&map_v);
     }
     pdl_wait();
-    if (tid == 0) a.meta[2 * c] = make_int4(0, 0, 0, 0);
+    if (tid == 0) a.meta[c] = make_int4(0, 0, 0, 0);
     if (tc_smem(sm) & 1023u) {                      // swizzled tiles would not be where the products look for them
         if (tid == 0) atomicOr(a.err, AIE_DEV_WAIT_TIMEOUT);
         return;

@@ -354,9 +354,9 @@ PyObject* paged_attention_chunks(PyObject*, PyObject* const* a, Py_ssize_t n) {
             const int64_t wide = form == FLOAT32 ? (p.d <= 64 ? 64 : p.d <= 128 ? 128 : 256) : p.d;
             const int64_t M = form == TCGEN05 ? 256 : 32;
             const int64_t blocks = form > MMA ? 0 : sm_count * (form == MMA ? 2 : 1), parts = 2 * blocks * M;
-            // parts [parts][wide], their maxima and sums [parts][2], what is to be joined [blocks][2] int4
+            // parts [parts][wide], their maxima and sums [parts][2], what is to be joined [blocks] int4
             at::Tensor scratch;
-            if (blocks) scratch = fresh({parts * (wide + 2) + 8 * blocks}, at::kFloat, q);
+            if (blocks) scratch = fresh({parts * (wide + 2) + 4 * blocks}, at::kFloat, q);
             float* s = blocks ? scratch.data_ptr<float>() : nullptr;
             const ChCall call = {q.data_ptr(), kp.data_ptr(), vp.data_ptr(), out.data_ptr(), start.data_ptr(), len.data_ptr(), ctx.data_ptr(),
                                  table.data_ptr(), s, s + parts * wide, s + parts * (wide + 2), q.stride(0), q.stride(1), (int)R, (int)W, (int)T,
