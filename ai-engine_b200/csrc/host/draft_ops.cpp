@@ -1,6 +1,6 @@
 // Host side of the operators of a step that verifies drafted tokens: checks of their operands, outputs and scratch from torch's allocator,
 // one call of the CUDA launcher on the current stream.  Python's share of a call (checks and twenty arguments through ctypes)
-// was 8 to 17 us, as long as or longer than the kernels of a small step; here it is 3 to 6.
+// was 9 to 18 us, as long as or longer than the kernels of a small step; here it is 3.5 to 7.5.
 //
 // The launchers live in the libraries that kernels/loader.py compiles; the first call that wants one has it loaded.
 #include <Python.h>
@@ -274,9 +274,9 @@ PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
 enum { FLOAT32 = 0, MMA = 16, TCGEN05 = 1 };
 
 // Which of them takes a call, by what the host knows: tokens, requests, and how many keys a request can have (the table's width; a
-// window).  The least of the times that each would take, in us, fitted to 643 calls (1 to 64 requests of 1 to 200 tokens behind 40 to 20,000, four head
-// layouts; the choice is 4 % above the best form of each call on average): a fixed part, and one for every key tile of the
-// busiest block.  Only these proportions count, so the machine's numbers are no promise.
+// window).  The least of the times that each would take, in us, fitted to 643 calls (1 to 64 requests of 1 to 200 tokens behind 40 to 20,000,
+// four head layouts; the choice takes 1.2 % more than the best form of each call on average, 40 % where it is worst): a fixed part, one
+// for every key tile of the busiest block, one for every part of an item that is joined.  Only these proportions count.
 int chunk_form(int code, const Pools& p, int64_t R, int64_t W, int64_t T, int64_t G, int64_t window) {
     if (code != 1 || (p.d != 64 && p.d != 128)) return FLOAT32;
     auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
@@ -285,7 +285,8 @@ int chunk_form(int code, const Pools& p, int64_t R, int64_t W, int64_t T, int64_
     if (window > 0) keys = std::min(keys, window + up(T, R));
     const int64_t tiles = up(keys, tile);
     int form = MMA;
-    double least = 6.5 + 1.5 * up(items * up(rows, 32) * tiles, 2 * sm_count);
+    const int64_t all = items * up(rows, 32), blocks = 2 * sm_count;
+    double least = 6.5 + 1.5 * up(all * tiles, blocks) + (all < blocks ? 0.1 * std::min((double)tiles, (double)blocks / all) : 0.0);
     if (p.P % 8 == 0 && (128 % p.P == 0 || p.P % 128 == 0) && p.N * p.K * p.P / 8 < 0x7fffffff) {
         // a tile of more than 128 rows takes both streams of a block for every key tile, one of fewer rows takes one of them
         const int64_t rest = rows % 256, pairs = rows / 256 + (rest > 128), lone = rest > 0 && rest <= 128;
@@ -298,7 +299,7 @@ int chunk_form(int code, const Pools& p, int64_t R, int64_t W, int64_t T, int64_
     // clusters: every block there at once, a row tile or little more each, and few key tiles, since nothing evens out unequal lengths
     for (int S = 8; S >= 2 && rows <= 32; S /= 2) {
         const int64_t each = up(tiles, S);
-        if (items * S > 2 * sm_count || each > 8) continue;
+        if (items * S > blocks || each > 8) continue;
         const double t = 5.0 + 0.9 * each;
         if (t < least) {
             least = t;
