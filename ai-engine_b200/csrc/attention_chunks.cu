@@ -88,10 +88,10 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
     pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = warp / GW, mt = warp % GW, gt = mt * 32 + lane;
-    const int c = blockIdx.x, C = gridDim.x, rank = CLUSTER ? c % S_blocks : 0;
+    const int rank = CLUSTER ? blockIdx.x % S_blocks : 0;
     ChWalk w;
     if constexpr (CLUSTER) {
-        const int item = c / S_blocks;
+        const int item = blockIdx.x / S_blocks;
         unsigned bad_lengths = 0;
         w.r = item / a.K;
         w.kh = item - w.r * a.K;
@@ -101,8 +101,8 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
         if (w.req.n == 0) return;                 // the whole cluster
         cb_part<S>(a, w, 0, rank, S_blocks);
     } else {
-        if (tid == 0) a.meta[c] = make_int4(0, 0, 0, 0);
-        if (!ch_begin<THREADS, S>(a, c, C, &sh, w)) return;
+        if (tid == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+        if (!ch_begin<THREADS, S>(a, blockIdx.x, gridDim.x, &sh, w)) return;
     }
     const unsigned smem = (unsigned)__cvta_generic_to_shared(cb_smem);
     const unsigned ring = smem + group * NST * S::stage * 2, q_s = smem + S::q_off;
@@ -268,7 +268,6 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
         __syncthreads();
 
         // the groups meet
-        w = place_in_line;
         float* o_s = reinterpret_cast<float*>(cb_smem);      // [groups][M][D]
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -277,14 +276,15 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
             l += __shfl_xor_sync(0xffffffffu, l, 1);
             l += __shfl_xor_sync(0xffffffffu, l, 2);
             if ((lane & 3) == 0) *reinterpret_cast<float2*>(ml + (group * M + row) * 2) = make_float2(m_run[e], l);
-            if (row < w.tile.rows)
+            if (row < place_in_line.tile.rows)
 #pragma unroll
                 for (int x = 0; x < D / 8; ++x)
                     *reinterpret_cast<float2*>(o_s + (group * M + row) * D + ((x * 8 + col) ^ ((row & 3) << 3))) = make_float2(o[x][2 * e], o[x][2 * e + 1]);
         }
         __syncthreads();
+        w = place_in_line;
         const bool begins = w.k == 0, ends = w.k + n == w.tile.tiles;
-        const size_t place = (size_t)2 * c + (begins ? 1 : 0);
+        const size_t place = (size_t)2 * blockIdx.x + (begins ? 1 : 0);
         for (int i = tid; i < w.tile.rows * (D / 4); i += THREADS) {
             const int row = i / (D / 4), e = (i % (D / 4)) * 4;
             float2 g[CB_GROUPS];
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
             if ((w.m + 1) * M >= w.req.n * a.G) break;
             cb_part<S>(a, w, w.m + 1, rank, S_blocks);
         } else {
-            if (begins && !ends && tid == 0) ch_leave<S>(a, w, c);
+            if (begins && !ends && tid == 0) ch_leave<S>(a, w, blockIdx.x);
             if (!ch_next<S>(a, w, n)) break;
             __syncthreads();                  // the ring's memory is the next item's
         }
