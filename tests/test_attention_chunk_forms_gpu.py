@@ -50,3 +50,17 @@ def test_scales(form, scale):
     b = paged_batch([300, 40], [40, 3], 4, 2, 64, 16, BF16, 9)
     b["scale"] = scale
     check(b, BF16)
+
+
+def test_out_may_be_the_queries(form):
+    """In place: the rows that requests name become their results, the others stay.  Items of one block, of several, and of several tiles."""
+    from ai_engine_b200.kernels import ops
+
+    for cached, new, H, K, d in (([300, 0, 1500], [9, 70, 3], 8, 2, 64), ([20000], [3], 4, 1, 128), ([40] * 60, [2] * 60, 4, 4, 64)):
+        b = paged_batch(cached, new, H, K, d, 16, BF16, sum(new), slack=2)
+        e = torch.zeros(1, dtype=torch.int32, device="cuda")
+        a = (b["k_pages"], b["v_pages"], b["q_start"], b["q_len"], b["ctx_len"], b["table"], b["scale"], 0, e)
+        apart = ops.paged_attention_chunks(b["q"], *a, out=b["q"].clone())
+        place = b["q"].clone()
+        assert ops.paged_attention_chunks(place, *a, out=place).data_ptr() == place.data_ptr()
+        assert torch.equal(place, apart) and int(e) == 0
