@@ -43,7 +43,7 @@ template <int D> struct CtShape {
     static constexpr int NS = D == 128 ? 5 : 10;       // tiles of keys or values in the ring
     // [3 KB: barriers, what the walk and the streams tell one another | queries x 2 | ring], 227 KB at heads of 128: nothing is left
     // for aligning the start, which the runtime puts on 1 KB as long as there is no other shared memory
-    static constexpr int walk_off = 256, warps_off = 480, meet_off = 1024, q_off = 3072, kv_off = q_off + 2 * tile, bytes = kv_off + NS * tile;
+    static constexpr int walk_off = 256, warps_off = 480, meet_off = 1024, q_off = 3 * 1024, kv_off = q_off + 2 * tile, bytes = kv_off + NS * tile;
 };
 
 // The order in which an item's tiles of keys (K) and values (V) pass through the ring: `ahead` tiles of keys, then V(j), K(j + ahead).

@@ -45,7 +45,7 @@ step_tables_kernel(const int* cached, const int* counts, const int* held_in,
     int avail = *free_count;
     if (avail < 0 || avail > F) { bad |= AIE_DEV_SLOT_OOB; avail = avail < 0 ? 0 : F; }
 
-    long long tokens_before = 0, pages_before = 0;      // of all requests of earlier rounds
+    long long tokens_before = 0, pages_before = 0;      // of all requests before them
     for (int base = 0; base < R; base += ST_THREADS) {
         const int r = base + tid;
         long long n = 0, need = 0;
@@ -65,13 +65,13 @@ step_tables_kernel(const int* cached, const int* counts, const int* held_in,
             if (need < 0) need = 0;
             if (h + need > W) { bad |= AIE_DEV_SLOT_OOB; fits = false; need = 0; }
         }
-        long long tok = n, pag = need;       // inclusive sums over this round's requests
+        long long tok = n, pag = need;       // inclusive sums over these requests
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const long long a = st_shfl_up(tok, o), b = st_shfl_up(pag, o);
             if (lane >= o) { tok += a; pag += b; }
         }
-        __syncthreads();          // the round before has read the warps' sums
+        __syncthreads();          // the pass before has read the warps' sums
         if (lane == 31) { w_tokens[warp] = tok; w_pages[warp] = pag; }
         __syncthreads();
         long long all_tok = 0, all_pag = 0;
