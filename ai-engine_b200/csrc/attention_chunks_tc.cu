@@ -30,9 +30,16 @@
 #define CT_M 128
 #define CT_KT 128
 #define CT_THREADS 384
-#define CT_BAR_P 1             // named barriers 1, 2: the probabilities of a step of stream 0 / 1 are in tensor memory
-#define CT_BAR_MEET 3          // 3, 4: the two streams of an item of few rows
+// named barriers: the probabilities of a step of stream t are in tensor memory.  Its steps take turns at two (t + 1 and t + 3): scores are asked
+// for behind the step before, so a warp that has seen those of a step knows that the barrier of the step before that is over.
+#define CT_BAR_P 1
+#define CT_BARS 2
+#define CT_BAR_MEET 5          // 5, 6: the two streams of an item of few rows
 #define CT_RESCALE_STEP 8.0f
+
+#ifndef CT_STRAY               // tile of values whose barrier waits for more bytes than come: for the test of a wait that runs out
+#define CT_STRAY (-1)
+#endif
 
 template <int D> struct CtShape {
     static constexpr int M = 2 * CT_M, KT = CT_KT;     // rows of an item, keys of a tile
@@ -53,6 +60,7 @@ template <int D>
 __global__ void __launch_bounds__(CT_THREADS, 1)
 chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const ChArgs a, int end_group) {
     using S = CtShape<D>;
+    static_assert(CT_BARS == 2, "whose turn it is is a bit a stream");
     constexpr int M = S::M, NS = S::NS, TILE = S::tile, HV = D / 64, GROUP = HV * 1024, PC = D / 8;
     extern __shared__ __align__(1024) unsigned char sm[];
     ChShared* sh = reinterpret_cast<ChShared*>(sm + S::walk_off);
@@ -156,7 +164,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                     const int p3 = page_of(j + 2), group = group_of(j, p1);
                     if (lane == 0 && ok) {
                         ok = mbar_wait(&empty[slot], (unsigned)ph, abort_flag, a.err);
-                        if (ok) mbar_expect_tx(&full[slot], TILE);
+                        if (ok) mbar_expect_tx(&full[slot], TILE + (values && j == CT_STRAY ? 16 : 0));
                     }
                     ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
                     if (!ok) break;
@@ -185,6 +193,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             const bool lead = tc_elect();
             bool ok = true;                 // that lane's; once false, the warp only keeps its appointments at the barriers
             int slot = 0, ph = 0, nq = 0;   // next tile of the ring, tiles of queries used so far
+            unsigned turn = 0;              // bit t: at which of its barriers stream t hands over next
             auto scores = [&](int t, int qs, int ks_) {
                 const unsigned long long dq = dq0 + (unsigned long long)((qs * TILE) >> 4), dk = dk0 + (unsigned long long)((ks_ * TILE) >> 4);
 #pragma unroll
@@ -259,7 +268,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                     for (int t = pair ? 0 : j & 1; t < 2; t += pair ? 1 : 2) {
                         // the softmax threads of a stream arrive, this warp waits: a hardware barrier, since an mbarrier test costs
                         // the issuing thread some hundred cycles while the tensor pipe reads shared memory
-                        asm volatile("bar.sync %0, %1;\n" ::"r"(CT_BAR_P + t), "r"(CT_M + 32) : "memory");
+                        asm volatile("bar.sync %0, %1;\n" ::"r"(CT_BAR_P + t + 2 * (turn >> t & 1)), "r"(CT_M + 32) : "memory");
+                        turn ^= 1u << t;
                         if (!lead || !ok) continue;
                         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                         outputs(t, sv, j < L);
@@ -331,7 +341,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             bool first = true;
             if (lane == 0) walks[warp] = w;
             for (int j = pair ? 0 : t; j < n; j += pair ? 1 : 2, first = false) {
-                // (a warp that gave up still arrives for every step: the issuing warp waits there without a limit)
+                // (a warp that gave up still comes to the barrier of every step: the issuing warp waits there without a limit)
                 if (ok) {
                     if (lane == 0) ok = mbar_wait(&s_full[t], s_ph, abort_flag, a.err);
                     ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
@@ -407,7 +417,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                     asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
                     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
                 }
-                asm volatile("bar.arrive %0, %1;\n" ::"r"(CT_BAR_P + t), "r"(CT_M + 32) : "memory");
+                tc_hand_over(CT_BAR_P + t + 2 * (s_ph ^ 1u), CT_M + 32, ok);
             }
             // the item's end
             __syncwarp();

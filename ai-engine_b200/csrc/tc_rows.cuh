@@ -3,6 +3,15 @@
 #pragma once
 #include "tc_common.cuh"
 
+// A softmax warp's hand-over of a step's probabilities at a named barrier that the issuing warp waits at (bar.sync, without a limit).
+// A warp that gave up (`ok` false) does not stand at s_full any more and could run ahead: it waits at the barrier too, so that each of
+// the warps counts once a step.  Before it gave up it may have arrived for steps that the issuing warp has not come to yet: a stream's
+// steps take turns at so many barriers that the last use of the one at hand is over by then.
+__device__ __forceinline__ void tc_hand_over(unsigned barrier, int threads, bool ok) {
+    if (ok) asm volatile("bar.arrive %0, %1;\n" ::"r"(barrier), "r"(threads) : "memory");
+    else asm volatile("bar.sync %0, %1;\n" ::"r"(barrier), "r"(threads) : "memory");
+}
+
 // shared-memory descriptor of an MN-major operand: rows of 64 elements (128 bytes) along MN,
 // groups of 8 K-rows `sbo` bytes apart, blocks of 64 MN elements `lbo` bytes apart
 __device__ __forceinline__ unsigned long long umma_desc_mn(const void* tile, unsigned lbo_bytes, unsigned sbo_bytes) {
