@@ -46,10 +46,10 @@
 // window of 1,024: 69 -> 45.
 // The value rows of keys past the sequence's last token are zeroed in shared memory before the
 // last tile's P . V, so a probability of 0 never meets what an unwritten cache slot holds.
-// The softmax warps hand a tile's probabilities to the issuing warp at a named hardware barrier (bar.arrive /
+// The softmax warps hand a tile's probabilities to the issuing warp at a named hardware barrier (tc_hand_over and
 // bar.sync); every mbarrier wait is bounded (see tc_common.cuh) and a wait that runs out raises the device error
-// word; a softmax warp whose wait ran out still arrives at the named barrier for every tile, so the issuing warp's
-// bar.sync always returns.
+// word; a softmax warp whose wait ran out still comes to the named barrier of every tile and waits there itself (tc_hand_over), so the
+// issuing warp's bar.sync always returns.
 // Formula: crates/ai-engine-runtime/src/arch/attention.rs:148-157,177-196,203-224.
 #include "tc_rows.cuh"
 
@@ -58,13 +58,17 @@
 #define AT_THREADS 192      // loader warp, MMA warp, 4 softmax warps
 #define AT_HALF_BYTES (128 * 64 * 2)      // one [128 x 64] bf16 swizzle atom column: 16 KB
 
-#define AT_BAR_P 1            // named barriers 1, 2: the probabilities of an even / odd key tile are in tensor memory
+// named barriers 1 .. 4: the probabilities of a key tile are in tensor memory.  The scores of tile j are asked for behind the barrier of tile
+// j - 2, so a warp that has seen those of tile j - 1 and gives up at tile j knows that the barrier of tile j - 3 is over: tiles have to take turns
+// at three barriers or more (at four the turn is two bits of j).
+#define AT_BAR_P 1
+#define AT_BARS 4
                               // (two, because a softmax warp may be a tile ahead of another: its arrival for
                               // tile j + 1 must not count for tile j)
 // columns of the probabilities of keys 16 ks .. 16 ks + 15 (the extended form's second terms lie 16 further)
 #define AT_P_COL(ext, ks) (unsigned)((ext) ? 32 * ((ks) >> 1) + 8 * ((ks) & 1) : 8 * (ks))
 #define AT_EXT_THREADS 320      // the extended form: 8 softmax warps, two threads a query row
-#define AT_BAR_ROW 3          // ... whose two warps of the same 32 rows meet at named barriers 3 .. 6
+#define AT_BAR_ROW 5          // ... whose two warps of the same 32 rows meet at named barriers 5 .. 8
 #define AT_RESCALE_STEP 8.0f     // a row's reference maximum moves in steps of more than this (log2 units)
 
 // HD: head size, HD / 64 halves of 64 columns.  A tile of 128 keys (or queries) holds 16 KB per half.
@@ -465,7 +469,7 @@ paged_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                 // reads shared memory, and this hand-over is on the tile's critical path (P . V, then the scores of the tile
                 // after the next, which the softmax warps wait for).  (The tile's values landed with its keys; in the extended
                 // form they have a barrier of their own, waited for above.)
-                asm volatile("bar.sync %0, %1;\n" ::"r"(AT_BAR_P + (j & 1)), "r"((EXT ? 2 : 1) * AT_M + 32) : "memory");
+                asm volatile("bar.sync %0, %1;\n" ::"r"(AT_BAR_P + (j & (AT_BARS - 1))), "r"((EXT ? 2 : 1) * AT_M + 32) : "memory");
                 st = st1;
                 ph = ph1;
                 if (!lead || !ok) continue;
@@ -565,7 +569,7 @@ paged_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                     asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
                     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
                 }
-                asm volatile("bar.arrive %0, %1;\n" ::"r"(AT_BAR_P + (j & 1)), "r"(2 * AT_M + 32) : "memory");
+                tc_hand_over(AT_BAR_P + (j & (AT_BARS - 1)), 2 * AT_M + 32, ok);
             }
             row_x[half][row] = l_run;
             asm volatile("bar.sync %0, 64;\n" ::"r"(AT_BAR_ROW + quarter) : "memory");
@@ -616,7 +620,7 @@ paged_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             float m_run = -INFINITY, l_run = 0.f;
             bool ok = true;
             for (int j = 0; j < n_kt; ++j) {
-                // (a warp that gave up still arrives at the barrier for every tile: the issuing warp waits there
+                // (a warp that gave up still comes to the barrier of every tile: the issuing warp waits there
                 // without a limit)
                 const unsigned tmem_s = tmem_base + (unsigned)((j & 1) * AT_N);
                 if (ok) {
@@ -624,7 +628,7 @@ paged_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                     ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
                 }
                 if (!ok) {
-                    asm volatile("bar.arrive %0, %1;\n" ::"r"(AT_BAR_P + (j & 1)), "r"(AT_M + 32) : "memory");
+                    tc_hand_over(AT_BAR_P + (j & (AT_BARS - 1)), AT_M + 32, false);
                     continue;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
@@ -662,7 +666,7 @@ paged_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                     if (lane == 0) ok = mbar_wait(o_done, (j - 1) & 1, abort_flag, err);
                     ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
                     if (!ok) {
-                        asm volatile("bar.arrive %0, %1;\n" ::"r"(AT_BAR_P + (j & 1)), "r"(AT_M + 32) : "memory");
+                        tc_hand_over(AT_BAR_P + (j & (AT_BARS - 1)), AT_M + 32, false);
                         continue;
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
@@ -701,7 +705,7 @@ paged_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                 l_run = l_run * corr + (at_lo(psum2) + at_hi(psum2));
                 asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-                asm volatile("bar.arrive %0, %1;\n" ::"r"(AT_BAR_P + (j & 1)), "r"(AT_M + 32) : "memory");
+                tc_hand_over(AT_BAR_P + (j & (AT_BARS - 1)), AT_M + 32, true);
             }
             // the last P . V, then this row of O divided by the row's sum
             if (ok) {
@@ -776,7 +780,10 @@ paged_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
 // (233 us), the row read by one x128 load (233 us), a part of the exponentials as polynomials (slower).
 // Tile B sees 128 more keys than tile A: A takes part in key tiles 0 .. nA - 1, B in all of the unit's.
 #define AT2_THREADS 384
-#define AT2_BAR_P 1         // named barriers 1, 2: the probabilities of tile A / B are in tensor memory
+// named barriers: the probabilities of tile A / B are in tensor memory.  Key tiles take turns at two each (1 and 3, 2 and 4): scores are asked
+// for behind the barrier of the key tile before.
+#define AT2_BAR_P 1
+#define AT2_BARS 2
 
 template <int HD> struct At2Smem {
     static constexpr int HV = HD / 64;
@@ -989,7 +996,7 @@ paged_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __
                 // the tile's probabilities are written: its 128 softmax threads arrive, this warp waits.  A
                 // hardware barrier: an mbarrier test costs the issuing thread some hundred cycles while the
                 // tensor pipe reads shared memory, and stood between every softmax and its products.
-                asm volatile("bar.sync %0, %1;\n" ::"r"(AT2_BAR_P + t), "r"(AT_M + 32) : "memory");
+                asm volatile("bar.sync %0, %1;\n" ::"r"(AT2_BAR_P + t + 2 * (j & (AT2_BARS - 1))), "r"(AT_M + 32) : "memory");
                 if (lane != 0 || !ok) continue;
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                 // P . V, then at once the next scores over the same columns (which the P . V has read: the
@@ -1026,14 +1033,14 @@ paged_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __
         float m_run = -INFINITY, l_run = 0.f;
         bool ok = true;
         for (int j = 0; j < n_t; ++j) {
-            // (a warp that gave up still arrives at the barrier for every tile: the issuing warp waits there
+            // (a warp that gave up still comes to the barrier of every tile: the issuing warp waits there
             // without a limit)
             if (ok) {
                 if (lane == 0) ok = mbar_wait(&s_full[t], (unsigned)(j & 1), abort_flag, err);
                 ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
             }
             if (!ok) {
-                asm volatile("bar.arrive %0, %1;\n" ::"r"(AT2_BAR_P + t), "r"(AT_M + 32) : "memory");
+                tc_hand_over(AT2_BAR_P + t + 2 * (j & (AT2_BARS - 1)), AT_M + 32, false);
                 continue;
             }
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
@@ -1101,7 +1108,7 @@ paged_prefill_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __
             l_run = l_run * corr + (at_lo(psum2) + at_hi(psum2));
             asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-            asm volatile("bar.arrive %0, %1;\n" ::"r"(AT2_BAR_P + t), "r"(AT_M + 32) : "memory");
+            tc_hand_over(AT2_BAR_P + t + 2 * (j & (AT2_BARS - 1)), AT_M + 32, true);
         }
         if (ok && n_t > 0) {
             if (lane == 0) ok = mbar_wait(&o_done[t], 0, abort_flag, err);

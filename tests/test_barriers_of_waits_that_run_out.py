@@ -75,7 +75,7 @@ def test_the_search_finds_what_is_wrong_with_arriving_without_waiting():
 
 
 # source, constant with the number of barriers that a stream's steps take turns at, how many steps ahead scores are announced
-KERNELS = [("attention_chunks_tc.cu", "CT_BARS", 1)]
+KERNELS = [("attention_chunks_tc.cu", "CT_BARS", 1), ("attention_prefill_tc.cu", "AT_BARS", 2), ("attention_prefill_tc.cu", "AT2_BARS", 1)]
 
 
 @pytest.mark.parametrize("name,constant,ahead", KERNELS)
