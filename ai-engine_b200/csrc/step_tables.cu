@@ -199,8 +199,16 @@ extern "C" int aie_step_tables(const StArgs* args, cudaStream_t stream) {
     const long long tb = ((long long)R * ((W + piece - 1) / piece) + warps - 1) / warps, kb = (capacity + ST_THREADS - 1) / ST_THREADS;
     const int table_blocks = (int)(tb < most ? tb : most), token_blocks = (int)(kb < most ? kb : most);
     auto kern = vec ? step_tables_kernel<true> : step_tables_kernel<false>;
+    // more than 48 KB with what the kernel has besides; told once on each device
+    static unsigned long long done[2] = {0, 0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev >= 64 || !(done[vec] >> dev & 1))) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ST_MAX_REQUESTS * (int)sizeof(StRow));
+        if (e == cudaSuccess && dev < 64) done[vec] |= 1ull << dev;
+    }
+    if (e != cudaSuccess) return (int)e;
     const size_t smem = (size_t)R * sizeof(StRow);
-    if (smem > 48 * 1024) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     return (int)launch_pdl(kern, dim3(table_blocks + token_blocks), dim3(ST_THREADS), smem, stream, a.cached, a.counts, a.held_in, a.tables_in,
                            a.free_pages, a.free_count, R, W, a.F, a.P, a.num_pages, capacity, table_blocks, a.out, held, free_left, q_start,
                            q_len, positions, token_req, slots, a.err);
