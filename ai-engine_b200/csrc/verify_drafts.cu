@@ -83,7 +83,7 @@ verify_drafts_kernel(const float* target, long long target_row, int T, int V, co
     __shared__ u64 seg_sum[VD_MAX_SEGMENTS];
     __shared__ u64 warp_sum[VD_THREADS / 32];
     __shared__ u64 sums[2][VD_CLUSTER];     // of every block: of w, of p alone
-    __shared__ int s_kept;
+    __shared__ int s_kept, s_token;         // drafts kept; the refused one's token, -1: all were kept, or it is outside the vocabulary
     cg::cluster_group cluster = cg::this_cluster();
     pdl_launch_dependents();
     pdl_wait();
@@ -116,7 +116,7 @@ verify_drafts_kernel(const float* target, long long target_row, int T, int V, co
 
     // how many drafts are kept: a warp looks at 32 places at a time
     if (warp == 0) {
-        int kept = n;
+        int kept = n, token = -1;
         for (int base = 0; base < n; base += 32) {
             const int i = base + lane;
             bool refused = false;
@@ -135,17 +135,25 @@ verify_drafts_kernel(const float* target, long long target_row, int T, int V, co
                 }
             }
             const unsigned any = __ballot_sync(0xffffffffu, refused);
-            if (any) { kept = base + __ffs(any) - 1; break; }
+            if (any) {
+                kept = base + __ffs(any) - 1;
+                token = __shfl_sync(0xffffffffu, x0, __ffs(any) - 1);
+                if (token >= V) token = -1;
+                break;
+            }
         }
-        if (lane == 0) s_kept = kept;
+        if (lane == 0) {
+            s_kept = kept;
+            s_token = token;
+        }
     }
     __syncthreads();
     const int kept = s_kept;
     const float* p = target + (start + kept) * target_row;
     VdMinus minus = {nullptr, -1};
-    if (kept < n) {
+    if (s_token >= 0) {                     // (a token outside the vocabulary came out of no distribution: nothing is taken off for it)
         if (draft_probs) minus.row = draft_probs + r * draft_req + kept * draft_place;
-        else minus.token = draft_tokens[(size_t)r * N + kept];
+        else minus.token = s_token;
     }
 
     const int segments = (V + VD_SEGMENT - 1) / VD_SEGMENT, per = (segments + VD_CLUSTER - 1) / VD_CLUSTER;
@@ -187,7 +195,7 @@ verify_drafts_kernel(const float* target, long long target_row, int T, int V, co
             fits = fits && a != VD_TOO_MUCH;
         }
         if (!fits) total = 0;
-        if (total > 0 || round == 1 || kept == n) break;      // the same in all blocks
+        if (total > 0 || round == 1 || s_token < 0) break;      // the same in all blocks
         minus.row = nullptr;
         minus.token = -1;
     }

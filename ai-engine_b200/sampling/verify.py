@@ -23,7 +23,8 @@ def verify_drafts(target_probs: torch.Tensor, q_start: torch.Tensor, draft_token
 
     Probabilities and draws are float32, draws in [0, 1); rows may be any distance apart.  Returns int32 tokens [R, N + 1] (the kept
     ones, the new one, -1) and emitted [R] = k + 1 (0 for an idle request): by how many tokens the request has grown.  Rows that are
-    not there (the request is left idle), a drafted token outside the vocabulary (refused) and a row without mass or with that of
+    not there (the request is left idle), a drafted token outside the vocabulary (refused, and the one
+    behind it comes from the target's whole row) and a row without mass or with that of
     thousands (token 0: logits, say, are no probabilities) set the error word."""
     return draft_call("verify_drafts", 1, _nb(token_draws) and _nb(token_draws) * target_probs.shape[-1], target_probs, q_start, draft_tokens, draft_len,
                       draft_probs, accept_draws, token_draws, err)
