@@ -30,7 +30,10 @@ typedef unsigned long long u64;
 #define VD_TOO_MUCH (~0ull)     // a sum that does not fit
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() {
+    __syncwarp();                           // .aligned: a warp's threads come together, which what stands before may not have left them
+    asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
+}
 
 // in units of 2^-48; NaN and what is negative weigh nothing
 __device__ __forceinline__ u64 vd_fixed(float w) { return w > 0.f ? __float2ull_rn(fminf(w, 1.f) * 281474976710656.f) : 0ull; }
