@@ -10,6 +10,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -159,8 +160,8 @@ template <typename F> PyObject* guarded(const char* name, Py_ssize_t got, Py_ssi
         return f();
     } catch (const Refused&) {           // the error is set
         return nullptr;
-    } catch (const std::exception& e) {      // torch's allocator
-        PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {                      // torch's own, as the exceptions that its operators raise (torch.OutOfMemoryError among them)
+        torch::translate_exception_to_python(std::current_exception());
         return nullptr;
     }
 }
