@@ -34,5 +34,5 @@ def step_tables(cached: torch.Tensor, counts: torch.Tensor, held: torch.Tensor, 
 
     A request whose lengths are negative, do not fit the table's width or bring tokens past max_tokens waits and sets the error
     word; a page outside the pool sets it too and makes no slot."""
-    return StepTables(*draft_call("step_tables", 1, 2 * _nb(tables), cached, counts, held, tables, free_pages, free_count, page_size,
+    return StepTables(*draft_call("step_tables", 2 * _nb(tables), cached, counts, held, tables, free_pages, free_count, page_size,
                                   num_pages, max_tokens, err))

@@ -22,6 +22,7 @@ namespace {
 PyObject* kernel_error = nullptr;       // exception types of kernels/loader.py
 PyObject* kernel_unavailable = nullptr;
 PyObject* load = nullptr;               // load(name): compiles and loads a launcher, and hands its address to set_launcher
+PyObject* launches = nullptr;           // kernels/loader.py::LAUNCHES, a list of one number
 
 struct Refused {};                      // the Python error is set
 
@@ -78,8 +79,13 @@ PyObject* part(const at::Tensor& base, int64_t offset, at::IntArrayRef shape) {
     impl->set_storage_offset(offset);
     return THPVariable_Wrap(at::Tensor(std::move(impl)));
 }
-void launched(const char* what, int rc) {
-    if (rc == 0) return;
+// a launcher has returned; `kernels` of ours were launched where that is no error
+void launched(const char* what, int rc, int kernels) {
+    if (rc == 0) {
+        PyObject* sum = PyLong_FromLongLong(PyLong_AsLongLong(PyList_GetItem(launches, 0)) + kernels);
+        if (!sum || PyList_SetItem(launches, 0, sum) < 0 || PyErr_Occurred()) throw Refused();
+        return;
+    }
     refuse(what, rc == -1   ? "bad argument (dtype or shape combination not accepted)"
                  : rc == -2 ? "size not supported by this kernel"
                  : rc == -3 ? "size beyond the kernel's stated maximum"
@@ -191,7 +197,7 @@ PyObject* step_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
         at::Tensor out = fresh({R * W + 3 * R + 1 + 3 * most}, at::kInt, tables);
         const StArgs args = {cached.data_ptr(), counts.data_ptr(), held.data_ptr(), tables.data_ptr(), free_pages.data_ptr(),
                              free_count.data_ptr(), out.data_ptr(), err.data_ptr(), (int)R, (int)W, (int)F, (int)P, (int)num_pages, (int)most};
-        launched(w, loaded(step_tables_fn, "aie_step_tables")(&args, st));
+        launched(w, loaded(step_tables_fn, "aie_step_tables")(&args, st), 1);
         PyObject* t = PyTuple_New(8);
         if (!t) throw Refused();
         int64_t at_ = R * W;
@@ -223,7 +229,7 @@ PyObject* write_kv_slots(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (T) {
             const CwArgs args = {k.data_ptr(), v.data_ptr(), kp.data_ptr(), vp.data_ptr(), slots.data_ptr(), err.data_ptr(),
                                  k.stride(0), k.stride(1), v.stride(0), v.stride(1), code, p.code, (int)T, (int)p.N, (int)p.P, (int)p.K, (int)p.d};
-            launched(w, loaded(write_fn, "aie_write_kv_slots")(&args, st));
+            launched(w, loaded(write_fn, "aie_write_kv_slots")(&args, st), 1);
         }
         Py_RETURN_NONE;
     });
@@ -260,7 +266,7 @@ PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                  guess ? guess->data_ptr() : nullptr, accept.data_ptr(), pick.data_ptr(), tokens.data_ptr(), emitted.data_ptr(),
                                  err.data_ptr(), target.stride(0), guess ? guess->stride(0) : 0, guess ? guess->stride(1) : 0,
                                  (int)T, (int)V, (int)R, (int)N};
-            launched(w, loaded(verify_fn, "aie_verify_drafts")(&args, st));
+            launched(w, loaded(verify_fn, "aie_verify_drafts")(&args, st), 1);
         }
         PyObject* t = PyTuple_New(2);
         if (!t) throw Refused();
@@ -365,17 +371,19 @@ PyObject* paged_attention_chunks(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                  (int)p.N, (int)p.P, (int)H, (int)p.K, (int)G, (int)p.d, (int)window, (float)(scale * 1.4426950408889634), err.data_ptr()};
             launched(w, form == TCGEN05   ? loaded(chunks_tc_fn, "aie_attention_chunks_tc")(&call, st)
                         : form == FLOAT32 ? loaded(chunks_f32_fn, "aie_attention_chunks_f32")(&call, p.code, st)
-                                          : loaded(chunks_mma_fn, "aie_attention_chunks_bf16")(&call, (int)form - MMA, st));
+                                          : loaded(chunks_mma_fn, "aie_attention_chunks_bf16")(&call, (int)form - MMA, st),
+                     form > MMA ? 1 : 2);      // clusters join their parts themselves
         }
         return THPVariable_Wrap(std::move(out));
     });
 }
 
 PyObject* set_up(PyObject*, PyObject* args) {
-    if (!PyArg_ParseTuple(args, "OOO", &kernel_error, &kernel_unavailable, &load)) return nullptr;
+    if (!PyArg_ParseTuple(args, "OOOO!", &kernel_error, &kernel_unavailable, &load, &PyList_Type, &launches)) return nullptr;
     Py_INCREF(kernel_error);
     Py_INCREF(kernel_unavailable);
     Py_INCREF(load);
+    Py_INCREF(launches);
     Py_RETURN_NONE;
 }
 PyObject* set_launcher(PyObject*, PyObject* args) {
@@ -396,7 +404,7 @@ PyObject* set_launcher(PyObject*, PyObject* args) {
 }
 
 PyMethodDef methods[] = {
-    {"set_up", set_up, METH_VARARGS, "exception types (KernelError, KernelUnavailable), load(name)"},
+    {"set_up", set_up, METH_VARARGS, "exception types (KernelError, KernelUnavailable), load(name), the list that counts launches"},
     {"set_launcher", set_launcher, METH_VARARGS, "name of a launcher, its address"},
     {"step_tables", (PyCFunction)(void (*)(void))step_tables, METH_FASTCALL, nullptr},
     {"write_kv_slots", (PyCFunction)(void (*)(void))write_kv_slots, METH_FASTCALL, nullptr},

@@ -737,21 +737,19 @@ def draft_ops():
         def load(name: str) -> None:
             mod.set_launcher(name, cast_pointer(getattr(library(_DRAFT_SOURCES[name]), name), c_void_p).value)
 
-        mod.set_up(KernelError, KernelUnavailable, load)
+        mod.set_up(KernelError, KernelUnavailable, load, LAUNCHES)
         _DRAFT[0] = mod
     return _DRAFT[0]
 
 
-def draft_call(name: str, launches: int, cost: float, *args):
-    """One call of an operator of csrc/host/draft_ops.cpp; `cost`: bytes that it has to move, for the timers."""
+def draft_call(name: str, cost: float, *args):
+    """One call of an operator of csrc/host/draft_ops.cpp, which counts its launches; `cost`: bytes that it has to move, for the timers (0 where
+    only the device knows)."""
     fn = getattr(_DRAFT[0] or draft_ops(), name)
     if _profiling():
         with region(name, cost):
-            r = fn(*args)
-    else:
-        r = fn(*args)
-    LAUNCHES[0] += launches
-    return r
+            return fn(*args)
+    return fn(*args)
 
 
 def write_kv_slots(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor,
@@ -760,7 +758,7 @@ def write_kv_slots(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     [pages, K, P, d], at the slots that `cache.step_tables` made.  k, v: [T, K, d] float32 or bfloat16, each with any distance between
     tokens and between heads (columns of a fused projection); rounded once where the pool holds fewer bits.  A negative slot
     leaves its row out; one past the pool is left out and sets the error word.  Slots that are named must differ."""
-    draft_call("write_kv_slots", 1, _nb(k, v), k, v, k_pages, v_pages, slots, err)
+    draft_call("write_kv_slots", _nb(k, v), k, v, k_pages, v_pages, slots, err)
 
 
 CHUNK_FORM = -1      # the form that attention of new tokens takes (csrc/host/draft_ops.cpp: chunk_form); -1: by the sizes
@@ -778,7 +776,7 @@ def paged_attention_chunks(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     shared out over the whole machine.  Any head size up to 256 that is a multiple of 8.  Lengths that do not fit q or the table bring nothing and set the error word, so
     does a page outside the pool, whose keys count as zeros.  How a token's sums are ordered depends on the whole batch's lengths; a
     non-finite key or value reaches all of its request's tokens in the step."""
-    return draft_call("paged_attention_chunks", 2, 2 * _nb(q), q, k_pages, v_pages, q_start, q_len, ctx_len, block_table, scale, window,
+    return draft_call("paged_attention_chunks", 0.0, q, k_pages, v_pages, q_start, q_len, ctx_len, block_table, scale, window,
                       err, out, CHUNK_FORM)
 
 

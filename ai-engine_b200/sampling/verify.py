@@ -26,5 +26,5 @@ def verify_drafts(target_probs: torch.Tensor, q_start: torch.Tensor, draft_token
     not there (the request is left idle), a drafted token outside the vocabulary (refused, and the one
     behind it comes from the target's whole row) and a row without mass or with that of
     thousands (token 0: logits, say, are no probabilities) set the error word."""
-    return draft_call("verify_drafts", 1, _nb(token_draws) and _nb(token_draws) * target_probs.shape[-1], target_probs, q_start, draft_tokens, draft_len,
+    return draft_call("verify_drafts", _nb(token_draws) and _nb(token_draws) * target_probs.shape[-1], target_probs, q_start, draft_tokens, draft_len,
                       draft_probs, accept_draws, token_draws, err)
