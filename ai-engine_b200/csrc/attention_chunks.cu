@@ -52,6 +52,11 @@ __device__ __forceinline__ void cb_ldsm(unsigned (&r)[4], unsigned p) {
 __device__ __forceinline__ void cb_ldsm_t(unsigned (&r)[4], unsigned p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p));
 }
+__device__ __forceinline__ unsigned cb_load(unsigned p) {
+    unsigned v;
+    asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(v) : "r"(p) : "memory");
+    return v;
+}
 __device__ __forceinline__ void cb_mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -65,6 +70,18 @@ __device__ __forceinline__ float cb_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// whether any of `STAGE / 2` elements at `p` is not finite, for a whole warp
+template <int STAGE> __device__ __forceinline__ bool cb_unfinite(unsigned p, int lane) {
+    unsigned m[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < STAGE / 512; ++i) {
+        unsigned v[4];
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(p + (i * 32 + lane) * 16) : "memory");
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m[e] = ch_larger(m[e], v[e]);
+    }
+    return __any_sync(0xffffffffu, ch_unfinite(ch_larger(ch_larger(m[0], m[1]), ch_larger(m[2], m[3]))) != 0);
 }
 // byte offset of row r, 16-byte piece c of rows of D elements: pieces are permuted so that eight rows' pieces lie in different banks
 template <int D> __device__ __forceinline__ unsigned cb_at(int row, int piece) { return (unsigned)(row * (D * 2) + ((piece ^ (row & 7)) << 4)); }
@@ -184,6 +201,7 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
             slot = slot + 1 == NST ? 0 : slot + 1;
             const int k_at = (kt0 + i) * KT + group * CK;
             if (k_at >= hi || !live) continue;
+            const bool edge = k_at + CK - 1 > c0 + tl.i0 || k_at < last_low;      // some rows do not see some of these keys
             float s[CK / 8][4];
 #pragma unroll
             for (int x = 0; x < CK / 8; ++x)
@@ -207,7 +225,7 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[x][e] *= a.scale2;
             }
-            if (k_at + CK - 1 > c0 + tl.i0 || k_at < last_low) {
+            if (edge) {
 #pragma unroll
                 for (int x = 0; x < CK / 8; ++x)
 #pragma unroll
@@ -215,6 +233,32 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
                         const int key = k_at + x * 8 + col + (e & 1), q = e < 2 ? pos0 : pos1;
                         if (key > q || (a.window > 0 && key <= q - a.window)) s[x][e] = -INFINITY;
                     }
+                if (__builtin_expect(cb_unfinite<S::stage>(vs, lane), 0)) {
+#pragma unroll 1
+                    for (int kk = 0; kk < CK; ++kk) {
+                        const bool sees0 = ch_sees(pos0, k_at + kk, a.window), sees1 = ch_sees(pos1, k_at + kk, a.window);
+#pragma unroll
+                        for (int x = 0; x < D / 8; ++x) {
+                            const unsigned v = cb_load(vs + cb_at<D>(kk, x) + col * 2), u = ch_unfinite(v);
+                            const float v0 = __uint_as_float(v << 16), v1 = __uint_as_float(v & 0xffff0000u);
+                            if (sees0 && (u & 0x8000u)) o[x][0] += v0;
+                            if (sees0 && (u >> 31)) o[x][1] += v1;
+                            if (sees1 && (u & 0x8000u)) o[x][2] += v0;
+                            if (sees1 && (u >> 31)) o[x][3] += v1;
+                        }
+                    }
+                    // all warps that read the stage have added them: now they are taken out of it
+                    const bool both = tl.rows > 16;
+                    if (both) asm volatile("bar.sync %0, %1;\n" ::"r"(1 + group), "n"(32 * GW) : "memory");
+                    else __syncwarp();
+#pragma unroll 1
+                    for (int i = lane; i < CK * D / 2; i += 32) {
+                        const unsigned v = cb_load(vs + i * 4);
+                        asm volatile("st.shared.u32 [%0], %1;\n" ::"r"(vs + i * 4), "r"(ch_without(v, ch_unfinite(v))) : "memory");
+                    }
+                    if (both) asm volatile("bar.sync %0, %1;\n" ::"r"(1 + group), "n"(32 * GW) : "memory");
+                    else __syncwarp();
+                }
             }
             float top[2] = {-INFINITY, -INFINITY}, corr[2] = {1.f, 1.f}, use[2];
 #pragma unroll
@@ -228,7 +272,7 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
             for (int e = 0; e < 2; ++e) {
                 top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2)) * sl2;
                 if (top[e] > m_run[e] + CB_RESCALE_STEP) {
-                    corr[e] = m_run[e] == -INFINITY ? 0.f : cb_exp2(m_run[e] - top[e]);
+                    corr[e] = m_run[e] == -INFINITY ? 1.f : cb_exp2(m_run[e] - top[e]);      // (1: all is 0 yet, but for infinite values)
                     m_run[e] = top[e];
                 }
                 use[e] = m_run[e] == -INFINITY ? 0.f : m_run[e];
@@ -275,7 +319,7 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
             float l = l_run[e];
             l += __shfl_xor_sync(0xffffffffu, l, 1);
             l += __shfl_xor_sync(0xffffffffu, l, 2);
-            if ((lane & 3) == 0) *reinterpret_cast<float2*>(ml + (group * M + row) * 2) = make_float2(m_run[e], l);
+            if ((lane & 3) == 0) *reinterpret_cast<float2*>(ml + (group * M + row) * 2) = ch_left(m_run[e], l);
             if (row < place_in_line.tile.rows)
 #pragma unroll
                 for (int x = 0; x < D / 8; ++x)
@@ -304,7 +348,7 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
             }
             if constexpr (CLUSTER) {              // for the other blocks, where group 0's outputs were (this thread's alone to read)
                 *reinterpret_cast<float4*>(o_s + row * D + (e ^ ((row & 3) << 3))) = y;
-                if (e == 0) *reinterpret_cast<float2*>(cb_smem + S::block_ml_off + row * 8) = make_float2(m, l);
+                if (e == 0) *reinterpret_cast<float2*>(cb_smem + S::block_ml_off + row * 8) = ch_left(m, l);
             } else if (begins && ends) {
                 const float inv = ch_inverse(l);
                 const int full = w.tile.row0 + row, t = ch_over(full, a.by_g), h = w.kh * a.G + full - t * a.G;
@@ -312,7 +356,7 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
                              make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
             } else {
                 *reinterpret_cast<float4*>(a.part_o + (place * M + row) * D + e) = y;
-                if (e == 0) *reinterpret_cast<float2*>(a.part_ml + (place * M + row) * 2) = make_float2(m, l);
+                if (e == 0) *reinterpret_cast<float2*>(a.part_ml + (place * M + row) * 2) = ch_left(m, l);
             }
         }
         if constexpr (CLUSTER) {

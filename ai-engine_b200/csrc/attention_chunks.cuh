@@ -218,6 +218,23 @@ template <typename Sh> __device__ __forceinline__ bool ch_next(const ChArgs& a, 
     w.left -= n * Sh::weight(w.tile.rows);
     return w.left > 0 && ch_item<Sh>(a, w);
 }
+// A value that is not finite belongs to the rows that see its key and to no others, but a probability of 0 times it is NaN.  Where every row of an
+// item sees every key of a step that is as it should be; on the other steps, which touch the diagonal or a window's edge, the kernels take
+// such values out of the product and add them to the outputs of the rows that see them (whatever the weight: it is above 0).
+__device__ __forceinline__ bool ch_sees(int pos, int key, int window) { return key <= pos && (window <= 0 || key > pos - window); }
+// of two pairs of bfloat16, each the one that is larger in size, NaN where one of them is (the sign means nothing)
+__device__ __forceinline__ unsigned ch_larger(unsigned a, unsigned b) {
+    unsigned r;
+    asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// two bfloat16: bits 15 and 31 where the lower, the upper one is not finite
+__device__ __forceinline__ unsigned ch_unfinite(unsigned v) { return ((v & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
+__device__ __forceinline__ unsigned ch_without(unsigned v, unsigned unfinite) { return v & ~((unfinite >> 15) * 0xffffu); }
+
+// A row's maximum for those who join its parts: maxima pass over what is not a number, a sum that is none has to come along.
+__device__ __forceinline__ float2 ch_left(float m, float l) { return make_float2(l == l ? m : l, l); }
+
 // What the joining kernel has to know of the item that block c begins here and does not finish.
 template <typename Sh> __device__ __forceinline__ void ch_leave(const ChArgs& a, const ChWalk& w, int c) {
     const int last = (w.tile.tiles - 1) * Sh::weight(w.tile.rows);      // where its last tile begins, from the item's beginning
