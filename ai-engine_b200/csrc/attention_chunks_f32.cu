@@ -30,6 +30,11 @@ __device__ __forceinline__ float cf_exp2(float x) {      // 2^-22 relative; belo
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float cf_larger(float a, float b) {      // in size; NaN where one of them is (the sign means nothing)
+    float r;
+    asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 __device__ __forceinline__ u64 cf_pack(float lo, float hi) {
     u64 r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
@@ -145,7 +150,7 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
 
         const bool live = mt * 8 < rows;          // any row of this warp
         float m_run[4], l_run[4];                 // of rows 8 mt + 4 rq + r
-        int lim[4];                               // last key that a row sees, -1 for a row that is not there
+        int lim[4];                               // last key that a row sees (a row that is not there: the last one's)
         u64 o[2][2][CL];                          // rows 8 mt + 4 j + 2 e and the next, columns CL lane .. (128 further from the fifth on)
         const int reach = a.window > 0 ? a.window : 0x7fffffff;
 #pragma unroll
@@ -153,7 +158,7 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
             m_run[r] = -INFINITY;
             l_run[r] = 0.f;
             const int row = mt * 8 + rq * 4 + r;
-            lim[r] = row < rows ? c0 + ch_over(row0 + row, a.by_g) : -1;
+            lim[r] = c0 + ch_over(row0 + min(row, rows - 1), a.by_g);
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -213,8 +218,13 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
             }
             const int at = k_at + key;
             float top[4], corr[4];
+            bool edge = false;                    // some rows do not see some of these keys
 #pragma unroll
-            for (int r = 0; r < 4; ++r) top[r] = x[r] = at <= lim[r] && lim[r] - at < reach ? x[r] * a.scale2 : -INFINITY;
+            for (int r = 0; r < 4; ++r) {
+                const bool sees = at <= lim[r] && lim[r] - at < reach;
+                top[r] = x[r] = sees ? x[r] * a.scale2 : -INFINITY;
+                edge = edge || !sees;
+            }
 #pragma unroll
             for (int b = 0; b < 4; ++b)
 #pragma unroll
@@ -245,9 +255,7 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
                     }
             }
             __syncwarp();
-#pragma unroll 4
-            for (int kk = 0; kk < 16; ++kk) {
-                float v[CL];
+            auto values = [&](float (&v)[CL], int kk) {      // this lane's columns of key kk
                 if constexpr (CL == 2) {
                     const float2 t = *reinterpret_cast<const float2*>(vs + kk * D + lane * 2);
                     v[0] = t.x, v[1] = t.y;
@@ -258,6 +266,8 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
                         v[4 * y] = t.x, v[4 * y + 1] = t.y, v[4 * y + 2] = t.z, v[4 * y + 3] = t.w;
                     }
                 }
+            };
+            auto product = [&](const float (&v)[CL], int kk) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const ulonglong2 p2 = *reinterpret_cast<const ulonglong2*>(p_s + kk * S::PS + j * 4);
@@ -266,6 +276,45 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
                         const u64 vv = cf_pack(v[y], v[y]);
                         o[j][0][y] = cf_fma2(p2.x, vv, o[j][0][y]);
                         o[j][1][y] = cf_fma2(p2.y, vv, o[j][1][y]);
+                    }
+                }
+            };
+            float v[CL];
+            bool unfinite = false;
+            if (__any_sync(0xffffffffu, edge)) {
+                float most = 0.f;
+#pragma unroll 4
+                for (int kk = 0; kk < 16; ++kk) {
+                    values(v, kk);
+#pragma unroll
+                    for (int y = 0; y < CL; ++y) most = cf_larger(most, v[y]);
+                }
+                unfinite = __any_sync(0xffffffffu, !isfinite(most));
+            }
+            if (__builtin_expect(!unfinite, 1)) {
+#pragma unroll 4
+                for (int kk = 0; kk < 16; ++kk) {
+                    values(v, kk);
+                    product(v, kk);
+                }
+            } else {
+#pragma unroll 1
+                for (int kk = 0; kk < 16; ++kk) {
+                    values(v, kk);
+                    float some[CL];
+#pragma unroll
+                    for (int y = 0; y < CL; ++y) some[y] = isfinite(v[y]) ? v[y] : 0.f;
+                    product(some, kk);
+#pragma unroll
+                    for (int row = 0; row < 8; ++row) {
+                        const int pos = place_in_line.req.c + ch_over(place_in_line.tile.row0 + mt * 8 + row, a.by_g);
+                        if (!ch_sees(pos, k_at + kk, a.window)) continue;
+#pragma unroll
+                        for (int y = 0; y < CL; ++y) {
+                            float2 t = cf_both(o[row >> 2][(row & 3) >> 1][y]);
+                            if (!isfinite(v[y])) (row & 1 ? t.y : t.x) += v[y];
+                            o[row >> 2][(row & 3) >> 1][y] = cf_pack(t.x, t.y);
+                        }
                     }
                 }
             }
@@ -279,7 +328,7 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
             float l = l_run[r];
 #pragma unroll
             for (int b = 0; b < 4; ++b) l += __shfl_xor_sync(0xffffffffu, l, b < 2 ? 1 << b : 2 << b);
-            if (key == 0) *reinterpret_cast<float2*>(ml + (group * M + mt * 8 + rq * 4 + r) * 2) = make_float2(m_run[r], l);
+            if (key == 0) *reinterpret_cast<float2*>(ml + (group * M + mt * 8 + rq * 4 + r) * 2) = ch_left(m_run[r], l);
         }
         __syncthreads();
         w = place_in_line;
@@ -330,7 +379,7 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
                               make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
             } else {
                 *reinterpret_cast<float4*>(a.part_o + (place * M + row) * D + e) = y;
-                if (e == 0) *reinterpret_cast<float2*>(a.part_ml + (place * M + row) * 2) = make_float2(m, l);
+                if (e == 0) *reinterpret_cast<float2*>(a.part_ml + (place * M + row) * 2) = ch_left(m, l);
             }
         }
         if (begins && !ends && tid == 0) ch_leave<S>(a, w, c);

@@ -9,7 +9,8 @@ from test_attention_chunks_gpu import call
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
 INF, NAN = float("inf"), float("nan")
-FORMS = [pytest.param((16, BF16), id="mma"), pytest.param((18, BF16), id="clusters of 2"), pytest.param((20, BF16), id="clusters of 4"), pytest.param((24, BF16), id="clusters of 8")]
+FORMS = [pytest.param((-1, F32), id="float32"), pytest.param((0, BF16), id="float32 of bfloat16 pools"), pytest.param((16, BF16), id="mma"),
+         pytest.param((18, BF16), id="clusters of 2"), pytest.param((20, BF16), id="clusters of 4"), pytest.param((24, BF16), id="clusters of 8")]
 
 
 @pytest.fixture(params=FORMS)
@@ -96,6 +97,19 @@ def test_values_that_some_tokens_have_passed(dtype, window, cached, new):
             if key >= 0:
                 poison(b, "v", r, key, head, [column], INF)
         poison(b, "k", r, max(0, c - window), 1, [0], NAN)
+    check(b, dtype)
+
+
+@pytest.mark.parametrize("d", [8, 96, 200, 256])
+def test_other_head_sizes(dtype, d):
+    if dtype == BF16:
+        from ai_engine_b200.kernels import ops
+        if ops.CHUNK_FORM != 0:
+            pytest.skip("a form of heads of 64 and 128")
+    b = paged_batch([130, 3], [9, 40], 6, 2, d, 16, dtype, d)
+    for r, (c, n) in enumerate(zip(b["cached"], b["new"])):
+        poison(b, "v", r, c + n - 1, 0, [0, d - 1], -INF)
+        poison(b, "v", r, c + 4, 1, [d // 2], NAN)
     check(b, dtype)
 
 
