@@ -15,7 +15,7 @@
 //                    the tile's bytes take at heads of 64.)
 //   warp 9           issues the products: S = Q K^T and O += P V of a step of a stream, P from tensor memory, V as the MN-major
 //                    operand; zeroes the values past a request's last key, since a probability of 0 must not meet what an unwritten slot
-//                    holds;
+//                    holds, and what is not finite among those of keys that some rows do not see;
 //   warp 11          queries: rows = (token, head of the group) gathered by cp.async into the swizzled tile that TMA would write (tokens
 //                    and heads may lie any distance apart), ahead of the item that uses them where a place is free.
 // Tensor memory: scores of stream t at columns 128 t (P over the first 64), outputs at 256 + 128 t.
@@ -53,6 +53,36 @@ template <int D> struct CtShape {
     static constexpr int walk_off = 256, warps_off = 480, meet_off = 1024, q_off = 3 * 1024, kv_off = q_off + 2 * tile, bytes = kv_off + NS * tile;
 };
 
+// Adds to 32 columns of a row's outputs, from column c0 on, what is not finite among the values that the row sees of keys that not all of the
+// item's rows see, in this block's share (n tiles from w.k on); they are read out of the pages again.
+__device__ __forceinline__ void ct_add_unfinite(const ChArgs& a, const ChWalk& w, int n, int pos, int c0, unsigned (&ov)[32]) {
+    const int first_pos = w.req.c + w.tile.i0, last_low = a.window > 0 ? w.req.c + w.tile.i1 - a.window + 1 : 0;
+    const int k0 = (w.tile.first + w.k) * CT_KT, k1 = min(k0 + n * CT_KT, pos + 1);
+#pragma unroll 1
+    for (int key = k0; key < k1; ++key) {
+        if (key >= last_low && key <= first_pos) {      // on to the keys that the first row does not see
+            key = first_pos;
+            continue;
+        }
+        const int in = ch_over(key, a.by_p), page = ch_sees(pos, key, a.window) ? a.table[(size_t)w.r * a.W + in] : -1;
+        if (page < 0 || page >= a.num_pages) continue;
+        const uint4* row = reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.v_pages) +
+                                                          (((size_t)page * a.K + w.kh) * a.P + (key - in * a.P)) * a.d + c0);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const uint4 v4 = row[x];
+            const unsigned v[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned u = ch_unfinite(v[e]);
+                const int i = x * 8 + e * 2;
+                if (u & 0x8000u) ov[i] = __float_as_uint(__uint_as_float(ov[i]) + __uint_as_float(v[e] << 16));
+                if (u >> 31) ov[i + 1] = __float_as_uint(__uint_as_float(ov[i + 1]) + __uint_as_float(v[e] & 0xffff0000u));
+            }
+        }
+    }
+}
+
 // The order in which an item's tiles of keys (K) and values (V) pass through the ring: `ahead` tiles of keys, then V(j), K(j + ahead).
 __device__ __forceinline__ int ct_ahead(const ChTile& t) { return t.rows > CT_M ? 1 : 2; }
 
@@ -75,6 +105,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     unsigned long long* o_done = s_full + 2;        // [2] the last product of an item's stream is done
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(o_done + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    unsigned* unfinite = tmem_slot + 6;             // not 0: on some step of this block that not all rows see wholly, a value was not finite
     unsigned* armed = tmem_slot + 2;                // [2][2] tiles of the ring that the loaders asked for last, and of what phase (a bit each)
     unsigned char* q_s = sm + S::q_off;
     unsigned char* kv_s = sm + S::kv_off;
@@ -95,6 +126,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             mbar_init(&o_done[t], 1);
         }
         *abort_flag = 0;
+        *unfinite = 0u;
         for (int i = 0; i < 4; ++i) armed[i] = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
@@ -219,6 +251,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                 const int n = ch_share<S>(w), L = ct_ahead(w.tile);
                 const bool pair = L == 1, ends = w.k + n == w.tile.tiles;
                 const int past = w.req.c + w.tile.i1 + 1 - (w.tile.first + w.tile.tiles - 1) * CT_KT;      // keys of the item's last tile
+                const int first_pos = w.req.c + w.tile.i0, last_low = a.window > 0 ? w.req.c + w.tile.i1 - a.window + 1 : 0;
+                const int kt0 = w.tile.first + w.k;
                 const int q0 = nq & 1, q1 = pair ? q0 ^ 1 : q0, qp0 = (nq >> 1) & 1, qp1 = ((nq + 1) >> 1) & 1;
                 if (lead && ok) {
                     ok = mbar_wait(&q_full[q0], (unsigned)qp0, abort_flag, a.err);
@@ -253,13 +287,36 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                         ok = mbar_wait(&full[sv], (unsigned)pv, abort_flag, a.err);
                         if (ok && more) ok = mbar_wait(&full[sk], (unsigned)pk, abort_flag, a.err);
                     }
-                    if (ends && j == n - 1 && past < CT_KT) {
-                        const unsigned all = __ballot_sync(0xffffffffu, lead && ok);
-                        if (all) {
-                            for (int i = lane; i < (CT_KT - past) * PC; i += 32) {
-                                const int row = past + i / PC, x = i % PC;
-                                *reinterpret_cast<uint4*>(kv_s + sv * TILE + (row >> 3) * GROUP + (x >> 3) * 1024 + (row & 7) * 128 + (x & 7) * 16) =
-                                    make_uint4(0, 0, 0, 0);
+                    const int kbase = (kt0 + j) * CT_KT;
+                    if (kbase + CT_KT - 1 > first_pos || kbase < last_low) {
+                        // the keys past the request's end get zeros for values, and so does what is not finite among those of keys that
+                        // some rows do not see: a probability of 0 must not meet it (the softmax warps add it to the rows that see it)
+                        if (__ballot_sync(0xffffffffu, lead && ok)) {
+                            const int keys = ends && j == n - 1 ? min(past, CT_KT) : CT_KT;
+                            const int upto = max(0, min(last_low - kbase, keys)), from = max(upto, min(first_pos + 1 - kbase, keys));
+                            auto piece = [&](int row) {      // of this lane, which looks at every 32 / PC-th row
+                                const int x = lane % PC;
+                                return reinterpret_cast<uint4*>(kv_s + sv * TILE + (row >> 3) * GROUP + (x >> 3) * 1024 + (row & 7) * 128 + (x & 7) * 16);
+                            };
+                            unsigned most = 0u;
+#pragma unroll 1
+                            for (int half = 0; half < 2; ++half)      // the first keys, the last ones
+                                for (int row = (half ? from : 0) + lane / PC; row < (half ? keys : upto); row += 32 / PC) {
+                                    const uint4 v = *piece(row);
+                                    most = ch_larger(most, ch_larger(ch_larger(v.x, v.y), ch_larger(v.z, v.w)));
+                                }
+                            for (int row = keys + lane / PC; row < CT_KT; row += 32 / PC) *piece(row) = make_uint4(0, 0, 0, 0);
+                            if (__any_sync(0xffffffffu, ch_unfinite(most) != 0)) {
+#pragma unroll 1
+                                for (int half = 0; half < 2; ++half)
+#pragma unroll 1
+                                    for (int row = (half ? from : 0) + lane / PC; row < (half ? keys : upto); row += 32 / PC) {
+                                        const uint4 v = *piece(row);
+                                        *piece(row) = make_uint4(ch_without(v.x, ch_unfinite(v.x)), ch_without(v.y, ch_unfinite(v.y)),
+                                                                 ch_without(v.z, ch_unfinite(v.z)), ch_without(v.w, ch_unfinite(v.w)));
+                                    }
+                                if (lane == 0) atomicOr(unfinite, 1u);
+                                __threadfence_block();
                             }
                             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                         }
@@ -435,6 +492,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             const size_t place = ((size_t)2 * c + (begins ? 1 : 0)) * M + at;
             bf16* dst = reinterpret_cast<bf16*>(a.out) + ((size_t)(w.s0 + tok) * a.H + h) * D;
             float f0 = 1.f, f1 = 0.f;                                  // of this stream's outputs, of the other's
+            m_run = ch_left(m_run, l_run).x;
             if (!pair) {
                 // both streams have read the same rows: each puts together half of the columns
                 meet[t][row] = make_float2(m_run, l_run);
@@ -442,12 +500,14 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                 asm volatile("bar.sync %0, %1;\n" ::"r"(CT_BAR_MEET), "r"(2 * CT_M) : "memory");
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
                 const float2 y = meet[t ^ 1][row];
-                const float m = fmaxf(m_run, y.x);
+                const float m = l_run == l_run && y.y == y.y ? fmaxf(m_run, y.x) : NAN;
                 f0 = m_run == -INFINITY ? 0.f : exp2f(m_run - m);
                 f1 = y.x == -INFINITY ? 0.f : exp2f(y.x - m);
                 l_run = f0 * l_run + f1 * y.y;
                 m_run = m;
             }
+            // (set before the products whose end was waited for, by this stream or by the one that it met)
+            const bool some_unfinite = *reinterpret_cast<volatile unsigned*>(unfinite) != 0u;
             if (live && ok) {
                 const float inv = whole ? ch_inverse(l_run) : 1.f;
                 f0 *= inv;
@@ -469,6 +529,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                             for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) + __uint_as_float(ow[i]) * f1);
                         }
                     }
+                    if (__builtin_expect(some_unfinite, 0) && there) ct_add_unfinite(a, w, n, w.req.c + tok, c0, ov);
                     if (there && whole) {
 #pragma unroll
                         for (int i = 0; i < 32; i += 8) {

@@ -774,8 +774,8 @@ def paged_attention_chunks(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     bytes); block_table [R, W]; out [T, H, d] contiguous: rows that no request names are left as they are (in an `out` made
     here they hold nothing), rows that several name hold one's; it may be q itself, else it overlaps no operand.  Few tokens behind many keys are what it is made for: the keys are
     shared out over the whole machine.  Any head size up to 256 that is a multiple of 8.  Lengths that do not fit q or the table bring nothing and set the error word, so
-    does a page outside the pool, whose keys count as zeros.  How a token's sums are ordered depends on the whole batch's lengths; a
-    non-finite key or value reaches all of its request's tokens in the step."""
+    does a page outside the pool, whose keys count as zeros.  How a token's sums are ordered depends on the whole batch's lengths; keys
+    and values that are not finite reach the tokens that see them and no others."""
     return draft_call("paged_attention_chunks", 0.0, q, k_pages, v_pages, q_start, q_len, ctx_len, block_table, scale, window,
                       err, out, CHUNK_FORM)
 

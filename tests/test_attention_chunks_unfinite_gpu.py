@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
 INF, NAN = float("inf"), float("nan")
 FORMS = [pytest.param((-1, F32), id="float32"), pytest.param((0, BF16), id="float32 of bfloat16 pools"), pytest.param((16, BF16), id="mma"),
-         pytest.param((18, BF16), id="clusters of 2"), pytest.param((20, BF16), id="clusters of 4"), pytest.param((24, BF16), id="clusters of 8")]
+         pytest.param((1, BF16), id="tcgen05"), pytest.param((18, BF16), id="clusters of 2"), pytest.param((20, BF16), id="clusters of 4"), pytest.param((24, BF16), id="clusters of 8")]
 
 
 @pytest.fixture(params=FORMS)
