@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
 template <int D> static int launch_chunk_bf16(const ChArgs& a, cudaStream_t st) {
     using S = CbShape<D>;
     auto kern = chunk_bf16_kernel<D, false>;
-    const int C = S::blocks * aie_sm_count();
+    const int C = a.blocks;
     static unsigned long long done = 0;
     ch_prepare(kern, S::bytes, &done);
     const int rc = (int)launch_pdl(kern, dim3(C), dim3(S::threads), S::bytes, st, a, 1);
@@ -439,12 +439,12 @@ template <int D> static int launch_chunk_clusters(const ChArgs& a, int blocks, c
     return (int)cudaLaunchKernelEx(&cfg, kern, a, blocks);
 }
 
-// clusters 0: by the line, with a scratch of [2 * blocks * 32 * (d + 2)] floats and [2 * blocks] int4, two blocks an SM.  clusters 2 .. 8: blocks of
-// a cluster for every request and key head, no scratch.
+// clusters 0: by the line, as many blocks as the call says (the host: two an SM).  clusters 2 .. 8: blocks of a cluster for every request and
+// key head, no scratch.
 extern "C" int aie_attention_chunks_bf16(const ChCall* call, int clusters, cudaStream_t stream) {
     if (call->R <= 0 || call->T <= 0) return 0;
     ChArgs a;
-    const int rc = ch_args(call, 32, 64, 1, &a);
+    const int rc = ch_args(call, 32, 64, 1, !clusters, &a);
     if (rc) return rc;
     if (a.d != 64 && a.d != 128) return AIE_UNSUPPORTED;
     if (!clusters) return a.d == 64 ? launch_chunk_bf16<64>(a, stream) : launch_chunk_bf16<128>(a, stream);

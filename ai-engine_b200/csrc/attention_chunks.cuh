@@ -14,6 +14,7 @@
 // are taken in another order in another batch.
 #pragma once
 #include "common.cuh"
+#include "draft_args.h"
 
 // n / d for n < 2^31 by a multiplication (Granlund and Montgomery, 1994): (n + high half of n * mul) >> shift
 struct ChDiv {
@@ -27,28 +28,16 @@ static inline ChDiv ch_div(unsigned d) {
 }
 __device__ __forceinline__ int ch_over(int n, ChDiv d) { return (int)((__umulhi((unsigned)n, d.mul) + (unsigned)n) >> d.shift); }
 
-struct ChCall {                       // what a caller packs, in this order
-    const void* q;                    // [T, H, d], elements q_token / q_head apart
-    const void* k_pages;              // [num_pages, K, P, d]
-    const void* v_pages;
-    void* out;                        // [T, H, d]
-    const int *q_start, *q_len, *ctx_len, *table;
-    float* part_o;                    // [2 * C][M][D]
-    float* part_ml;                   // [2 * C][M][2]
-    int4* meta;                       // [C] of the item that block c began and did not finish: key head, first row, rows and 2^16 parts (0: none), first token
-    long long q_token, q_head;
-    int R, W, T, num_pages, P, H, K, G, d, window;
-    float scale2;                     // scale * log2 e: exponentials are powers of two
-    unsigned* err;
-};
 struct ChArgs : ChCall {
     ChDiv by_g, by_p;
 };
 
-// Checks a call and completes it; M, KT, weight: rows of an item, keys of a tile and its largest weight in the kernel that takes it.
-static inline int ch_args(const ChCall* call, int M, int KT, int weight, ChArgs* a) {
+// Checks a call and completes it; M, KT, weight: rows of an item, keys of a tile and its largest weight in the kernel that takes it; line: whether
+// blocks share it (what they leave has to have its place, and an item's parts are counted in 15 bits).
+static inline int ch_args(const ChCall* call, int M, int KT, int weight, bool line, ChArgs* a) {
     *static_cast<ChCall*>(a) = *call;
     if (a->W <= 0 || a->num_pages <= 0 || a->P <= 0 || a->K <= 0 || a->H <= 0 || a->H % a->K || a->G != a->H / a->K) return AIE_BAD_ARG;
+    if (line && (a->blocks <= 0 || a->blocks > 0x7fff || !a->part_o || !a->part_ml || !a->meta)) return AIE_BAD_ARG;
     // the line's length has to fit 31 bits: every request at least one row tile a key head, each over all the table's keys (where
     // requests name the same rows more than once, ch_begin finds what this does not)
     const double items = (double)a->T * a->H / M + (double)a->R * a->K, keys = (double)a->W * a->P / KT + 2;

@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
 template <typename T, int D> static int launch_chunk_f32(const ChArgs& a, cudaStream_t st) {
     using S = CfShape<D>;
     auto kern = chunk_f32_kernel<T, D>;
-    const int C = aie_sm_count();
+    const int C = a.blocks;
     static unsigned long long done = 0;
     ch_prepare(kern, S::bytes, &done);
     const int rc = (int)launch_pdl(kern, dim3(C), dim3(S::threads), S::bytes, st, a);
@@ -400,13 +400,12 @@ template <typename T, int D> static int launch_chunk_f32(const ChArgs& a, cudaSt
     return launch_chunk_join<T, S::M, D>(a, C, st);
 }
 
-// A block an SM.  The scratch is [2 * blocks * 32 * (D + 2)] floats and [2 * blocks] int4, D
-// the head size rounded up to 64, 128 or 256.
+// The scratch is for items of 32 rows and a head size D rounded up to 64, 128 or 256; the host gives it a block an SM.
 extern "C" int aie_attention_chunks_f32(const ChCall* call, int dtype, cudaStream_t stream) {
     if (call->R <= 0 || call->T <= 0) return 0;
     if (call->d <= 0 || call->d > 256 || call->d % 8) return AIE_UNSUPPORTED;
     ChArgs a;
-    const int rc = ch_args(call, 32, 32, 8, &a);
+    const int rc = ch_args(call, 32, 32, 8, true, &a);
     if (rc) return rc;
     const int w = a.d <= 64 ? 0 : a.d <= 128 ? 1 : 2;
     if (dtype == AIE_F32) return w == 0 ? launch_chunk_f32<float, 64>(a, stream) : w == 1 ? launch_chunk_f32<float, 128>(a, stream) : launch_chunk_f32<float, 256>(a, stream);

@@ -571,7 +571,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     }
 }
 
-template <int D> static int launch_chunk_tc(const ChArgs& a, int C, cudaStream_t st) {
+template <int D> static int launch_chunk_tc(const ChArgs& a, cudaStream_t st) {
+    const int C = a.blocks;
     using S = CtShape<D>;
     CUtensorMap mk, mv;
     const unsigned long long rows = (unsigned long long)a.num_pages * a.K * a.P;
@@ -587,15 +588,15 @@ template <int D> static int launch_chunk_tc(const ChArgs& a, int C, cudaStream_t
     return launch_chunk_join<bf16, S::M, D>(a, C, st);
 }
 
-// Scratch as for the other forms, with 256 rows an item and a block an SM.  Pages of 8 .. 128 keys that divide 128, or of a multiple of 128; up
+// Scratch for items of 256 rows; the host gives it a block an SM.  Pages of 8 .. 128 keys that divide 128, or of a multiple of 128; up
 // to 2^31 - 1 groups of 8 rows in a pool.
 extern "C" int aie_attention_chunks_tc(const ChCall* call, cudaStream_t stream) {
     if (call->R <= 0 || call->T <= 0) return 0;
     ChArgs a;
-    const int rc = ch_args(call, 128, CT_KT, 2, &a);
+    const int rc = ch_args(call, 128, CT_KT, 2, true, &a);
     if (rc) return rc;
     if (a.P % 8 || (CT_KT % a.P && a.P % CT_KT) || (long long)a.num_pages * a.K * a.P / 8 > 0x7ffffffe) return AIE_UNSUPPORTED;
-    if (a.d == 64) return launch_chunk_tc<64>(a, aie_sm_count(), stream);
-    if (a.d == 128) return launch_chunk_tc<128>(a, aie_sm_count(), stream);
+    if (a.d == 64) return launch_chunk_tc<64>(a, stream);
+    if (a.d == 128) return launch_chunk_tc<128>(a, stream);
     return AIE_UNSUPPORTED;
 }

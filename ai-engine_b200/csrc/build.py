@@ -157,7 +157,8 @@ def draft_module_path() -> str:
 
     src = os.path.join(CSRC, "host", "draft_ops.cpp")
     flags = CXX_FLAGS + [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
-    key = _hash([src], flags + [torch.__version__, sysconfig.get_config_var("SOABI") or sys.version])
+    deps = [src, os.path.join(CSRC, "draft_args.h")]
+    key = _hash(deps, flags + [torch.__version__, sysconfig.get_config_var("SOABI") or sys.version])
     target = os.path.join(build_dir(), f"_aie_draft_ops-{key}.so")
     if os.path.exists(target):
         return target
@@ -169,7 +170,7 @@ def draft_module_path() -> str:
     cxx = os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++")
     if not cxx:
         raise BuildError("no C++ compiler found (g++): the host side of the draft operators cannot be built")
-    return _build(target, [cxx], [src] + libs, [src], flags + places, "csrc/host/draft_ops.cpp")
+    return _build(target, [cxx], [src] + libs, deps, flags + places, "csrc/host/draft_ops.cpp")
 
 
 def load_host_module():

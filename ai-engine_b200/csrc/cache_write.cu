@@ -6,6 +6,7 @@
 // consecutive elements of one head (16 bytes of bfloat16), four of them under way, the loads of its rows asked for before the slots are
 // known.
 #include "common.cuh"
+#include "draft_args.h"
 
 #define CW_THREADS 256
 #define CW_UNITS 4      // units of a thread under way
@@ -94,15 +95,6 @@ static int launch_write_rows(bool wide, const void* k, const void* v, long long 
     return wide ? launch_write<I, C, 8>(k, v, kt, kh, vt, vh, kp, vp, slots, T, num_pages, P, K, d, err, st)
                 : launch_write<I, C, 1>(k, v, kt, kh, vt, vh, kp, vp, slots, T, num_pages, P, K, d, err, st);
 }
-
-struct CwArgs {                       // what a caller packs, in this order
-    const void *k, *v;                // [T, K, d], elements k_token / k_head (v_token / v_head) apart between tokens and heads
-    void *k_pages, *v_pages;
-    const int* slots;
-    unsigned* err;
-    long long k_token, k_head, v_token, v_head;
-    int row_dtype, cache_dtype, T, num_pages, P, K, d;      // num_pages * P and 2 * K * d fit 31 bits
-};
 
 extern "C" int aie_write_kv_slots(const CwArgs* args, cudaStream_t stream) {
     const CwArgs& a = *args;

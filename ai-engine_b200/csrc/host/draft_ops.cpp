@@ -17,6 +17,8 @@
 #include <initializer_list>
 #include <string>
 
+#include "../draft_args.h"
+
 namespace {
 
 PyObject* kernel_error = nullptr;       // exception types of kernels/loader.py
@@ -55,6 +57,8 @@ void ints(const char* what, const char* name, const at::Tensor& t, std::initiali
     if (t.scalar_type() != at::kInt || t.sizes() != at::IntArrayRef(shape) || !t.is_contiguous())
         refuse(what, std::string(name) + " must be a contiguous int32 tensor " + shape_text(at::IntArrayRef(shape)) + ", got " + type_text(t));
 }
+int* words(const at::Tensor& t) { return t.data_ptr<int>(); }
+unsigned* bits(const at::Tensor& t) { return reinterpret_cast<unsigned*>(t.data_ptr<int>()); }
 // The current device's stream, for operands that all live on that device.
 cudaStream_t stream_of(const char* what, std::initializer_list<const at::Tensor*> ts) {
     for (const at::Tensor* t : ts)
@@ -108,45 +112,12 @@ Pools pools(const char* what, const at::Tensor& k, const at::Tensor& v) {
     return p;
 }
 
-// ---- arguments of the launchers, as csrc/*.cu declare them ----
-struct StArgs {
-    const void *cached, *counts, *held_in, *tables_in, *free_pages, *free_count;
-    void* out;
-    void* err;
-    int R, W, F, P, num_pages, capacity;
-};
-struct CwArgs {
-    const void *k, *v;
-    void *k_pages, *v_pages;
-    const void* slots;
-    void* err;
-    long long k_token, k_head, v_token, v_head;
-    int row_dtype, cache_dtype, T, num_pages, P, K, d;
-};
-struct VdArgs {
-    const void *target, *q_start, *draft_tokens, *draft_len, *draft_probs, *accept_draws, *token_draws;
-    void *tokens, *emitted, *err;
-    long long target_row, draft_req, draft_place;
-    int T, V, R, N;
-};
-struct ChCall {
-    const void *q, *k_pages, *v_pages;
-    void* out;
-    const void *q_start, *q_len, *ctx_len, *table;
-    void *part_o, *part_ml, *meta;
-    long long q_token, q_head;
-    int R, W, T, num_pages, P, H, K, G, d, window;
-    float scale2;
-    void* err;
-};
-
 int (*step_tables_fn)(const StArgs*, cudaStream_t) = nullptr;
 int (*write_fn)(const CwArgs*, cudaStream_t) = nullptr;
 int (*verify_fn)(const VdArgs*, cudaStream_t) = nullptr;
 int (*chunks_f32_fn)(const ChCall*, int, cudaStream_t) = nullptr;
 int (*chunks_mma_fn)(const ChCall*, int, cudaStream_t) = nullptr;
 int (*chunks_tc_fn)(const ChCall*, cudaStream_t) = nullptr;
-int sm_count = 0;
 
 template <typename F> F* loaded(F*& fn, const char* name) {
     if (!fn) {
@@ -195,8 +166,8 @@ PyObject* step_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const cudaStream_t st = stream_of(w, {&cached, &counts, &held, &tables, &free_pages, &free_count, &err});
         // tables, held, free_count, q_start, q_len, positions, token_req, slots, one behind the other
         at::Tensor out = fresh({R * W + 3 * R + 1 + 3 * most}, at::kInt, tables);
-        const StArgs args = {cached.data_ptr(), counts.data_ptr(), held.data_ptr(), tables.data_ptr(), free_pages.data_ptr(),
-                             free_count.data_ptr(), out.data_ptr(), err.data_ptr(), (int)R, (int)W, (int)F, (int)P, (int)num_pages, (int)most};
+        const StArgs args = {words(cached), words(counts), words(held), words(tables), words(free_pages),
+                             words(free_count), words(out), bits(err), (int)R, (int)W, (int)F, (int)P, (int)num_pages, (int)most};
         launched(w, loaded(step_tables_fn, "aie_step_tables")(&args, st), 1);
         PyObject* t = PyTuple_New(8);
         if (!t) throw Refused();
@@ -227,7 +198,7 @@ PyObject* write_kv_slots(PyObject*, PyObject* const* a, Py_ssize_t n) {
         ints(w, "err", err, {1});
         const cudaStream_t st = stream_of(w, {&slots, &k, &v, &kp, &vp, &err});
         if (T) {
-            const CwArgs args = {k.data_ptr(), v.data_ptr(), kp.data_ptr(), vp.data_ptr(), slots.data_ptr(), err.data_ptr(),
+            const CwArgs args = {k.data_ptr(), v.data_ptr(), kp.data_ptr(), vp.data_ptr(), words(slots), bits(err),
                                  k.stride(0), k.stride(1), v.stride(0), v.stride(1), code, p.code, (int)T, (int)p.N, (int)p.P, (int)p.K, (int)p.d};
             launched(w, loaded(write_fn, "aie_write_kv_slots")(&args, st), 1);
         }
@@ -262,9 +233,9 @@ PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const cudaStream_t st = stream_of(w, {&start, &ids, lens, &err, &target, guess, &accept, &pick});
         at::Tensor tokens = fresh({R, N + 1}, at::kInt, ids), emitted = fresh({R}, at::kInt, ids);
         if (R) {
-            const VdArgs args = {target.data_ptr(), start.data_ptr(), ids.data_ptr(), lens ? lens->data_ptr() : nullptr,
-                                 guess ? guess->data_ptr() : nullptr, accept.data_ptr(), pick.data_ptr(), tokens.data_ptr(), emitted.data_ptr(),
-                                 err.data_ptr(), target.stride(0), guess ? guess->stride(0) : 0, guess ? guess->stride(1) : 0,
+            const VdArgs args = {target.data_ptr<float>(), words(start), words(ids), lens ? words(*lens) : nullptr,
+                                 guess ? guess->data_ptr<float>() : nullptr, accept.data_ptr<float>(), pick.data_ptr<float>(), words(tokens),
+                                 words(emitted), bits(err), target.stride(0), guess ? guess->stride(0) : 0, guess ? guess->stride(1) : 0,
                                  (int)T, (int)V, (int)R, (int)N};
             launched(w, loaded(verify_fn, "aie_verify_drafts")(&args, st), 1);
         }
@@ -284,7 +255,7 @@ enum { FLOAT32 = 0, MMA = 16, TCGEN05 = 1 };
 // window).  The least of the times that each would take, in us, fitted to 643 calls (1 to 64 requests of 1 to 200 tokens behind 40 to 20,000,
 // four head layouts; the choice takes 1.2 % more than the best form of each call on average, 40 % where it is worst): a fixed part, one
 // for every key tile of the busiest block, one for every part of an item that is joined.  Only these proportions count.
-int chunk_form(int code, const Pools& p, int64_t R, int64_t W, int64_t T, int64_t G, int64_t window) {
+int chunk_form(int code, const Pools& p, int64_t R, int64_t W, int64_t T, int64_t G, int64_t window, int64_t sm_count) {
     if (code != 1 || (p.d != 64 && p.d != 128)) return FLOAT32;
     auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     const int64_t items = R * p.K, rows = up(T * G, R), tile = p.d == 128 ? 64 : 128;
@@ -357,8 +328,8 @@ PyObject* paged_attention_chunks(PyObject*, PyObject* const* a, Py_ssize_t n) {
         at::Tensor out = given ? *given : fresh(q.sizes(), q.scalar_type(), q);
         if (T && R) {
             const int64_t G = H / p.K;
-            if (!sm_count) sm_count = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-            if (form < 0) form = chunk_form(p.code, p, R, W, T, G, window);
+            const int64_t sm_count = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+            if (form < 0) form = chunk_form(p.code, p, R, W, T, G, window, sm_count);
             const int64_t wide = form == FLOAT32 ? (p.d <= 64 ? 64 : p.d <= 128 ? 128 : 256) : p.d;
             const int64_t M = form == TCGEN05 ? 256 : 32;
             const int64_t blocks = form > MMA ? 0 : sm_count * (form == MMA ? 2 : 1), parts = 2 * blocks * M;
@@ -366,9 +337,9 @@ PyObject* paged_attention_chunks(PyObject*, PyObject* const* a, Py_ssize_t n) {
             at::Tensor scratch;
             if (blocks) scratch = fresh({parts * (wide + 2) + 4 * blocks}, at::kFloat, q);
             float* s = blocks ? scratch.data_ptr<float>() : nullptr;
-            const ChCall call = {q.data_ptr(), kp.data_ptr(), vp.data_ptr(), out.data_ptr(), start.data_ptr(), len.data_ptr(), ctx.data_ptr(),
-                                 table.data_ptr(), s, s + parts * wide, s + parts * (wide + 2), q.stride(0), q.stride(1), (int)R, (int)W, (int)T,
-                                 (int)p.N, (int)p.P, (int)H, (int)p.K, (int)G, (int)p.d, (int)window, (float)(scale * 1.4426950408889634), err.data_ptr()};
+            const ChCall call = {q.data_ptr(), kp.data_ptr(), vp.data_ptr(), out.data_ptr(), words(start), words(len), words(ctx),
+                                 words(table), s, s ? s + parts * wide : nullptr, s ? reinterpret_cast<int4*>(s + parts * (wide + 2)) : nullptr, q.stride(0), q.stride(1), (int)R, (int)W, (int)T,
+                                 (int)p.N, (int)p.P, (int)H, (int)p.K, (int)G, (int)p.d, (int)window, (float)(scale * 1.4426950408889634), bits(err), (int)blocks};
             launched(w, form == TCGEN05   ? loaded(chunks_tc_fn, "aie_attention_chunks_tc")(&call, st)
                         : form == FLOAT32 ? loaded(chunks_f32_fn, "aie_attention_chunks_f32")(&call, p.code, st)
                                           : loaded(chunks_mma_fn, "aie_attention_chunks_bf16")(&call, (int)form - MMA, st),

@@ -14,6 +14,7 @@
 // then the grid shares out the table, a warp taking pieces of 512 entries of a row (four 16-byte loads a lane under way), and the tokens,
 // which find their request by bisection.
 #include "common.cuh"
+#include "draft_args.h"
 
 #define ST_THREADS 512
 #define ST_MAX_REQUESTS 4096      // 16 bytes of shared memory each
@@ -177,13 +178,6 @@ step_tables_kernel(const int* cached, const int* counts, const int* held_in,
     }
     if (bad) atomicOr(err, bad);
 }
-
-struct StArgs {                       // what a caller packs, in this order
-    const int *cached, *counts, *held_in, *tables_in, *free_pages, *free_count;      // [R], [R], [R], [R, W], [F], [1]
-    int* out;                         // tables [R, W], held [R], free_left [1], q_start [R], q_len [R], then positions, token_req, slots [capacity]
-    unsigned* err;
-    int R, W, F, P, num_pages, capacity;      // num_pages * P fits 31 bits
-};
 
 extern "C" int aie_step_tables(const StArgs* args, cudaStream_t stream) {
     const StArgs& a = *args;

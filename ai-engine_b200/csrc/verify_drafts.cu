@@ -20,6 +20,7 @@
 #include <cooperative_groups.h>
 
 #include "common.cuh"
+#include "draft_args.h"
 
 namespace cg = cooperative_groups;
 typedef unsigned long long u64;
@@ -268,17 +269,6 @@ verify_drafts_kernel(const float* target, long long target_row, int T, int V, co
         }
     }
 }
-
-struct VdArgs {                       // what a caller packs, in this order
-    const float* target;              // rows of V floats, target_row apart
-    const int *q_start, *draft_tokens, *draft_len;      // [R], [R, N], [R] or null: N each
-    const float* draft_probs;         // row i of request r at r * draft_req + i * draft_place, or null
-    const float *accept_draws, *token_draws;            // [R, N], [R]
-    int *tokens, *emitted;            // [R, N + 1], [R]
-    unsigned* err;
-    long long target_row, draft_req, draft_place;
-    int T, V, R, N;
-};
 
 extern "C" int aie_verify_drafts(const VdArgs* args, cudaStream_t stream) {
     const VdArgs& a = *args;
