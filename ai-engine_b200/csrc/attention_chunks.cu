@@ -144,14 +144,14 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
         auto key_of = [&](int i) { return (kt0 + i) * KT + group * CK + gt / TPK; };
         auto page_of = [&](int i) {
             const int key = key_of(i);
-            return i < n && key < hi && key >= low_all ? bt[ch_over(key, a.by_p)] : -1;
+            return i < n && key < hi && key >= low_all ? bt[fast_over(key, a.by_p)] : -1;
         };
         int page = page_of(0), page_next = page_of(1);
         // queries of the item: they land with the first stage
         for (int i = tid; i < M * PC; i += THREADS) {
             const int row = i / PC, pc = i % PC;
             const bool there = row < tl.rows;
-            const int full = tl.row0 + (there ? row : 0), t = ch_over(full, a.by_g), g = full - t * a.G;
+            const int full = tl.row0 + (there ? row : 0), t = fast_over(full, a.by_g), g = full - t * a.G;
             cb_fetch(q_s + cb_at<D>(row, pc), reinterpret_cast<const bf16*>(a.q) + (s0 + t) * a.q_token + (long long)(w.kh * a.G + g) * a.q_head + pc * 8, there);
         }
         auto issue = [&](int i, int slot) {
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
                     bad |= AIE_DEV_PAGE_OOB;
                     there = false;
                 }
-                const size_t off = there ? (((size_t)page * a.K + w.kh) * a.P + (key - ch_over(key, a.by_p) * a.P)) * D + gt % TPK * 8 : 0;
+                const size_t off = there ? (((size_t)page * a.K + w.kh) * a.P + (key - fast_over(key, a.by_p) * a.P)) * D + gt % TPK * 8 : 0;
 #pragma unroll
                 for (int y = 0; y < PC / TPK; ++y) {
                     const unsigned to = st + cb_at<D>(gt / TPK, gt % TPK + y * TPK);
@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
 
         const bool live = mt * 16 < tl.rows;             // any row of this warp
         float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f}, o[D / 8][4];
-        const int pos0 = c0 + ch_over(tl.row0 + mt * 16 + r0, a.by_g), pos1 = c0 + ch_over(tl.row0 + mt * 16 + r0 + 8, a.by_g);
+        const int pos0 = c0 + fast_over(tl.row0 + mt * 16 + r0, a.by_g), pos1 = c0 + fast_over(tl.row0 + mt * 16 + r0 + 8, a.by_g);
 #pragma unroll
         for (int x = 0; x < D / 8; ++x)
 #pragma unroll
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
                 if (e == 0) *reinterpret_cast<float2*>(cb_smem + S::block_ml_off + row * 8) = ch_left(m, l);
             } else if (begins && ends) {
                 const float inv = ch_inverse(l);
-                const int full = w.tile.row0 + row, t = ch_over(full, a.by_g), h = w.kh * a.G + full - t * a.G;
+                const int full = w.tile.row0 + row, t = fast_over(full, a.by_g), h = w.kh * a.G + full - t * a.G;
                 store4<bf16>(reinterpret_cast<bf16*>(a.out) + ((size_t)(w.s0 + t) * a.H + h) * D + e,
                              make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
             } else {
@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(CbShape<D>::threads, CbShape<D>::blocks) chunk
                     m = top;
                 }
                 const float inv = ch_inverse(l);
-                const int full = w.tile.row0 + row, t = ch_over(full, a.by_g), h = w.kh * a.G + full - t * a.G;
+                const int full = w.tile.row0 + row, t = fast_over(full, a.by_g), h = w.kh * a.G + full - t * a.G;
                 store4<bf16>(reinterpret_cast<bf16*>(a.out) + ((size_t)(w.s0 + t) * a.H + h) * D + e,
                              make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
             }

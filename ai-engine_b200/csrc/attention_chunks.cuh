@@ -14,22 +14,11 @@
 // are taken in another order in another batch.
 #pragma once
 #include "common.cuh"
+#include "division.cuh"
 #include "draft_args.h"
 
-// n / d for n < 2^31 by a multiplication (Granlund and Montgomery, 1994): (n + high half of n * mul) >> shift
-struct ChDiv {
-    unsigned mul, shift;
-};
-static inline ChDiv ch_div(unsigned d) {
-    ChDiv v = {0u, 0u};
-    while ((1ull << v.shift) < d) ++v.shift;
-    v.mul = (unsigned)(((1ull << 32) * ((1ull << v.shift) - d)) / d + 1);
-    return v;
-}
-__device__ __forceinline__ int ch_over(int n, ChDiv d) { return (int)((__umulhi((unsigned)n, d.mul) + (unsigned)n) >> d.shift); }
-
 struct ChArgs : ChCall {
-    ChDiv by_g, by_p;
+    FastDiv by_g, by_p;
 };
 
 // Checks a call and completes it; M, KT, weight: rows of an item, keys of a tile and its largest weight in the kernel that takes it; line: whether
@@ -42,8 +31,8 @@ static inline int ch_args(const ChCall* call, int M, int KT, int weight, bool li
     // requests name the same rows more than once, ch_begin finds what this does not)
     const double items = (double)a->T * a->H / M + (double)a->R * a->K, keys = (double)a->W * a->P / KT + 2;
     if (items * keys * weight > 2147000000.0) return -3;
-    a->by_g = ch_div((unsigned)a->G);
-    a->by_p = ch_div((unsigned)a->P);
+    a->by_g = fast_div((unsigned)a->G);
+    a->by_p = fast_div((unsigned)a->P);
     return 0;
 }
 
@@ -62,8 +51,8 @@ template <typename Sh> __device__ __forceinline__ ChTile ch_tile(const ChArgs& a
     ChTile t;
     t.row0 = m * Sh::M;
     t.rows = min(Sh::M, q.n * a.G - t.row0);
-    t.i0 = ch_over(t.row0, a.by_g);
-    t.i1 = ch_over(t.row0 + t.rows - 1, a.by_g);
+    t.i0 = fast_over(t.row0, a.by_g);
+    t.i1 = fast_over(t.row0 + t.rows - 1, a.by_g);
     const int lo = a.window > 0 ? max(0, q.c + t.i0 - a.window + 1) : 0;
     t.first = lo / Sh::KT;
     t.tiles = (q.c + t.i1) / Sh::KT - t.first + 1;
@@ -287,7 +276,7 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const ChArgs a, int C) 
                 m = top;
             }
             const float inv = ch_inverse(l);
-            const int full = it.y + row, tok = ch_over(full, a.by_g), h = it.x * a.G + full - tok * a.G;
+            const int full = it.y + row, tok = fast_over(full, a.by_g), h = it.x * a.G + full - tok * a.G;
             store4<T>(reinterpret_cast<T*>(a.out) + ((size_t)(it.w + tok) * a.H + h) * a.d + e,
                       make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
         }

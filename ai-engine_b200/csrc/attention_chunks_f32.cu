@@ -109,14 +109,14 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
         const int my_key = group * 16 + (gt >> 3);
         auto page_of = [&](int i) {
             const int k_at = (kt0 + i) * KT + my_key;
-            return i < n && k_at < hi && k_at >= low_all ? bt[ch_over(k_at, a.by_p)] : -1;
+            return i < n && k_at < hi && k_at >= low_all ? bt[fast_over(k_at, a.by_p)] : -1;
         };
         int page = page_of(0), page_next = page_of(1);
         // queries of the item: they land with the first stage
         for (int i = tid; i < M * CH; i += THREADS) {
             const int row = i / CH, ch = i - row * CH, e = ch * 4;
             const bool there = row < rows && e < a.d;
-            const int full = row0 + (there ? row : 0), t = ch_over(full, a.by_g), g = full - t * a.G;
+            const int full = row0 + (there ? row : 0), t = fast_over(full, a.by_g), g = full - t * a.G;
             cf_fetch(q_s + row * S::KS + e, reinterpret_cast<const T*>(a.q) + (w.s0 + t) * a.q_token + (long long)(kh * a.G + g) * a.q_head + (there ? e : 0), there);
         }
         auto issue = [&](int i, int slot) {
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
                     bad |= AIE_DEV_PAGE_OOB;
                     there = false;
                 }
-                const size_t row_at = there ? (((size_t)page * a.K + kh) * a.P + (k_at - ch_over(k_at, a.by_p) * a.P)) * a.d : 0;
+                const size_t row_at = there ? (((size_t)page * a.K + kh) * a.P + (k_at - fast_over(k_at, a.by_p) * a.P)) * a.d : 0;
                 float* to = ring + slot * S::stage;
 #pragma unroll
                 for (int y = 0; y < CH / 8; ++y) {
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
             m_run[r] = -INFINITY;
             l_run[r] = 0.f;
             const int row = mt * 8 + rq * 4 + r;
-            lim[r] = c0 + ch_over(row0 + min(row, rows - 1), a.by_g);
+            lim[r] = c0 + fast_over(row0 + min(row, rows - 1), a.by_g);
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
                     product(some, kk);
 #pragma unroll
                     for (int row = 0; row < 8; ++row) {
-                        const int pos = place_in_line.req.c + ch_over(place_in_line.tile.row0 + mt * 8 + row, a.by_g);
+                        const int pos = place_in_line.req.c + fast_over(place_in_line.tile.row0 + mt * 8 + row, a.by_g);
                         if (!ch_sees(pos, k_at + kk, a.window)) continue;
 #pragma unroll
                         for (int y = 0; y < CL; ++y) {
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(CfShape<D>::threads, 1) chunk_f32_kernel(const
             }
             if (begins && ends) {
                 const float inv = ch_inverse(l);
-                const int full = w.tile.row0 + row, t = ch_over(full, a.by_g), h = w.kh * a.G + full - t * a.G;
+                const int full = w.tile.row0 + row, t = fast_over(full, a.by_g), h = w.kh * a.G + full - t * a.G;
                 if (e < a.d)
                     store4<T>(reinterpret_cast<T*>(a.out) + ((size_t)(w.s0 + t) * a.H + h) * a.d + e,
                               make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));

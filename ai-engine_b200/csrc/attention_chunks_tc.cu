@@ -64,7 +64,7 @@ __device__ __forceinline__ void ct_add_unfinite(const ChArgs& a, const ChWalk& w
             key = first_pos;
             continue;
         }
-        const int in = ch_over(key, a.by_p), page = ch_sees(pos, key, a.window) ? a.table[(size_t)w.r * a.W + in] : -1;
+        const int in = fast_over(key, a.by_p), page = ch_sees(pos, key, a.window) ? a.table[(size_t)w.r * a.W + in] : -1;
         if (page < 0 || page >= a.num_pages) continue;
         const uint4* row = reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.v_pages) +
                                                           (((size_t)page * a.K + w.kh) * a.P + (key - in * a.P)) * a.d + c0);
@@ -180,11 +180,11 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                     const int key = (kt0 + j) * CT_KT + lane * BP;
                     return j < n && lane < boxes && key < hi && key + BP > low;
                 };
-                auto page_of = [&](int j) { return wanted(j) ? bt[ch_over((kt0 + j) * CT_KT + lane * BP, a.by_p)] : -1; };
+                auto page_of = [&](int j) { return wanted(j) ? bt[fast_over((kt0 + j) * CT_KT + lane * BP, a.by_p)] : -1; };
                 auto group_of = [&](int j, int page) {
                     if (!wanted(j)) return end_group;
                     if (page >= 0 && page < a.num_pages) {
-                        const int key = (kt0 + j) * CT_KT + lane * BP, in = key - ch_over(key, a.by_p) * a.P;
+                        const int key = (kt0 + j) * CT_KT + lane * BP, in = key - fast_over(key, a.by_p) * a.P;
                         return (int)((((long long)page * a.K + w.kh) * a.P + in) >> 3);
                     }
                     bad |= AIE_DEV_PAGE_OOB;
@@ -360,7 +360,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                     for (int x4 = 0; x4 < 4; ++x4) {
                         const int row = x4 * 32 + lane, at = t * CT_M + row;
                         const bool there = at < w.tile.rows;
-                        const int fl = w.tile.row0 + (there ? at : 0), tok = ch_over(fl, a.by_g), g = fl - tok * a.G;
+                        const int fl = w.tile.row0 + (there ? at : 0), tok = fast_over(fl, a.by_g), g = fl - tok * a.G;
                         const bf16* src = reinterpret_cast<const bf16*>(a.q) + (w.s0 + tok) * a.q_token + (long long)(w.kh * a.G + g) * a.q_head;
                         // [halves of 64 columns][128 rows][128 bytes], 16-byte pieces permuted by row & 7
                         const unsigned d = tc_smem(q_s + (nq & 1) * TILE + row * 128);
@@ -391,8 +391,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             const bool pair = w.tile.rows > CT_M;
             const int at = pair ? t * CT_M + row : row;                // row of the item
             const bool live = at - lane < w.tile.rows;                 // any row of this warp
-            const int qpos = w.req.c + ch_over(w.tile.row0 + at, a.by_g);
-            const int p_min = w.req.c + ch_over(w.tile.row0 + (pair ? t * CT_M : 0), a.by_g);
+            const int qpos = w.req.c + fast_over(w.tile.row0 + at, a.by_g);
+            const int p_min = w.req.c + fast_over(w.tile.row0 + (pair ? t * CT_M : 0), a.by_g);
             const int low = a.window > 0 ? qpos - a.window + 1 : 0, low_last = a.window > 0 ? w.req.c + w.tile.i1 - a.window + 1 : 0;
             float m_run = -INFINITY, l_run = 0.f;
             bool first = true;
@@ -488,7 +488,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             }
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             const bool begins = w.k == 0, ends = w.k + n == w.tile.tiles, whole = begins && ends, there = ok && at < w.tile.rows;
-            const int fl = w.tile.row0 + at, tok = ch_over(fl, a.by_g), h = w.kh * a.G + fl - tok * a.G;
+            const int fl = w.tile.row0 + at, tok = fast_over(fl, a.by_g), h = w.kh * a.G + fl - tok * a.G;
             const size_t place = ((size_t)2 * c + (begins ? 1 : 0)) * M + at;
             bf16* dst = reinterpret_cast<bf16*>(a.out) + ((size_t)(w.s0 + tok) * a.H + h) * D;
             float f0 = 1.f, f1 = 0.f;                                  // of this stream's outputs, of the other's

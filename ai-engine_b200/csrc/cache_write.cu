@@ -6,22 +6,11 @@
 // consecutive elements of one head (16 bytes of bfloat16), four of them under way, the loads of its rows asked for before the slots are
 // known.
 #include "common.cuh"
+#include "division.cuh"
 #include "draft_args.h"
 
 #define CW_THREADS 256
 #define CW_UNITS 4      // units of a thread under way
-
-// n / d for n < 2^31 by a multiplication (Granlund and Montgomery, 1994)
-struct CwDiv {
-    unsigned mul, shift;
-};
-static inline CwDiv cw_div(unsigned d) {
-    CwDiv v = {0u, 0u};
-    while ((1ull << v.shift) < d) ++v.shift;
-    v.mul = (unsigned)(((1ull << 32) * ((1ull << v.shift) - d)) / d + 1);
-    return v;
-}
-__device__ __forceinline__ unsigned cw_over(unsigned n, CwDiv d) { return (__umulhi(n, d.mul) + n) >> d.shift; }
 
 template <typename T, int V> struct CwVec { T e[V]; };
 
@@ -39,7 +28,7 @@ template <typename I, typename C, int V>
 __global__ void __launch_bounds__(CW_THREADS)
 write_kv_slots_kernel(const I* k, const I* v, long long k_token, long long k_head, long long v_token,
                       long long v_head, C* k_pages, C* v_pages, const int* slots,
-                      unsigned total, unsigned per_plane, CwDiv by_token, CwDiv by_head, CwDiv by_p, int P, int K, int d, int n_slots,
+                      unsigned total, unsigned per_plane, FastDiv by_token, FastDiv by_head, FastDiv by_p, int P, int K, int d, int n_slots,
                       unsigned* err) {
     pdl_launch_dependents();
     pdl_wait();
@@ -51,7 +40,7 @@ write_kv_slots_kernel(const I* k, const I* v, long long k_token, long long k_hea
         const unsigned i = first + u * CW_THREADS;
         slot[u] = -1;
         if (i < total) {
-            const unsigned t = cw_over(i, by_token), unit = i - t * (2 * per_plane), h = cw_over(unit, by_head);
+            const unsigned t = fast_over(i, by_token), unit = i - t * (2 * per_plane), h = fast_over(unit, by_head);
             head[u] = (int)h;
             at[u] = (int)(unit - h * per_head) * V;
             const bool is_v = (int)h >= K;
@@ -64,7 +53,7 @@ write_kv_slots_kernel(const I* k, const I* v, long long k_token, long long k_hea
         if (slot[u] < 0) continue;
         if (slot[u] >= n_slots) { atomicOr(err, AIE_DEV_PAGE_OOB); continue; }
         const bool is_v = head[u] >= K;
-        const int page = (int)cw_over((unsigned)slot[u], by_p);
+        const int page = (int)fast_over((unsigned)slot[u], by_p);
         C* to = (is_v ? v_pages : k_pages) + (((size_t)page * K + (is_v ? head[u] - K : head[u])) * P + (slot[u] - page * P)) * d + at[u];
         if constexpr (V == 8) {
             alignas(16) CwVec<C, V> y;
@@ -85,8 +74,8 @@ static int launch_write(const void* k, const void* v, long long kt, long long kh
     if (total > 0x7ffffc00) return -3;
     const unsigned blocks = (unsigned)((total + CW_THREADS * CW_UNITS - 1) / (CW_THREADS * CW_UNITS)), per_plane = (unsigned)(K * (d / V));
     return (int)launch_pdl(write_kv_slots_kernel<I, C, V>, dim3(blocks), dim3(CW_THREADS), 0, st, (const I*)k, (const I*)v, kt, kh, vt, vh,
-                           (C*)kp, (C*)vp, slots, (unsigned)total, per_plane, cw_div(2 * per_plane), cw_div((unsigned)(d / V)),
-                           cw_div((unsigned)P), P, K, d, num_pages * P, err);
+                           (C*)kp, (C*)vp, slots, (unsigned)total, per_plane, fast_div(2 * per_plane), fast_div((unsigned)(d / V)),
+                           fast_div((unsigned)P), P, K, d, num_pages * P, err);
 }
 
 template <typename I, typename C>
