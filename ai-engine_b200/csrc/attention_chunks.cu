@@ -7,14 +7,15 @@
 // the item and reads the group's keys and values.  Groups meet only at an item's end, where their outputs are added up in shared memory.
 // What bounds it: reading keys and values once, and 10 us of a small call's chain of waits (lengths, pages, rows, outputs that meet).  One
 // warp for 32 rows (255 registers, eight warps an SM) waited for its own instructions, 5.3 cycles each, at half of the memory's rate
-// (56 requests of heads of 64: 84 us, now 71); items of 16 rows or of 64 were at most a twentieth better anywhere.
+// (56 requests of heads of 64: 84 us, now 73); items of 16 rows or of 64 were at most a twentieth better anywhere.
 // Scores, maxima and sums are float32, a row's reference maximum moves by more than 8 (log2 units) or not at all; probabilities are rounded
-// to bfloat16 for the product with the values, as the values are, which the result's own rounding hides (2^-9 each on average).
+// to bfloat16 for the product with the values, as the values are (a product in two terms would be half as many instructions again); sums take them unrounded.
+// An error of 0.0021 to 0.0023 of the result's norm, of which the result's own rounding is 0.0017.
 //
 // Two ways to share the work out.  The line of attention_chunks.cuh balances any lengths, at the price of a second kernel.  For few requests
 // with few keys that is a third of the call, so there a cluster of S blocks takes a (request, key head), each block a part of every item's
 // key tiles, and the parts are joined in the cluster's shared memory (one request of 5 tokens behind 1,000, 32 heads of 128: 10.3 us
-// by the line, 7.3 by clusters of eight; eight requests behind 500 to 2,000: 20.0, and 18.5 by clusters of four).
+// by the line, 7.3 by clusters of eight; eight requests behind 500 to 2,000: 20.5, and 18.7 by clusters of four).
 #include <cooperative_groups.h>
 
 #include "attention_chunks.cuh"

@@ -10,7 +10,7 @@
 // rows a lane: 512 cycles of reads a warp's step against 128 of multiply-adds, 47 us for the case below.)
 // Outputs: a lane has D / 32 columns of the warp's rows, two rows an instruction (fma.rn.f32x2).
 // What bounds it: these reads, twice what the packed multiply-adds beside them take: full items reach 30 TFLOP/s of 74.  3 to 7 tokens x 4
-// heads behind 500 to 3,000 keys, 8 requests: 37 us, 14.7 TFLOP/s (their multiply-adds and their bytes take 9 each): items of 12 to 28 of 32 rows.
+// heads behind 500 to 3,000 keys, 8 requests: 37.2 us, 14.5 TFLOP/s (their multiply-adds and their bytes take 9 each): items of 12 to 28 of 32 rows.
 #include "attention_chunks.cuh"
 
 typedef unsigned long long u64;

@@ -20,9 +20,9 @@
 //                    and heads may lie any distance apart), ahead of the item that uses them where a place is free.
 // Tensor memory: scores of stream t at columns 128 t (P over the first 64), outputs at 256 + 128 t.
 // What bounds it: long chunks the exponentials (16 a cycle and SM: 2,048 cycles for two rows' tiles of 128 keys, against 2,048 of
-// products; four requests of 300 to 500 tokens behind 6,000 to 9,000, 32 heads of 128: 223 to 231 us, 905 to 937 TFLOP/s, tensor pipe
+// products; four requests of 300 to 500 tokens behind 6,000 to 9,000, 32 heads of 128: 226 to 229 us, 913 to 925 TFLOP/s, tensor pipe
 // 0.51 busy; 273 us back to back under the power limit), few rows behind many keys the reading of those (four requests of 6 to 9 tokens
-// behind 30,000: 90 us, 5.7 TB/s).  A call of any size takes 12 to 16 us more than its tiles: the start, the queries, the first tiles, the join.
+// behind 30,000: 92.5 us, 5.6 TB/s).  A call of any size takes 12 to 16 us more than its tiles: the start, the queries, the first tiles, the join.
 // Probabilities are rounded to bfloat16 for the product with the values, as the values are; sums take them unrounded.
 #include "attention_chunks.cuh"
 #include "tc_rows.cuh"

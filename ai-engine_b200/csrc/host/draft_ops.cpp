@@ -253,8 +253,10 @@ enum { FLOAT32 = 0, MMA = 16, TCGEN05 = 1 };
 
 // Which of them takes a call, by what the host knows: tokens, requests, and how many keys a request can have (the table's width; a
 // window).  The least of the times that each would take, in us, fitted to 643 calls (1 to 64 requests of 1 to 200 tokens behind 40 to 20,000,
-// four head layouts; the choice takes 1.2 % more than the best form of each call on average, 40 % where it is worst): a fixed part, one
-// for every key tile of the busiest block, one for every part of an item that is joined.  Only these proportions count.
+// four head layouts, tables as wide as the longest request: there the choice takes 1.2 % more than the best form of each call on average, 40 % where
+// it is worst): a fixed part, one for every key tile of the busiest block, one for every part of an item that is joined.  Only these proportions
+// count.  A wider table is taken for longer requests: with 512 pages of 16 one request of five tokens behind 1,000 goes by the line (10.1 us) and
+// not by clusters (7.2), with 256 eight requests behind 500 to 2,000 do (20.4 and 18.7).
 int chunk_form(int code, const Pools& p, int64_t R, int64_t W, int64_t T, int64_t G, int64_t window, int64_t sm_count) {
     if (code != 1 || (p.d != 64 && p.d != 128)) return FLOAT32;
     auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };

@@ -6,12 +6,14 @@
 // Behind the k kept ones one token is drawn, by v in [0, 1), from the weights
 //     w = max(p_k - q_k, 0)   where draft k was refused,        w = p_n   where all were kept:
 // the first token whose cumulative weight is above floor(v W), W the sum of all.  If every w is 0 (p_k nowhere above q_k: possible only
-// by the rounding of their sums) the weights are p_k.  Which tokens come out then follows the target's distribution exactly.
+// by the rounding of their sums) the weights are p_k.  Which tokens come out then follows the target's distribution as far as the
+// draws tell shares apart: u and v are float32, as a rule multiples of 2^-24, so a draft is kept, and a token drawn, with a probability that is off
+// by up to 2^-24, and a token whose interval lies between two such multiples is never drawn; p_k - q_k is rounded to float32.
 // Weights are integers, w clipped to 1 in units of 2^-48 rounded to nearest: 2^-49 is off at most, a float below 2^-25 of
-// the largest mass, and sums are exact, the same whatever their order.
+// the largest mass, and sums are exact, the same whatever their order.  A drafted token outside the vocabulary is refused and takes nothing off p.
 //
-// What bounds it: one row of p and one of q a request (64 requests of 128,256 tokens: 18.6 us, 3.1 TB/s), and the chain of waits around
-// them: lengths, the drafts' probabilities, the blocks' sums, a segment again (one request: 7.5 us).  A cluster of eight blocks shares a
+// What bounds it: one row of p and one of q a request (64 requests of 128,256 tokens: 14.3 us, 4.0 TB/s), and the chain of waits around
+// them: lengths, the drafts' probabilities, the blocks' sums, a segment again (one request: 7.3 us).  A cluster of eight blocks shares a
 // request's row: every warp adds up segments of 512 tokens (eight 16-byte loads a lane under way), the segments' sums stay in shared
 // memory, the blocks' sums meet in everyone's shared memory, and the block that holds the wanted one looks for its segment and reads that
 // once more.  Eight blocks because a row of 128,256 floats twice is 128 KB for each, about 2 us of what an SM can load.  At 64 registers a

@@ -772,10 +772,12 @@ def paged_attention_chunks(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     the pages too).  softmax(q.k * scale over keys j <= position, and j > position - window where window > 0) . v per token and head,
     query head h with key head h // (H / K).  q [T, H, d] in the pools' dtype, any distance between tokens and heads (multiples of 16
     bytes); block_table [R, W]; out [T, H, d] contiguous: rows that no request names are left as they are (in an `out` made
-    here they hold nothing), rows that several name hold one's; it may be q itself, else it overlaps no operand.  Few tokens behind many keys are what it is made for: the keys are
-    shared out over the whole machine.  Any head size up to 256 that is a multiple of 8.  Lengths that do not fit q or the table bring nothing and set the error word, so
-    does a page outside the pool, whose keys count as zeros.  How a token's sums are ordered depends on the whole batch's lengths; keys
-    and values that are not finite reach the tokens that see them and no others."""
+    here they hold nothing), rows that several name hold one's; it may be q itself where no two requests name a row, else it
+    overlaps no operand.  Few tokens behind many keys are what it is made for: the keys are shared out over the whole machine.  Any
+    head size up to 256 that is a multiple of 8.  Lengths that do not fit q or the table bring nothing and set the error word; so
+    does a page outside the pool, whose keys count as zeros.  How a token's sums are ordered depends on the whole batch's lengths.
+    Keys and values that are not finite reach the tokens that see them and no others.  The form of the kernel is chosen by the
+    sizes of q and of the table alone, so a table much wider than the requests are long can cost up to 1.4 times the time."""
     return draft_call("paged_attention_chunks", 0.0, q, k_pages, v_pages, q_start, q_len, ctx_len, block_table, scale, window,
                       err, out, CHUNK_FORM)
 

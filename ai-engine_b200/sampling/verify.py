@@ -11,7 +11,8 @@ from ..kernels.ops import _nb, draft_call
 def verify_drafts(target_probs: torch.Tensor, q_start: torch.Tensor, draft_tokens: torch.Tensor, draft_len: Optional[torch.Tensor],
                   draft_probs: Optional[torch.Tensor], accept_draws: torch.Tensor, token_draws: torch.Tensor,
                   err: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Which drafted tokens are kept, and the token behind them, distributed as the target alone would draw them.
+    """Which drafted tokens are kept, and the token behind them, distributed as the target alone would draw them (to the resolution of the
+    draws: 2^-24 where they are multiples of that, as torch.rand makes them).
 
     Request r drafted n = draft_len[r] of the N tokens draft_tokens[r] (None: all N; negative: the request is idle and gets
     nothing) from the distributions draft_probs[r, :n] (None: drafts without probabilities, each taken as certain).  Rows
