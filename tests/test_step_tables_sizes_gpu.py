@@ -1,5 +1,5 @@
-"""Batches whose rows take about as much shared memory as a kernel gets without asking for more (3,072 requests of 16 bytes, and what the
-kernel has besides), in a process of their own: what a kernel was once told about its shared memory stays."""
+"""Batches whose rows (16 bytes a request) take about as much shared memory as a kernel gets without asking for more, 48 KB with what the
+kernel has besides, in a process of their own: what a kernel was once told about its shared memory stays."""
 import os
 import subprocess
 import sys
@@ -15,7 +15,7 @@ sys.path[:0] = [{here!r}, {root!r}]
 from draft_helpers import plain_tables
 from test_step_tables_gpu import batch, call
 for W in {widths}:
-    for R in (3055, 3056, 3064, 3072, 3073, 4096):
+    for R in (3055, 3056, 3064, 3071, 3100, 4096):
         cached, counts, held, table, free, n_pages = batch(R, 16, W, R + W)
         want = plain_tables(cached, counts, held, table, free, len(free) // 20, 16, sum(counts))
         got, word = call(cached, counts, held, table, free, len(free) // 20, 16, n_pages, sum(counts))
